@@ -55,7 +55,8 @@ typedef enum qxc_model {
   QXC_MODEL_QWEN3 = 1    /* 32 q heads, 4 kv heads, head_dim 128, scale 1/sqrt(128), QK-RMSNorm, RoPE theta 1e6 */
 } qxc_model;
 
-typedef enum qxc_dtype { QXC_F32 = 0, QXC_BF16 = 1, QXC_F16 = 2 } qxc_dtype;
+/* QXC_Q4 is a storage type of KV arenas only (see "4-bit arenas"). */
+typedef enum qxc_dtype { QXC_F32 = 0, QXC_BF16 = 1, QXC_F16 = 2, QXC_Q4 = 3 } qxc_dtype;
 
 /* Decode flags. */
 #define QXC_DECODE_NO_ADVANCE 0x1 /* do not advance the cursor (caller advances after the last layer) */
@@ -130,6 +131,78 @@ qxc_status qxc_kv_read(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, in
                        void* host_keys, void* host_values);
 qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, int32_t count,
                         const void* host_keys, const void* host_values);
+
+/* ---- 4-bit arenas ----------------------------------------------------------- */
+/* key_dtype = value_dtype = QXC_Q4 (new; the reference keeps caches in f32 or
+ * f16): keys and values are quantised as they are written, per kv head and
+ * group of 32 dims, by the value rule of the Q4 weights below: an FP16 scale
+ * s = fp16(max |x| / 7) and codes c = clamp(rint(x / s), -7, 7) + 7 that stand
+ * for (c - 7) * s (all zero when s rounds to zero). Keys are rotated first and
+ * rounded to f32. A row, one position's keys or values of all kv heads, is 288
+ * bytes for either model: the kv heads' codes, head_dim / 2 bytes each, then
+ * the scales [kv_heads][head_dim / 32]. With NG = head_dim / 32, dim 32 j + r
+ * of a head is
+ *   keys    nibble r % 8 (low first) of its 32-bit word (r / 8) * NG + j
+ *   values  nibble r / 8 (low first) of its 16-bit half (r % 8) * NG + j
+ * Contiguous or paged, any input type of either model; first_position must be
+ * 0. Cursors, paging, views (bytes), qxc_kv_read / write (raw rows) work as on
+ * any arena, qxc_decode reads and writes it, qxc_attention_layer and
+ * qxc_attention_stack run on it through qxc_decode. The verify, partials,
+ * exchange, prefill and hash calls return QXC_ERR_UNSUPPORTED. A value beyond
+ * 7 * 65504, an infinity or a NaN in a new row is reported by qxc_sync
+ * (QXC_ERR_NONFINITE); what that row then holds is unspecified. */
+
+/* Write the rows of counts[i] new tokens of each of seq_count sequences
+ * (packed one after another) into layers [layer_begin, layer_begin +
+ * layer_count), and rotate their queries, in one pass: per head RMSNorm (Qwen:
+ * sum of squares in f64) and rotation of q and k at positions positions[i],
+ * positions[i] + 1, ..., keys and values quantised into the cache. positions[i]
+ * must equal the sequence's length, positions[i] + counts[i] <= capacity, else
+ * QXC_ERR_POSITION; counts may be 0, a sequence may appear once. Lengths
+ * advance by counts unless QXC_DECODE_NO_ADVANCE. Device pointers of any
+ * element alignment (16-byte aligned ones are read and written faster);
+ * asynchronous. q and q_rot may both be NULL (keys and values only), k_rot may
+ * be NULL. */
+typedef struct qxc_append_args {
+  int32_t layer_begin;
+  int32_t layer_count;
+  int32_t seq_count;
+  const int32_t* seq_ids;   /* host [seq_count]; NULL = 0..seq_count-1 */
+  const int32_t* positions; /* host [seq_count]: first position of the new tokens */
+  const int32_t* counts;    /* host [seq_count]: new tokens */
+  const void* q;            /* in_dtype [tokens][layer_count][Hq*D] */
+  const void* k;            /* in_dtype [tokens][layer_count][Hkv*D] */
+  const void* v;            /* in_dtype [tokens][layer_count][Hkv*D] */
+  void* q_rot;              /* rot_dtype [tokens][layer_count][Hq*D], dense */
+  void* k_rot;              /* rot_dtype [tokens][layer_count][Hkv*D], dense: rotated, not quantised */
+  int64_t q_stride;         /* elements from one token to the next; 0 = dense */
+  int64_t k_stride;
+  int64_t v_stride;
+  const float* q_norm;      /* Qwen: device [128] RMSNorm weight for q, NULL = 1.0 */
+  const float* k_norm;      /* Qwen: device [128] RMSNorm weight for k, NULL = 1.0 */
+  int32_t in_dtype;
+  int32_t rot_dtype;
+  int32_t flags;            /* QXC_DECODE_NO_ADVANCE */
+} qxc_append_args;
+qxc_status qxc_kv_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* args);
+
+/* Rows [begins[i], begins[i] + counts[i]) of each of seq_count sequences
+ * (packed one after another) of a 4-bit arena as plain values, rounded once to
+ * out_dtype. The rows may lie past the sequence's length but not past its
+ * capacity (QXC_ERR_POSITION) or its mapped pages. A sequence may appear more
+ * than once. Either output may be NULL. Device pointers, asynchronous. */
+typedef struct qxc_read_rows_args {
+  int32_t layer_begin;
+  int32_t layer_count;
+  int32_t seq_count;
+  const int32_t* seq_ids; /* host [seq_count]; NULL = 0..seq_count-1 */
+  const int32_t* begins;  /* host [seq_count] */
+  const int32_t* counts;  /* host [seq_count] */
+  void* key_out;          /* out_dtype [tokens][layer_count][Hkv*D] */
+  void* value_out;        /* out_dtype [tokens][layer_count][Hkv*D] */
+  int32_t out_dtype;
+} qxc_read_rows_args;
+qxc_status qxc_kv_read_rows(qxc_ctx* ctx, qxc_kv* kv, const qxc_read_rows_args* args);
 
 /* ---- paged arenas -------------------------------------------------------- */
 /* A paged arena replaces the fixed [capacity] cache per (sequence, layer) for
@@ -409,6 +482,58 @@ typedef struct qxc_prefill_args {
   int32_t flags;
 } qxc_prefill_args;
 qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* args);
+
+/* ---- packed prompts -------------------------------------------------------- */
+/* Causal grouped-query attention of seq_count prompts packed one after
+ * another: token i of a prompt attends tokens 0..i of the same prompt, softmax
+ * scale and head layout of `model`. q and k are already rotated. bf16 or f16
+ * in and out, f32 scores, softmax and accumulation (the weights of one key
+ * tile are rounded to the input type for their product with the values).
+ * lengths may be 0; at most 2^24 tokens. Each tensor is [tokens][heads *
+ * head_dim], 16-byte aligned, with token strides in elements that are
+ * multiples of 8 (0 = dense): q, k and v may be parts of one joint projection.
+ * Rows of `out` past the last prompt are not written. A row that attends a
+ * NaN or an infinity is not finite (QXC_ERR_NONFINITE at qxc_sync); rows that
+ * do not attend it are unaffected. Device pointers, asynchronous. */
+typedef struct qxc_packed_args {
+  int32_t model;
+  int32_t seq_count;
+  const int32_t* lengths; /* host [seq_count] */
+  const void* q;          /* dtype [tokens][Hq*D] */
+  const void* k;          /* dtype [tokens][Hkv*D] */
+  const void* v;          /* dtype [tokens][Hkv*D] */
+  void* out;              /* dtype [tokens][Hq*D], dense */
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  int32_t dtype;          /* BF16 or F16 */
+} qxc_packed_args;
+qxc_status qxc_attend_packed(qxc_ctx* ctx, const qxc_packed_args* args);
+
+/* Prefill of seq_count prompts into EMPTY sequences of one layer of a 4-bit
+ * arena: qxc_kv_append at positions 0.. and qxc_attend_packed over the rotated
+ * queries, the rotated keys before quantisation (rounded to dtype) and the
+ * values as given. Arguments, position and alignment rules as theirs (q and k
+ * any alignment). Lengths advance unless QXC_DECODE_NO_ADVANCE (more layers to
+ * come). Device pointers, asynchronous. */
+typedef struct qxc_prefill_packed_args {
+  int32_t layer;
+  int32_t seq_count;
+  const int32_t* seq_ids; /* host [seq_count]; NULL = 0..seq_count-1 */
+  const int32_t* lengths; /* host [seq_count] */
+  const void* q;          /* dtype [tokens][Hq*D] */
+  const void* k;          /* dtype [tokens][Hkv*D] */
+  const void* v;          /* dtype [tokens][Hkv*D] */
+  void* out;              /* dtype [tokens][Hq*D], dense */
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  const float* q_norm;
+  const float* k_norm;
+  int32_t dtype;          /* BF16 or F16 */
+  int32_t flags;
+} qxc_prefill_packed_args;
+qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed_args* args);
 
 /* ---- KV-length split across GPUs --------------------------------------- */
 /* Partial attention of one (sequence, layer) over this arena's slots

@@ -16,7 +16,7 @@ OK, ERR_INVALID_ARG, ERR_POSITION, ERR_NONFINITE, ERR_CUDA, ERR_NCCL, ERR_TIMEOU
     ERR_OUT_OF_MEMORY = range(9)
 # qxc_model / qxc_dtype
 MODEL_GRANITE, MODEL_QWEN3 = 0, 1
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, Q4 = 0, 1, 2, 3
 DECODE_NO_ADVANCE, DECODE_NATIVE_EXP, DECODE_PINNED_EXP = 0x1, 0x2, 0x4
 VERIFY_PER_TOKEN = 0x8
 HASH_AUTO, HASH_PER_CHUNK, HASH_PER_SLOT = 0, 1, 2
@@ -104,6 +104,39 @@ class StaticDecodeArgs(C.Structure):
                 ("flags", C.c_int32), ("split", C.c_int32), ("device_error", C.c_void_p)]
 
 
+class AppendArgs(C.Structure):
+    """qxc_append_args (rows of new tokens into a 4-bit arena)."""
+    _fields_ = [("layer_begin", C.c_int32), ("layer_count", C.c_int32), ("seq_count", C.c_int32),
+                ("seq_ids", C.POINTER(C.c_int32)), ("positions", C.POINTER(C.c_int32)),
+                ("counts", C.POINTER(C.c_int32)), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_rot", C.c_void_p), ("k_rot", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("in_dtype", C.c_int32),
+                ("rot_dtype", C.c_int32), ("flags", C.c_int32)]
+
+
+class ReadRowsArgs(C.Structure):
+    """qxc_read_rows_args (rows of a 4-bit arena as values)."""
+    _fields_ = [("layer_begin", C.c_int32), ("layer_count", C.c_int32), ("seq_count", C.c_int32),
+                ("seq_ids", C.POINTER(C.c_int32)), ("begins", C.POINTER(C.c_int32)),
+                ("counts", C.POINTER(C.c_int32)), ("key_out", C.c_void_p), ("value_out", C.c_void_p),
+                ("out_dtype", C.c_int32)]
+
+
+class PackedArgs(C.Structure):
+    """qxc_packed_args (causal attention of packed prompts)."""
+    _fields_ = [("model", C.c_int32), ("seq_count", C.c_int32), ("lengths", C.POINTER(C.c_int32)),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("dtype", C.c_int32)]
+
+
+class PrefillPackedArgs(C.Structure):
+    """qxc_prefill_packed_args (packed prompts into a 4-bit arena)."""
+    _fields_ = [("layer", C.c_int32), ("seq_count", C.c_int32), ("seq_ids", C.POINTER(C.c_int32)),
+                ("lengths", C.POINTER(C.c_int32)), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("out", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("dtype", C.c_int32), ("flags", C.c_int32)]
+
+
 _lib = None
 
 
@@ -148,6 +181,10 @@ def load() -> C.CDLL:
         "qxc_kv_value_buffer": (C.c_int, [vp, i32, i32, pp, C.POINTER(C.c_size_t)]),
         "qxc_kv_read": (C.c_int, [vp, i32, i32, i32, i32, vp, vp]),
         "qxc_kv_write": (C.c_int, [vp, i32, i32, i32, i32, vp, vp]),
+        "qxc_kv_append": (C.c_int, [vp, vp, C.POINTER(AppendArgs)]),
+        "qxc_kv_read_rows": (C.c_int, [vp, vp, C.POINTER(ReadRowsArgs)]),
+        "qxc_attend_packed": (C.c_int, [vp, C.POINTER(PackedArgs)]),
+        "qxc_prefill_packed": (C.c_int, [vp, vp, C.POINTER(PrefillPackedArgs)]),
         "qxc_decode": (C.c_int, [vp, vp, C.POINTER(DecodeArgs)]),
         "qxc_decode_host": (C.c_int, [vp, vp, C.POINTER(DecodeArgs)]),
         "qxc_granite_attention_decode": (C.c_int, [vp, vp, vp, vp, vp, i32, vp]),

@@ -11,11 +11,11 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqxcuda.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
-SOURCES = ["qxcuda.cu", "noalloc.cu"]
+SOURCES = ["qxcuda.cu", "noalloc.cu", "q4_cache.cu", "q4_decode.cu", "packed.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads", "0",
     "-I", os.path.join(ROOT, "include"),
 ]
 

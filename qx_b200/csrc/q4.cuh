@@ -1,0 +1,200 @@
+// q4.cuh — the 4-bit cache row and the arithmetic of a new token's heads.
+//
+// A row (one position, all kv heads) is 288 bytes for both models:
+//   [0, 256)    codes, kv head after kv head, D / 2 bytes each
+//   [256, 288)  fp16 scales [kv head][D / 32]
+// A code c in 0..14 of a group of 32 dims stands for (c - 7) * scale, the
+// value rule of the framework's Q4 weights. Within a head the codes are laid
+// out for the lane that reads them in the attention kernel (group j of
+// D / 32, dim 32 j + r):
+//   keys    32-bit word t * (D / 32) + j holds dims r = 8 t .. 8 t + 7, low
+//           nibble first: lane t of a quad reads its words of all groups at
+//           once
+//   values  16-bit half g * (D / 32) + j holds dims r = 8 i + g in nibble i
+//           (i = 0..3): lane group g reads its halves of all groups at once
+//
+// A head is D / 8 neighbouring lanes of eight dims each: lane `c` of a head
+// holds dims 8 c .. 8 c + 7, group c / 4, t = c % 4. Rotation pairs dim d with
+// d + D / 2, half a head's lanes away.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "q4.h"
+#include "qx_math.cuh"
+#include "qx_ptx.cuh"
+
+namespace qx {
+
+struct GraniteHeads {
+  static constexpr bool QWEN = false;
+  static constexpr int HQ = 16, HKV = 8, D = 64, G = 2;
+  static constexpr float SCALE = 0.015625f;  // ATTENTION_MULTIPLIER, qx-model lib.rs:20
+};
+struct Qwen3Heads {
+  static constexpr bool QWEN = true;
+  static constexpr int HQ = 32, HKV = 4, D = 128, G = 8;
+  static constexpr float SCALE = 0.08838834764831845f;  // 1/sqrt(128)
+};
+
+constexpr int kQ4CodeBytes = 256;
+constexpr int kQ4RowBytes = 288;
+
+template <class M>
+struct Q4Row {
+  static constexpr int NG = M::D / 32;   // groups per head
+  static constexpr int LPH = M::D / 8;   // lanes per head
+  static constexpr int HEAD = M::D / 2;  // code bytes per head
+  static_assert(M::HKV * HEAD == kQ4CodeBytes, "codes of a row");
+  static_assert(kQ4CodeBytes + M::HKV * NG * 2 == kQ4RowBytes, "codes and scales of a row");
+  static __device__ __forceinline__ int key_word(int head, int c) { return head * HEAD + 4 * ((c & 3) * NG + (c >> 2)); }
+  static __device__ __forceinline__ int value_half(int head, int j, int g) { return head * HEAD + 2 * (g * NG + j); }
+  static __device__ __forceinline__ int scale(int head, int j) { return kQ4CodeBytes + 2 * (head * NG + j); }
+};
+
+// Eight neighbouring elements as f32 (vec: base + i is 16-byte aligned).
+__device__ __forceinline__ void load8(const void* base, long long i, int dtype, bool vec, float* x) {
+  if (!vec) {
+    load_any_n<8>(base, i, 1, dtype, x);
+  } else if (dtype == 1) {
+    Vec16<__nv_bfloat16>::load(reinterpret_cast<const __nv_bfloat16*>(base) + i, x);
+  } else if (dtype == 2) {
+    Vec16<__half>::load(reinterpret_cast<const __half*>(base) + i, x);
+  } else {
+    Vec16<float>::load(reinterpret_cast<const float*>(base) + i, x);
+    Vec16<float>::load(reinterpret_cast<const float*>(base) + i + 4, x + 4);
+  }
+}
+
+__device__ __forceinline__ void store8(void* base, long long i, int dtype, bool vec, const float* x) {
+  if (!vec) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) store_any(base, i + e, dtype, x[e]);
+  } else if (dtype == 0) {
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i);
+    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (dtype == 1) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b);
+      } else {
+        const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// 1 / sqrt(mean + 1e-6) rounded once to f32. The sum of squares is a double
+// (products of two 16-bit inputs and their sum are exact in it), so its order
+// does not matter: quantised keys sit next to rounding borders, where an ulp
+// of the norm would decide a code.
+template <class M>
+__device__ __forceinline__ float head_inv_rms(const float* x) {
+  double sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum = fma((double)x[e], (double)x[e], sum);
+#pragma unroll
+  for (int o = Q4Row<M>::LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return (float)rsqrt(sum * (1.0 / M::D) + 1.0e-6);
+}
+
+// Norm (Qwen) and rotation of this lane's eight dims of a head at `position`.
+// The operation order is each model's: granite_rope_pair's fused pair
+// (qx-consensus-math lib.rs:199-207), cpu_qk_norm_rope's separately rounded
+// one (qx-qwen-parity main.rs:1170-1210). False when a result is not finite.
+template <class M>
+__device__ __forceinline__ bool rotate_head(float* x, int c, int position, const float* norm, const float2* rope) {
+  constexpr int LPH = Q4Row<M>::LPH;
+  if constexpr (M::QWEN) {
+    const float inv = head_inv_rms<M>(x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inv), norm ? norm[8 * c + e] : 1.0f);
+  }
+  const bool right = c >= LPH / 2;
+  const float2* tab = rope + (long long)position * (M::D / 2) + 8 * (c & (LPH / 2 - 1));
+  bool good = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = __shfl_xor_sync(0xffffffffu, x[e], LPH / 2);
+    const float2 t = tab[e];
+    if constexpr (M::QWEN)
+      x[e] = right ? __fadd_rn(__fmul_rn(x[e], t.x), __fmul_rn(y, t.y))
+                   : __fsub_rn(__fmul_rn(x[e], t.x), __fmul_rn(y, t.y));
+    else
+      x[e] = right ? __fmaf_rn(x[e], t.y, __fmul_rn(y, t.x)) : __fmaf_rn(-y, t.x, __fmul_rn(x[e], t.y));
+    good &= isfinite(x[e]);
+  }
+  return good;
+}
+
+// Codes of this lane's eight dims (nibble e: dim 8 c + e) and its group's
+// scale. False when the scale is not finite: a value above 7 * 65504, an
+// infinity, or a NaN (which fmaxf alone would drop).
+__device__ __forceinline__ bool quantise8(const float* x, uint32_t* codes, __half* scale) {
+  float top = 0.0f;
+  bool good = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top = fmaxf(top, fabsf(x[e]));
+    good &= isfinite(x[e]);
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const __half h = __float2half_rn(__fdiv_rn(top, 7.0f));
+  const float s = __half2float(h);
+  uint32_t w = 0x77777777u;  // a scale that rounds to zero: every value is zero
+  if (s > 0.0f) {
+    w = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int code = __float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f)) + 7;
+      w |= (uint32_t)code << (4 * e);
+    }
+  }
+  *codes = w;
+  *scale = h;
+  return good && isfinite(s);
+}
+
+// Store this lane's codes and scale as part of a key row.
+template <class M>
+__device__ __forceinline__ void put_key(char* row, int head, int c, uint32_t codes, __half scale) {
+  *reinterpret_cast<uint32_t*>(row + Q4Row<M>::key_word(head, c)) = codes;
+  if ((c & 3) == 0) *reinterpret_cast<__half*>(row + Q4Row<M>::scale(head, c >> 2)) = scale;
+}
+
+// Store this lane's codes and scale as part of a value row: nibble i of half
+// g comes from lane t = i of the group, which holds dims 8 i + g.
+template <class M>
+__device__ __forceinline__ void put_value(char* row, int head, int c, uint32_t codes, __half scale) {
+  const int t = c & 3, j = c >> 2, quad = (threadIdx.x & 31) & ~3;
+  uint32_t lo = 0u, hi = 0u;  // halves g = 2 t and 2 t + 1
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = __shfl_sync(0xffffffffu, codes, quad + i) >> (8 * t);
+    lo |= (w & 15u) << (4 * i);
+    hi |= ((w >> 4) & 15u) << (4 * i);
+  }
+  *reinterpret_cast<uint16_t*>(row + Q4Row<M>::value_half(head, j, 2 * t)) = (uint16_t)lo;
+  *reinterpret_cast<uint16_t*>(row + Q4Row<M>::value_half(head, j, 2 * t + 1)) = (uint16_t)hi;
+  if (t == 0) *reinterpret_cast<__half*>(row + Q4Row<M>::scale(head, j)) = scale;
+}
+
+// The entry of seqs (in rising order of `first`) that holds index i.
+__device__ __forceinline__ int find_seq(const Q4Seq* seqs, int n, int i) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (seqs[mid].first <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+}  // namespace qx

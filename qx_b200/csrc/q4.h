@@ -1,0 +1,95 @@
+// q4.h — launches of the 4-bit KV cache and packed-prompt kernels
+// (q4_cache.cu, q4_decode.cu, packed.cu), as qxcuda.cu calls them.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_row.cuh"
+
+namespace qx {
+
+// Sequences of one launch: they travel in the parameter block (under 4 KB),
+// so a call copies no table and a captured graph keeps its own. Calls with
+// more sequences make one launch per kQ4Seqs of them.
+constexpr int kQ4Seqs = 200;
+
+// One sequence's rows in a call.
+struct Q4Seq {
+  int seq;    // sequence index in the arena
+  int begin;  // first cache row (append, read) or rows attended (decode)
+  int first;  // first packed token of this sequence (append, read) or first work item (decode)
+};
+
+// A 4-bit arena as the kernels see it.
+struct Q4Arena {
+  char* k;
+  char* v;
+  int capacity;  // rows per (sequence, layer) of a contiguous arena
+  int layers;
+  KvPaging paging;
+};
+
+struct Q4AppendParams {
+  Q4Arena arena;
+  int layer_begin, layer_count;
+  int n_seq;
+  int token_begin, token_count;  // packed tokens of this launch
+  const void* q;                 // null: only keys and values
+  const void* k;
+  const void* v;
+  void* q_rot;  // rotated queries [token][layer][HQ * D], or null
+  void* k_rot;  // rotated keys before quantisation, or null
+  long long q_stride, k_stride, v_stride;  // elements between tokens
+  const float* q_norm;
+  const float* k_norm;
+  const float2* rope;  // Granite: (sin, cos); Qwen: (cos, sin); [position][D / 2]
+  int q_dtype, in_dtype, rot_dtype;
+  int vec;  // q, k, v and their strides allow 16-byte loads, q_rot and k_rot 16-byte stores
+  unsigned* err;
+  Q4Seq seqs[kQ4Seqs];
+};
+
+struct Q4ReadParams {
+  Q4Arena arena;
+  int layer_begin, layer_count;
+  int n_seq;
+  int token_begin, token_count;
+  void* key_out;    // [token][layer][HKV * D], or null
+  void* value_out;  // likewise
+  int out_dtype;
+  int vec;  // the outputs allow 16-byte stores
+  Q4Seq seqs[kQ4Seqs];
+};
+
+struct Q4DecodeParams {
+  Q4Arena arena;
+  int layer_begin, layer_count;
+  int n_seq;
+  int seq_begin;  // index of seqs[0] among the call's sequences
+  const float* q;  // rotated queries [sequence][layer][HQ * D]
+  void* out;       // [sequence][layer][HQ * D]
+  int out_dtype;
+  unsigned* err;
+  Q4Seq seqs[kQ4Seqs];
+};
+
+struct PackedParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;  // [token][HQ][D]
+  long long q_stride, k_stride, v_stride;  // elements between tokens
+  int dtype;
+  int n_seq;
+  int token_begin, token_count;
+  unsigned* err;
+  Q4Seq seqs[kQ4Seqs];  // begin: tokens of the sequence; first: its first packed token
+};
+
+cudaError_t launch_q4_append(bool qwen, const Q4AppendParams& p, cudaStream_t stream);
+cudaError_t launch_q4_read(bool qwen, const Q4ReadParams& p, cudaStream_t stream);
+cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream);
+cudaError_t launch_packed(bool qwen, const PackedParams& p, cudaStream_t stream);
+
+}  // namespace qx

@@ -31,8 +31,14 @@
 #include "pages.cuh"
 #include "exchange.cuh"
 #include "stack.cuh"
+#include "q4.h"
 
 using namespace qx;
+
+struct Workspace {
+  char* ptr = nullptr;
+  size_t bytes = 0;
+};
 
 struct qxc_ctx {
   int device = 0;
@@ -89,6 +95,11 @@ struct qxc_ctx {
   unsigned* stack_words = nullptr;
   unsigned stack_gen = 0;
   unsigned stack_tickets = 0;  // every head's merge-ticket count after the launches so far
+  // 4-bit decode's and packed prefill's workspaces; the buffers they have
+  // outgrown are kept until the context goes, since a captured graph may
+  // still name them
+  Workspace q4_q, packed_rot;
+  std::vector<void*> outgrown;
   // prefill's rotated-query scratch (bf16 elements)
   unsigned short* prefill_q = nullptr;
   size_t prefill_q_cap = 0;
@@ -122,7 +133,7 @@ struct qxc_kv {
   qxc_ctx* ctx = nullptr;
   qxc_kv_desc desc{};
   int hq = 0, hkv = 0, d = 0;
-  size_t kes = 0, ves = 0;
+  size_t krow = 0, vrow = 0;  // bytes of one position's keys / values, all kv heads
   char* base = nullptr;
   char* k_region = nullptr;
   char* v_region = nullptr;
@@ -182,6 +193,15 @@ qxc_status fail(qxc_ctx* ctx, qxc_status st, const char* fmt, ...) {
 size_t dtype_size(int dt) { return dt == QXC_F32 ? 4 : 2; }
 bool valid_dtype(int dt) { return dt == QXC_F32 || dt == QXC_BF16 || dt == QXC_F16; }
 
+// Bytes of one position's keys or values: a 4-bit row is two codes a byte and
+// an fp16 scale per 32 of them.
+size_t row_bytes(int dt, int hkv, int d) {
+  const size_t n = (size_t)hkv * d;
+  return dt == QXC_Q4 ? n / 2 + n / 32 * 2 : n * dtype_size(dt);
+}
+
+bool is_q4(const qxc_kv* kv) { return kv->desc.key_dtype == QXC_Q4; }
+
 void model_shape(int model, int* hq, int* hkv, int* d) {
   if (model == QXC_MODEL_QWEN3) {
     *hq = 32, *hkv = 4, *d = 128;
@@ -196,8 +216,13 @@ qxc_status check_desc(qxc_ctx* ctx, const qxc_kv_desc* d) {
     return fail(ctx, QXC_ERR_INVALID_ARG, "unknown model %d", d->model);
   if (d->layers < 1 || d->sequences < 1)
     return fail(ctx, QXC_ERR_INVALID_ARG, "layers and sequences must be >= 1");
-  if (!valid_dtype(d->key_dtype) || !valid_dtype(d->value_dtype))
+  const bool q4 = d->key_dtype == QXC_Q4 && d->value_dtype == QXC_Q4;
+  if (!q4 && (d->key_dtype == QXC_Q4 || d->value_dtype == QXC_Q4))
+    return fail(ctx, QXC_ERR_UNSUPPORTED, "a 4-bit arena holds both keys and values in 4 bits");
+  if (!q4 && (!valid_dtype(d->key_dtype) || !valid_dtype(d->value_dtype)))
     return fail(ctx, QXC_ERR_INVALID_ARG, "unknown KV dtype");
+  if (q4 && d->first_position > 0)
+    return fail(ctx, QXC_ERR_UNSUPPORTED, "a 4-bit arena cannot be a KV-length shard");
   if (d->first_position < 0) return fail(ctx, QXC_ERR_INVALID_ARG, "first_position must be >= 0");
   if (d->model == QXC_MODEL_GRANITE) {
     // ExecutionPlan::granite_with_kv_element_bytes (qx-runtime-v2 lib.rs:6587-6589)
@@ -898,8 +923,7 @@ qxc_status launch_hash(qxc_ctx* ctx, const HashParams& p, int ctas, void (*fn)(H
 // 256-byte chunks (encode_verification_hashes' rule, qx-metal lib.rs:9288-9302).
 qxc_status hash_params(qxc_ctx* ctx, const qxc_kv* kv, int seq, HashParams* p) {
   memset(p, 0, sizeof(*p));
-  const long long krow = (long long)kv->hkv * kv->d * (long long)kv->kes;
-  const long long vrow = (long long)kv->hkv * kv->d * (long long)kv->ves;
+  const long long krow = (long long)kv->krow, vrow = (long long)kv->vrow;
   for (long long b : {krow, vrow}) {
     const long long c = b / 256;
     if (b % 256 != 0 || c < 1 || c > 8 || (c & (c - 1)) != 0)
@@ -995,6 +1019,253 @@ qxc_status launch_verify_shared(qxc_ctx* ctx, qxc_kv* kv, const qxc_verify_args*
   return launch_verify_typed<__nv_bfloat16, __nv_bfloat16>(ctx, kv, a);
 }
 
+// ---- 4-bit arenas and packed prompts -----------------------------------------------
+namespace {
+
+// The caller's current device, put back when a call leaves.
+struct DeviceGuard {
+  int before = -1;
+  bool ok;
+  explicit DeviceGuard(int device) {
+    ok = cudaGetDevice(&before) == cudaSuccess && (before == device || cudaSetDevice(device) == cudaSuccess);
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+// At least `bytes` of workspace. Growing keeps the old buffer (see outgrown)
+// and is refused under stream capture, where nothing may be allocated.
+qxc_status reserve(qxc_ctx* ctx, Workspace* w, size_t bytes) {
+  if (bytes <= w->bytes) return QXC_OK;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  QXC_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+  if (capture != cudaStreamCaptureStatusNone)
+    return fail(ctx, QXC_ERR_UNSUPPORTED, "a workspace of %zu bytes is needed: make the call once before its capture",
+                bytes);
+  const size_t want = std::max(bytes, 2 * w->bytes);
+  void* p = nullptr;
+  QXC_CUDA(ctx, cudaMalloc(&p, want));
+  if (w->ptr) ctx->outgrown.push_back(w->ptr);
+  w->ptr = static_cast<char*>(p);
+  w->bytes = want;
+  return QXC_OK;
+}
+
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+Q4Arena q4_arena(const qxc_kv* kv) {
+  Q4Arena a;
+  a.k = kv->k_region;
+  a.v = kv->v_region;
+  a.capacity = kv->desc.capacity;
+  a.layers = kv->desc.layers;
+  a.paging = kv_paging(kv);
+  return a;
+}
+
+const float2* rope_of(const qxc_ctx* ctx, const qxc_kv* kv) {
+  return kv->desc.model == QXC_MODEL_QWEN3 ? ctx->qwen_rope : ctx->granite_rope;
+}
+
+bool is_qwen(const qxc_kv* kv) { return kv->desc.model == QXC_MODEL_QWEN3; }
+
+// Call `launch(seqs, n, first token, tokens)` for every kQ4Seqs sequences
+// that have rows: `begins` and `counts` per sequence, packed one after another.
+template <class F>
+qxc_status each_part(int seq_count, const int32_t* seq_ids, const int32_t* begins, const int32_t* counts, F launch) {
+  Q4Seq seqs[kQ4Seqs];
+  int n = 0;
+  long long at = 0, first = 0;
+  for (int i = 0; i < seq_count; ++i) {
+    if (counts[i]) {
+      seqs[n].seq = seq_ids ? seq_ids[i] : i;
+      seqs[n].begin = begins[i];
+      seqs[n].first = (int)at;
+      ++n;
+    }
+    at += counts[i];
+    if (n == kQ4Seqs || (i == seq_count - 1 && n)) {
+      qxc_status st = launch(seqs, n, (int)first, (int)(at - first));
+      if (st != QXC_OK) return st;
+      n = 0;
+      first = at;
+    }
+  }
+  return QXC_OK;
+}
+
+// Layers, sequences and rows of a call that writes or reads many rows of a
+// 4-bit arena; `rows[i]` becomes the end of sequence i's range.
+qxc_status check_rows(qxc_ctx* ctx, const qxc_kv* kv, int layer_begin, int layer_count, int seq_count,
+                      const int32_t* seq_ids, const int32_t* begins, const int32_t* counts, std::vector<int>* ids,
+                      std::vector<int>* ends, long long* total) {
+  if (kv->ctx != ctx) return fail(ctx, QXC_ERR_INVALID_ARG, "KV arena belongs to another context");
+  if (!is_q4(kv)) return fail(ctx, QXC_ERR_UNSUPPORTED, "the call needs a 4-bit arena");
+  if (layer_count < 1 || layer_begin < 0 || (long long)layer_begin + layer_count > kv->desc.layers)
+    return fail(ctx, QXC_ERR_INVALID_ARG, "layers [%d, %lld) outside the arena's %d layers", layer_begin,
+                (long long)layer_begin + layer_count, kv->desc.layers);
+  if (seq_count < 1 || !begins || !counts)
+    return fail(ctx, QXC_ERR_INVALID_ARG, "seq_count >= 1, first rows and counts required");
+  *total = 0;
+  for (int i = 0; i < seq_count; ++i) {
+    const int seq = seq_ids ? seq_ids[i] : i;
+    qxc_status st = check_seq(ctx, kv, seq);
+    if (st != QXC_OK) return st;
+    if (counts[i] < 0 || begins[i] < 0)
+      return fail(ctx, QXC_ERR_INVALID_ARG, "sequence %d: %d rows from row %d", seq, counts[i], begins[i]);
+    if ((long long)begins[i] + counts[i] > kv->desc.capacity)
+      return fail(ctx, QXC_ERR_POSITION, "KV position %lld exceeds context %d", (long long)begins[i] + counts[i] - 1,
+                  kv->desc.capacity);
+    ids->push_back(seq);
+    ends->push_back(begins[i] + counts[i]);
+    *total += counts[i];
+  }
+  // the kernels' grids and packed token indices are 32-bit
+  if (*total * layer_count * 16 > 0x7fffffffLL)
+    return fail(ctx, QXC_ERR_INVALID_ARG, "too many rows in one call (%lld tokens x %d layers)", *total, layer_count);
+  return QXC_OK;
+}
+
+qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a, int q_dtype, int rot_dtype) {
+  Q4AppendParams p;
+  p.arena = q4_arena(kv);
+  p.layer_begin = a->layer_begin;
+  p.layer_count = a->layer_count;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.q_rot = a->q_rot;
+  p.k_rot = a->k_rot;
+  const long long qn = (long long)a->layer_count * kv->hq * kv->d, kn = (long long)a->layer_count * kv->hkv * kv->d;
+  p.q_stride = a->q_stride ? a->q_stride : qn;
+  p.k_stride = a->k_stride ? a->k_stride : kn;
+  p.v_stride = a->v_stride ? a->v_stride : kn;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.rope = rope_of(ctx, kv);
+  p.q_dtype = q_dtype;
+  p.in_dtype = a->in_dtype;
+  p.rot_dtype = rot_dtype;
+  // elements of a 16-byte load
+  const long long lanes = 16 / (long long)std::min(dtype_size(a->in_dtype), dtype_size(q_dtype));
+  p.vec = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->q_rot, 16) &&
+          aligned(a->k_rot, 16) && p.q_stride % lanes == 0 && p.k_stride % lanes == 0 && p.v_stride % lanes == 0;
+  p.err = ctx->err_dev;
+  return each_part(a->seq_count, a->seq_ids, a->positions, a->counts, [&](const Q4Seq* seqs, int n, int first, int tokens) {
+    memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
+    p.n_seq = n;
+    p.token_begin = first;
+    p.token_count = tokens;
+    QXC_CUDA(ctx, launch_q4_append(is_qwen(kv), p, ctx->stream));
+    ctx->launches++;
+    note_rows_written(ctx, kv, -1, 0);
+    return QXC_OK;
+  });
+}
+
+// One decode step on a 4-bit arena, its arguments checked and its pages
+// mapped: the new rows and rotated queries, then the attention.
+qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
+  const size_t heads = (size_t)a->seq_count * a->layer_count * kv->hq * kv->d;
+  float* q = a->q_rot_out;
+  if (!q) {
+    qxc_status st = reserve(ctx, &ctx->q4_q, heads * sizeof(float));
+    if (st != QXC_OK) return st;
+    q = reinterpret_cast<float*>(ctx->q4_q.ptr);
+  }
+  std::vector<int32_t> ones(a->seq_count, 1), attend(a->seq_count);
+  for (int i = 0; i < a->seq_count; ++i) attend[i] = a->positions[i] + 1;
+  qxc_append_args ap;
+  memset(&ap, 0, sizeof(ap));
+  ap.layer_begin = a->layer_begin;
+  ap.layer_count = a->layer_count;
+  ap.seq_count = a->seq_count;
+  ap.seq_ids = a->seq_ids;
+  ap.positions = a->positions;
+  ap.counts = ones.data();
+  ap.q = a->q;
+  ap.k = a->k;
+  ap.v = a->v;
+  ap.q_rot = q;
+  ap.q_norm = a->q_norm;
+  ap.k_norm = a->k_norm;
+  ap.in_dtype = a->in_dtype;
+  qxc_status st = q4_append(ctx, kv, &ap, a->q_dtype, QXC_F32);
+  if (st != QXC_OK) return st;
+  Q4DecodeParams p;
+  p.arena = q4_arena(kv);
+  p.layer_begin = a->layer_begin;
+  p.layer_count = a->layer_count;
+  p.q = q;
+  p.out = a->out;
+  p.out_dtype = a->out_dtype;
+  p.err = ctx->err_dev;
+  return each_part(a->seq_count, a->seq_ids, attend.data(), ones.data(), [&](const Q4Seq* seqs, int n, int first, int) {
+    memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
+    p.n_seq = n;
+    p.seq_begin = first;
+    QXC_CUDA(ctx, launch_q4_decode(is_qwen(kv), p, ctx->stream));
+    ctx->launches++;
+    return QXC_OK;
+  });
+}
+
+// Lengths of packed prompts: every one >= 0, together within 32-bit indices.
+qxc_status check_lengths(qxc_ctx* ctx, int seq_count, const int32_t* lengths, long long* total) {
+  if (seq_count < 1 || !lengths) return fail(ctx, QXC_ERR_INVALID_ARG, "seq_count >= 1 and lengths required");
+  *total = 0;
+  for (int i = 0; i < seq_count; ++i) {
+    if (lengths[i] < 0) return fail(ctx, QXC_ERR_INVALID_ARG, "prompt %d has length %d", i, lengths[i]);
+    *total += lengths[i];
+  }
+  if (*total > (1 << 24)) return fail(ctx, QXC_ERR_INVALID_ARG, "%lld packed tokens; at most 2^24", *total);
+  return QXC_OK;
+}
+
+qxc_status attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
+  int hq, hkv, d;
+  model_shape(a->model, &hq, &hkv, &d);
+  PackedParams p;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.out = a->out;
+  p.q_stride = a->q_stride ? a->q_stride : (long long)hq * d;
+  p.k_stride = a->k_stride ? a->k_stride : (long long)hkv * d;
+  p.v_stride = a->v_stride ? a->v_stride : (long long)hkv * d;
+  p.dtype = a->dtype;
+  p.err = ctx->err_dev;
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) || p.q_stride % 8 ||
+      p.k_stride % 8 || p.v_stride % 8)
+    return fail(ctx, QXC_ERR_INVALID_ARG, "packed tensors must be 16-byte aligned, their token strides multiples of 8");
+  if (p.q_stride < (long long)hq * d || p.k_stride < (long long)hkv * d || p.v_stride < (long long)hkv * d)
+    return fail(ctx, QXC_ERR_INVALID_ARG, "a token stride is shorter than a token's heads");
+  return each_part(a->seq_count, nullptr, a->lengths, a->lengths, [&](const Q4Seq* seqs, int n, int first, int tokens) {
+    memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
+    p.n_seq = n;
+    p.token_begin = first;
+    p.token_count = tokens;
+    QXC_CUDA(ctx, launch_packed(a->model == QXC_MODEL_QWEN3, p, ctx->stream));
+    ctx->launches++;
+    return QXC_OK;
+  });
+}
+
+// No C++ exception leaves a C entry point.
+template <class F>
+qxc_status guarded(qxc_ctx* ctx, F body) {
+  try {
+    return body();
+  } catch (const std::bad_alloc&) {
+    return fail(ctx, QXC_ERR_OUT_OF_MEMORY, "host allocation failed");
+  } catch (...) {
+    return fail(ctx, QXC_ERR_INVALID_ARG, "unexpected exception");
+  }
+}
+
+}  // namespace
+
 extern "C" {
 
 int qxc_abi_version(void) { return QXC_ABI_VERSION; }
@@ -1059,6 +1330,9 @@ void qxc_destroy(qxc_ctx* ctx) {
   cudaFree(ctx->stack_f);
   cudaFree(ctx->stack_words);
   cudaFree(ctx->prefill_q);
+  cudaFree(ctx->q4_q.ptr);
+  cudaFree(ctx->packed_rot.ptr);
+  for (void* p : ctx->outgrown) cudaFree(p);
   if (ctx->err_host) cudaFreeHost(ctx->err_host);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   delete ctx;
@@ -1120,9 +1394,9 @@ qxc_status qxc_kv_bytes(const qxc_kv_desc* d, size_t* key_bytes, size_t* value_b
   if (st != QXC_OK) return st;
   int hq, hkv, hd;
   model_shape(d->model, &hq, &hkv, &hd);
-  const size_t per = (size_t)d->capacity * hkv * hd * (size_t)d->layers * d->sequences;
-  if (key_bytes) *key_bytes = per * dtype_size(d->key_dtype);
-  if (value_bytes) *value_bytes = per * dtype_size(d->value_dtype);
+  const size_t rows = (size_t)d->capacity * (size_t)d->layers * d->sequences;
+  if (key_bytes) *key_bytes = rows * row_bytes(d->key_dtype, hkv, hd);
+  if (value_bytes) *value_bytes = rows * row_bytes(d->value_dtype, hkv, hd);
   return QXC_OK;
 }
 
@@ -1156,10 +1430,10 @@ static qxc_status kv_create(qxc_ctx* ctx, const qxc_kv_desc* desc, const qxc_kv_
   kv->ctx = ctx;
   kv->desc = *desc;
   model_shape(desc->model, &kv->hq, &kv->hkv, &kv->d);
-  kv->kes = dtype_size(desc->key_dtype);
-  kv->ves = dtype_size(desc->value_dtype);
-  kv->k_unit = (size_t)desc->capacity * kv->hkv * kv->d * kv->kes;
-  kv->v_unit = (size_t)desc->capacity * kv->hkv * kv->d * kv->ves;
+  kv->krow = row_bytes(desc->key_dtype, kv->hkv, kv->d);
+  kv->vrow = row_bytes(desc->value_dtype, kv->hkv, kv->d);
+  kv->k_unit = (size_t)desc->capacity * kv->krow;
+  kv->v_unit = (size_t)desc->capacity * kv->vrow;
   size_t rows = (size_t)desc->layers * desc->sequences * desc->capacity;
   if (paging) {
     for (int s2 = 1; (1 << s2) <= paging->page_size; ++s2) kv->page_shift = s2;
@@ -1170,7 +1444,7 @@ static qxc_status kv_create(qxc_ctx* ctx, const qxc_kv_desc* desc, const qxc_kv_
     for (int pg = paging->pool_pages - 1; pg >= 0; --pg) kv->free_pages.push_back(pg);
     rows = (size_t)desc->layers * paging->pool_pages * paging->page_size;
   }
-  const size_t kbytes = rows * kv->hkv * kv->d * kv->kes, vbytes = rows * kv->hkv * kv->d * kv->ves;
+  const size_t kbytes = rows * kv->krow, vbytes = rows * kv->vrow;
   const size_t koff_v = ((kbytes + 255) / 256) * 256;
   cudaError_t e = cudaMalloc(&kv->base, koff_v + vbytes);
   if (e == cudaSuccess && paging) {
@@ -1188,8 +1462,13 @@ static qxc_status kv_create(qxc_ctx* ctx, const qxc_kv_desc* desc, const qxc_kv_
   kv->k_region = kv->base;
   kv->v_region = kv->base + koff_v;
   kv->len.assign(desc->sequences, 0);
-  qxc_status mst = encode_kv_map(ctx, &kv->tmk, kv->k_region, desc->key_dtype, kv->hkv, kv->d, rows);
-  if (mst == QXC_OK) mst = encode_kv_map(ctx, &kv->tmv, kv->v_region, desc->value_dtype, kv->hkv, kv->d, rows);
+  qxc_status mst = QXC_OK;
+  if (!is_q4(kv)) {
+    mst = encode_kv_map(ctx, &kv->tmk, kv->k_region, desc->key_dtype, kv->hkv, kv->d, rows);
+    if (mst == QXC_OK) mst = encode_kv_map(ctx, &kv->tmv, kv->v_region, desc->value_dtype, kv->hkv, kv->d, rows);
+  } else if (desc->model == QXC_MODEL_GRANITE) {
+    mst = ensure_granite_rope(ctx);  // the 4-bit kernels rotate from the table of pinned values
+  }
   if (mst == QXC_OK && desc->model == QXC_MODEL_QWEN3) mst = ensure_qwen_rope(ctx);
   if (mst != QXC_OK) {
     cudaFree(kv->base);
@@ -1219,9 +1498,9 @@ qxc_status qxc_kv_paged_bytes(const qxc_kv_desc* d, const qxc_kv_paging* pg, siz
   if (st != QXC_OK) return st;
   int hq, hkv, hd;
   model_shape(d->model, &hq, &hkv, &hd);
-  const size_t per = (size_t)d->layers * pg->pool_pages * pg->page_size * hkv * hd;
-  if (key_bytes) *key_bytes = per * dtype_size(d->key_dtype);
-  if (value_bytes) *value_bytes = per * dtype_size(d->value_dtype);
+  const size_t rows = (size_t)d->layers * pg->pool_pages * pg->page_size;
+  if (key_bytes) *key_bytes = rows * row_bytes(d->key_dtype, hkv, hd);
+  if (value_bytes) *value_bytes = rows * row_bytes(d->value_dtype, hkv, hd);
   return QXC_OK;
 }
 
@@ -1239,7 +1518,7 @@ qxc_status qxc_kv_pool_buffer(qxc_kv* kv, int32_t key, void** ptr, size_t* bytes
   if (!kv->paged()) return fail(kv->ctx, QXC_ERR_UNSUPPORTED, "the arena is not paged");
   const size_t rows = (size_t)kv->desc.layers * kv->pool_pages << kv->page_shift;
   *ptr = key ? kv->k_region : kv->v_region;
-  if (bytes) *bytes = rows * kv->hkv * kv->d * (key ? kv->kes : kv->ves);
+  if (bytes) *bytes = rows * (key ? kv->krow : kv->vrow);
   return QXC_OK;
 }
 
@@ -1369,7 +1648,7 @@ static qxc_status kv_copy(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin,
     }
   }
   QXC_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-  const size_t krow = (size_t)kv->hkv * kv->d * kv->kes, vrow = (size_t)kv->hkv * kv->d * kv->ves;
+  const size_t krow = kv->krow, vrow = kv->vrow;
   const KvPaging pg = kv_paging(kv);
   // runs of rows contiguous in the arena: the whole range, or one page at a time
   for (int r = begin; r < begin + count;) {
@@ -1419,8 +1698,15 @@ qxc_status qxc_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
   if (!a->q || !a->k || !a->v || !a->out) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
   if (!valid_dtype(a->q_dtype) || !valid_dtype(a->in_dtype) || !valid_dtype(a->out_dtype))
     return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
-  if (kv->desc.model == QXC_MODEL_QWEN3 && (a->q_dtype != kv->desc.key_dtype || a->in_dtype != kv->desc.key_dtype))
+  if (is_q4(kv)) {
+    if (a->flags & QXC_DECODE_PINNED_EXP)
+      return fail(ctx, QXC_ERR_UNSUPPORTED, "a 4-bit arena decodes with the hardware exponential");
+    if (a->split < 0 || a->split % 64 != 0)
+      return fail(ctx, QXC_ERR_INVALID_ARG, "split %d must be a positive multiple of 64", a->split);
+  } else if (kv->desc.model == QXC_MODEL_QWEN3 &&
+             (a->q_dtype != kv->desc.key_dtype || a->in_dtype != kv->desc.key_dtype)) {
     return fail(ctx, QXC_ERR_INVALID_ARG, "Qwen q/k/v must use the KV cache's 16-bit type");
+  }
   if (kv->desc.first_position != 0)
     return fail(ctx, QXC_ERR_INVALID_ARG, "a KV-length shard decodes through qxc_decode_partials");
   std::vector<int> attend(a->seq_count), new_slot(a->seq_count), rope(a->seq_count);
@@ -1447,6 +1733,12 @@ qxc_status qxc_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
     for (int i = 0; i < a->seq_count; ++i) ids[i] = a->seq_ids ? a->seq_ids[i] : i;
     qxc_status st = ensure_pages(ctx, kv, a->seq_count, ids.data(), attend.data());
     if (st != QXC_OK) return st;
+  }
+  if (is_q4(kv)) {
+    qxc_status st = q4_decode(ctx, kv, a);
+    if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
+      for (int i = 0; i < a->seq_count; ++i) kv->len[a->seq_ids ? a->seq_ids[i] : i] += 1;
+    return st;
   }
   CallPlan plan;
   qxc_status st = plan_call(ctx, kv, a->seq_count, a->seq_ids, attend.data(), new_slot.data(), rope.data(),
@@ -1767,6 +2059,7 @@ qxc_status qxc_decode_verify(qxc_ctx* ctx, qxc_kv* kv, const qxc_verify_args* a)
   if (!a->q || !a->k || !a->v || !a->out) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
   if (!valid_dtype(a->q_dtype) || !valid_dtype(a->in_dtype) || !valid_dtype(a->out_dtype))
     return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
+  if (is_q4(kv)) return fail(ctx, QXC_ERR_UNSUPPORTED, "verify does not read a 4-bit arena");
   if (kv->desc.model == QXC_MODEL_QWEN3 && (a->q_dtype != kv->desc.key_dtype || a->in_dtype != kv->desc.key_dtype))
     return fail(ctx, QXC_ERR_INVALID_ARG, "Qwen q/k/v must use the KV cache's 16-bit type");
   if (kv->desc.first_position != 0)
@@ -1977,6 +2270,7 @@ static qxc_status decode_partials_impl(qxc_ctx* ctx, qxc_kv* kv, const qxc_parti
   if (a->layer < 0 || a->layer >= kv->desc.layers) return fail(ctx, QXC_ERR_INVALID_ARG, "layer %d out of range", a->layer);
   if (!a->q || (!a->partials && !g) || (a->append && (!a->k || !a->v)))
     return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+  if (is_q4(kv)) return fail(ctx, QXC_ERR_UNSUPPORTED, "partials are not taken from a 4-bit arena");
   if (kv->desc.model == QXC_MODEL_QWEN3 && (a->q_dtype != kv->desc.key_dtype || (a->append && a->in_dtype != kv->desc.key_dtype)))
     return fail(ctx, QXC_ERR_INVALID_ARG, "Qwen q/k/v must use the KV cache's 16-bit type");
   const int first = kv->desc.first_position;
@@ -2351,6 +2645,153 @@ qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* a) {
   ctx->launches += 2;
   if (!(a->flags & QXC_DECODE_NO_ADVANCE)) kv->len[a->seq] = a->length;
   return QXC_OK;
+}
+
+// ---- 4-bit arenas and packed prompts -----------------------------------------------
+qxc_status qxc_kv_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
+  if (!ctx || !kv || !a) return fail(ctx, QXC_ERR_INVALID_ARG, "null argument");
+  return guarded(ctx, [&]() -> qxc_status {
+    std::vector<int> ids, ends;
+    long long total;
+    qxc_status st = check_rows(ctx, kv, a->layer_begin, a->layer_count, a->seq_count, a->seq_ids, a->positions,
+                               a->counts, &ids, &ends, &total);
+    if (st != QXC_OK) return st;
+    if (!valid_dtype(a->in_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
+    if (!a->q != !a->q_rot) return fail(ctx, QXC_ERR_INVALID_ARG, "q and q_rot go together");
+    if ((a->q_rot || a->k_rot) && !valid_dtype(a->rot_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
+    if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0)
+      return fail(ctx, QXC_ERR_INVALID_ARG, "negative token stride");
+    std::vector<char> seen(kv->desc.sequences, 0);
+    for (int i = 0; i < a->seq_count; ++i) {
+      if (seen[ids[i]]) return fail(ctx, QXC_ERR_INVALID_ARG, "sequence %d appears twice in one call", ids[i]);
+      seen[ids[i]] = 1;
+      // KvCache::append (qx-runtime lib.rs:385-398)
+      if (a->positions[i] != kv->len[ids[i]])
+        return fail(ctx, QXC_ERR_POSITION, "KV position %d does not follow cache length %d", a->positions[i],
+                    kv->len[ids[i]]);
+    }
+    if (total == 0) return QXC_OK;
+    if (!a->k || !a->v) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+    DeviceGuard device(ctx->device);
+    if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
+    st = ensure_pages(ctx, kv, a->seq_count, ids.data(), ends.data());
+    if (st == QXC_OK) st = q4_append(ctx, kv, a, a->in_dtype, a->rot_dtype);
+    if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
+      for (int i = 0; i < a->seq_count; ++i) kv->len[ids[i]] = ends[i];
+    return st;
+  });
+}
+
+qxc_status qxc_kv_read_rows(qxc_ctx* ctx, qxc_kv* kv, const qxc_read_rows_args* a) {
+  if (!ctx || !kv || !a) return fail(ctx, QXC_ERR_INVALID_ARG, "null argument");
+  return guarded(ctx, [&]() -> qxc_status {
+    std::vector<int> ids, ends;
+    long long total;
+    qxc_status st = check_rows(ctx, kv, a->layer_begin, a->layer_count, a->seq_count, a->seq_ids, a->begins, a->counts,
+                               &ids, &ends, &total);
+    if (st != QXC_OK) return st;
+    if (!valid_dtype(a->out_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
+    for (int i = 0; i < a->seq_count; ++i)
+      if (kv->paged() && a->counts[i] && kv->pages_for(ends[i]) > kv->mapped[ids[i]])
+        return fail(ctx, QXC_ERR_INVALID_ARG, "slots [%d, %d) are not all mapped (%d pages of %d rows)", a->begins[i],
+                    ends[i], kv->mapped[ids[i]], 1 << kv->page_shift);
+    if (total == 0) return QXC_OK;
+    if (!a->key_out && !a->value_out) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+    DeviceGuard device(ctx->device);
+    if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
+    Q4ReadParams p;
+    p.arena = q4_arena(kv);
+    p.layer_begin = a->layer_begin;
+    p.layer_count = a->layer_count;
+    p.key_out = a->key_out;
+    p.value_out = a->value_out;
+    p.out_dtype = a->out_dtype;
+    p.vec = aligned(a->key_out, 16) && aligned(a->value_out, 16);
+    return each_part(a->seq_count, a->seq_ids, a->begins, a->counts, [&](const Q4Seq* seqs, int n, int first, int tokens) {
+      memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
+      p.n_seq = n;
+      p.token_begin = first;
+      p.token_count = tokens;
+      QXC_CUDA(ctx, launch_q4_read(is_qwen(kv), p, ctx->stream));
+      ctx->launches++;
+      return QXC_OK;
+    });
+  });
+}
+
+qxc_status qxc_attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
+  if (!ctx || !a) return fail(ctx, QXC_ERR_INVALID_ARG, "null argument");
+  return guarded(ctx, [&]() -> qxc_status {
+    if (a->model != QXC_MODEL_GRANITE && a->model != QXC_MODEL_QWEN3)
+      return fail(ctx, QXC_ERR_INVALID_ARG, "unknown model %d", a->model);
+    if (a->dtype != QXC_BF16 && a->dtype != QXC_F16)
+      return fail(ctx, QXC_ERR_UNSUPPORTED, "packed attention takes bf16 or f16");
+    if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0)
+      return fail(ctx, QXC_ERR_INVALID_ARG, "negative token stride");
+    long long total;
+    qxc_status st = check_lengths(ctx, a->seq_count, a->lengths, &total);
+    if (st != QXC_OK || total == 0) return st;
+    if (!a->q || !a->k || !a->v || !a->out) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+    DeviceGuard device(ctx->device);
+    if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
+    return attend_packed(ctx, a);
+  });
+}
+
+qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed_args* a) {
+  if (!ctx || !kv || !a) return fail(ctx, QXC_ERR_INVALID_ARG, "null argument");
+  return guarded(ctx, [&]() -> qxc_status {
+    long long total;
+    qxc_status st = check_lengths(ctx, a->seq_count, a->lengths, &total);
+    if (st != QXC_OK) return st;
+    if (a->dtype != QXC_BF16 && a->dtype != QXC_F16)
+      return fail(ctx, QXC_ERR_UNSUPPORTED, "packed prefill takes bf16 or f16");
+    if (total && (!a->q || !a->k || !a->v || !a->out)) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+    if (total && (!aligned(a->v, 16) || !aligned(a->out, 16) || a->v_stride % 8))
+      return fail(ctx, QXC_ERR_INVALID_ARG, "v and out must be 16-byte aligned, v's token stride a multiple of 8");
+    if (a->v_stride && a->v_stride < (long long)kv->hkv * kv->d)
+      return fail(ctx, QXC_ERR_INVALID_ARG, "a token stride is shorter than a token's heads");
+    DeviceGuard device(ctx->device);
+    if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
+    const size_t qn = (size_t)total * kv->hq * kv->d, kn = (size_t)total * kv->hkv * kv->d;
+    st = reserve(ctx, &ctx->packed_rot, 2 * (qn + kn));
+    if (st != QXC_OK) return st;
+    std::vector<int32_t> zeros(a->seq_count, 0);
+    qxc_append_args ap;
+    memset(&ap, 0, sizeof(ap));
+    ap.layer_begin = a->layer;
+    ap.layer_count = 1;
+    ap.seq_count = a->seq_count;
+    ap.seq_ids = a->seq_ids;
+    ap.positions = zeros.data();
+    ap.counts = a->lengths;
+    ap.q = a->q;
+    ap.k = a->k;
+    ap.v = a->v;
+    ap.q_rot = total ? ctx->packed_rot.ptr : nullptr;
+    ap.k_rot = total ? ctx->packed_rot.ptr + 2 * qn : nullptr;
+    ap.q_stride = a->q_stride;
+    ap.k_stride = a->k_stride;
+    ap.v_stride = a->v_stride;
+    ap.q_norm = a->q_norm;
+    ap.k_norm = a->k_norm;
+    ap.in_dtype = ap.rot_dtype = a->dtype;
+    ap.flags = a->flags;
+    st = qxc_kv_append(ctx, kv, &ap);
+    if (st != QXC_OK || total == 0) return st;
+    qxc_packed_args pa;
+    memset(&pa, 0, sizeof(pa));
+    pa.model = kv->desc.model;
+    pa.seq_count = a->seq_count;
+    pa.lengths = a->lengths;
+    pa.q = ap.q_rot;
+    pa.k = ap.k_rot;
+    pa.v = a->v;
+    pa.out = a->out;
+    pa.v_stride = a->v_stride;
+    pa.dtype = a->dtype;
+    return attend_packed(ctx, &pa);
+  });
 }
 
 // ---- commitments -----------------------------------------------------------------

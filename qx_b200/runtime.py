@@ -24,7 +24,8 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import BF16, F16, F32, HASH_AUTO, HASH_PER_CHUNK, HASH_PER_SLOT, MODEL_GRANITE, MODEL_QWEN3  # noqa: F401
+from ._lib import (BF16, DECODE_NO_ADVANCE, F16, F32, HASH_AUTO, HASH_PER_CHUNK, HASH_PER_SLOT, MODEL_GRANITE,  # noqa: F401
+                   MODEL_QWEN3, Q4)
 
 HIDDEN, ATTENTION_HEADS, KV_HEADS, HEAD_DIM, MAX_CONTEXT, LAYERS = 1024, 16, 8, 64, 4096, 24  # qx-model lib.rs:9-17
 ATTENTION_MULTIPLIER = 0.015625  # qx-model lib.rs:20
@@ -52,6 +53,29 @@ def _ptr(x) -> int | None:
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot take a pointer of {type(x)}")
+
+
+def _i32(values):
+    """A host int32 array of `values`, or None."""
+    return None if values is None else (C.c_int32 * len(values))(*values)
+
+
+def _token_stride(x, features: int) -> int:
+    """Elements between the tokens of a tensor [tokens, ...] whose remaining
+    dimensions are dense and hold `features` elements; 0 (dense) for a raw
+    pointer."""
+    if x is None or isinstance(x, int) or not hasattr(x, "stride"):
+        return 0
+    shape, stride, dense = tuple(x.shape), tuple(x.stride()), 1
+    for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if n != 1 and s != dense:
+            raise QxError(_lib.ERR_INVALID_ARG, f"the heads of a token must be dense: strides {stride}")
+        dense *= n
+    if dense != features:
+        raise QxError(_lib.ERR_INVALID_ARG, f"a token of shape {shape[1:]} must hold {features} elements")
+    if shape[0] > 1 and stride[0] < features:
+        raise QxError(_lib.ERR_INVALID_ARG, f"the tokens of a tensor must not overlap: strides {stride}")
+    return stride[0] if shape[0] > 1 else 0
 
 
 class Context:
@@ -131,6 +155,17 @@ class Context:
             self.handle, x.ctypes.data_as(C.c_void_p), int(x.size), out.ctypes.data_as(C.c_void_p)))
         return [tuple(int(v) for v in row) for row in out]
 
+    def attend_packed(self, model: int, q, k, v, out, lengths, dtype: int = BF16) -> None:
+        """Causal grouped-query attention of prompts packed one after another
+        (qxc_attend_packed): q, k (both already rotated) and v are device
+        tensors [tokens, ...] of `dtype`, their token strides taken from the
+        tensors; out is dense."""
+        hq, hkv, d = model_shape(model)
+        n = _i32(lengths)
+        a = _lib.PackedArgs(model, len(lengths), n, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _token_stride(q, hq * d),
+                            _token_stride(k, hkv * d), _token_stride(v, hkv * d), dtype)
+        self.check(self.lib.qxc_attend_packed(self.handle, C.byref(a)))
+
     def lse_merge(self, model: int, n_parts: int, partials, out, out_dtype: int = F32) -> None:
         self.check(self.lib.qxc_lse_merge(self.handle, model, n_parts, _ptr(partials), _ptr(out), out_dtype))
 
@@ -200,7 +235,11 @@ def model_shape(model: int):
 
 
 def _np_dtype(dtype: int):
-    return np.float32 if dtype == F32 else np.uint16
+    return np.float32 if dtype == F32 else np.uint8 if dtype == Q4 else np.uint16
+
+
+def _typestr(dtype: int) -> str:
+    return {F32: "<f4", Q4: "|u1"}.get(dtype, "<i2")
 
 
 class KvArena:
@@ -228,6 +267,8 @@ class KvArena:
         self.model, self.layers, self.sequences, self.capacity = model, layers, sequences, capacity
         self.key_dtype, self.value_dtype, self.first_position = key_dtype, value_dtype, first_position
         self.hq, self.hkv, self.d = model_shape(model)
+        # one position's keys (or values): [kv_heads][head_dim], or the bytes of a 4-bit row
+        self.row_shape = (self.hkv * self.d * 9 // 16,) if key_dtype == Q4 else (self.hkv, self.d)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -258,15 +299,16 @@ class KvArena:
 
     def pool_tensor(self, key: bool = True):
         """Zero-copy torch view [layers][pool_pages][page_size][kv_heads][head_dim]
-        of a paged arena's key (or value) pool (int16 for 16-bit storage)."""
+        of a paged arena's key (or value) pool (int16 for 16-bit storage; a
+        4-bit arena's rows as bytes, [...][288])."""
         import torch
         p, n = C.c_void_p(), C.c_size_t()
         self.ctx.check(self.lib.qxc_kv_pool_buffer(self.handle, 1 if key else 0, C.byref(p), C.byref(n)))
         dt = self.key_dtype if key else self.value_dtype
-        shape = (self.layers, self.paging.pool_pages, self.paging.page_size, self.hkv, self.d)
+        shape = (self.layers, self.paging.pool_pages, self.paging.page_size, *self.row_shape)
 
         class _View:
-            __cuda_array_interface__ = {"shape": shape, "typestr": "<f4" if dt == F32 else "<i2",
+            __cuda_array_interface__ = {"shape": shape, "typestr": _typestr(dt),
                                         "data": (p.value, False), "version": 3, "strides": None}
         return torch.as_tensor(_View(), device=f"cuda:{self.ctx.device}")
 
@@ -301,20 +343,20 @@ class KvArena:
 
     def tensor(self, seq: int, layer: int, key: bool = True):
         """Zero-copy torch view [capacity][kv_heads][head_dim] of one cache
-        (int16 for 16-bit storage), through __cuda_array_interface__."""
+        (int16 for 16-bit storage; a 4-bit arena's rows as bytes,
+        [capacity][288]), through __cuda_array_interface__."""
         import torch
         ptr, nbytes = self.key_buffer(seq, layer) if key else self.value_buffer(seq, layer)
         dt = self.key_dtype if key else self.value_dtype
-        typestr = "<f4" if dt == F32 else "<i2"
 
         class _View:
-            __cuda_array_interface__ = {"shape": (self.capacity, self.hkv, self.d), "typestr": typestr,
+            __cuda_array_interface__ = {"shape": (self.capacity, *self.row_shape), "typestr": _typestr(dt),
                                         "data": (ptr, False), "version": 3, "strides": None}
         return torch.as_tensor(_View(), device=f"cuda:{self.ctx.device}")
 
     def read(self, seq: int, layer: int, begin: int, count: int):
-        k = np.zeros((count, self.hkv, self.d), _np_dtype(self.key_dtype))
-        v = np.zeros((count, self.hkv, self.d), _np_dtype(self.value_dtype))
+        k = np.zeros((count, *self.row_shape), _np_dtype(self.key_dtype))
+        v = np.zeros((count, *self.row_shape), _np_dtype(self.value_dtype))
         self.ctx.check(self.lib.qxc_kv_read(self.handle, seq, layer, begin, count, k.ctypes.data, v.ctypes.data))
         return k, v
 
@@ -329,6 +371,55 @@ class KvArena:
                                              None if values is None else values.ctypes.data))
 
     # compute
+    def _default_dtype(self) -> int:
+        """Input type of a decode call that names none."""
+        if self.key_dtype == Q4:
+            return BF16 if self.model == MODEL_QWEN3 else F32
+        return self.key_dtype if self.model == MODEL_QWEN3 else F32
+
+    def append(self, q, k, v, positions, counts, seq_ids=None, layer_begin: int = 0, layer_count: int | None = None,
+               in_dtype: int | None = None, q_rot=None, k_rot=None, rot_dtype: int = BF16, q_norm=None, k_norm=None,
+               flags: int = 0) -> None:
+        """Write the rows of counts[i] new tokens of each sequence, packed one
+        after another, into a 4-bit arena and rotate their queries into q_rot
+        (qxc_kv_append); device tensors [tokens, layer_count, ...] whose token
+        strides are taken from the tensors. q and q_rot may both be None; k_rot
+        receives the rotated keys before quantisation."""
+        layer_count = self.layers - layer_begin if layer_count is None else layer_count
+        if len(counts) != len(positions) or (seq_ids is not None and len(seq_ids) != len(positions)):
+            raise QxError(_lib.ERR_INVALID_ARG, "positions, counts and seq_ids differ in length")
+        qn, kn = layer_count * self.hq * self.d, layer_count * self.hkv * self.d
+        a = _lib.AppendArgs(layer_begin, layer_count, len(positions), _i32(seq_ids), _i32(positions), _i32(counts),
+                            _ptr(q), _ptr(k), _ptr(v), _ptr(q_rot), _ptr(k_rot), _token_stride(q, qn),
+                            _token_stride(k, kn), _token_stride(v, kn), _ptr(q_norm), _ptr(k_norm),
+                            self._default_dtype() if in_dtype is None else in_dtype, rot_dtype, flags)
+        self.ctx.check(self.lib.qxc_kv_append(self.ctx.handle, self.handle, C.byref(a)))
+
+    def read_rows(self, key_out, value_out, begins, counts, seq_ids=None, layer_begin: int = 0,
+                  layer_count: int | None = None, out_dtype: int = F32) -> None:
+        """Rows [begins[i], begins[i] + counts[i]) of each sequence of a 4-bit
+        arena as values, packed into the device tensors key_out and value_out
+        [tokens][layer_count][kv_heads][head_dim] (qxc_kv_read_rows)."""
+        layer_count = self.layers - layer_begin if layer_count is None else layer_count
+        if len(counts) != len(begins) or (seq_ids is not None and len(seq_ids) != len(begins)):
+            raise QxError(_lib.ERR_INVALID_ARG, "begins, counts and seq_ids differ in length")
+        a = _lib.ReadRowsArgs(layer_begin, layer_count, len(begins), _i32(seq_ids), _i32(begins), _i32(counts),
+                              _ptr(key_out), _ptr(value_out), out_dtype)
+        self.ctx.check(self.lib.qxc_kv_read_rows(self.ctx.handle, self.handle, C.byref(a)))
+
+    def prefill_packed(self, q, k, v, out, lengths, seq_ids=None, layer: int = 0, dtype: int = BF16, q_norm=None,
+                       k_norm=None, flags: int = 0) -> None:
+        """Prefill of prompts packed one after another into empty sequences of
+        one layer of a 4-bit arena (qxc_prefill_packed); device tensors
+        [tokens, ...] of `dtype`, token strides taken from the tensors."""
+        if seq_ids is not None and len(seq_ids) != len(lengths):
+            raise QxError(_lib.ERR_INVALID_ARG, "lengths and seq_ids differ in length")
+        qn, kn = self.hq * self.d, self.hkv * self.d
+        a = _lib.PrefillPackedArgs(layer, len(lengths), _i32(seq_ids), _i32(lengths), _ptr(q), _ptr(k), _ptr(v),
+                                   _ptr(out), _token_stride(q, qn), _token_stride(k, kn), _token_stride(v, kn),
+                                   _ptr(q_norm), _ptr(k_norm), dtype, flags)
+        self.ctx.check(self.lib.qxc_prefill_packed(self.ctx.handle, self.handle, C.byref(a)))
+
     def _decode_args(self, q, k, v, out, positions, layer_begin, layer_count, seq_ids, q_dtype, in_dtype,
                      out_dtype, flags, split, q_rot_out, q_norm, k_norm):
         n = len(positions)
@@ -345,7 +436,7 @@ class KvArena:
                split: int = 0, q_rot_out=None, q_norm=None, k_norm=None) -> None:
         """Asynchronous decode step on device tensors (qxc_decode)."""
         layer_count = self.layers - layer_begin if layer_count is None else layer_count
-        dflt = self.key_dtype if self.model == MODEL_QWEN3 else F32
+        dflt = self._default_dtype()
         a = self._decode_args(q, k, v, out, positions, layer_begin, layer_count, seq_ids,
                               dflt if q_dtype is None else q_dtype, dflt if in_dtype is None else in_dtype,
                               out_dtype, flags, split, q_rot_out, q_norm, k_norm)
@@ -412,7 +503,7 @@ class KvArena:
                     out: np.ndarray | None = None, q_norm=None, k_norm=None) -> np.ndarray:
         """Synchronous decode step on host arrays (qxc_decode_host)."""
         layer_count = self.layers - layer_begin if layer_count is None else layer_count
-        dflt = self.key_dtype if self.model == MODEL_QWEN3 else F32
+        dflt = self._default_dtype()
         q_dtype = dflt if q_dtype is None else q_dtype
         in_dtype = dflt if in_dtype is None else in_dtype
         units = len(positions) * layer_count
@@ -515,12 +606,13 @@ def apply_granite_rope(query: np.ndarray, key: np.ndarray, position: int, ctx: C
 
 # ---- qx-runtime-v2 KV plan mirror ------------------------------------------------
 class KvPrecision(enum.Enum):
-    """qx_format::KvPrecision (crates/qx-format/src/lib.rs:136-141) plus bf16 for B200."""
+    """qx_format::KvPrecision (crates/qx-format/src/lib.rs:136-141) plus bf16 and 4 bits for B200."""
     Fp32 = (F32, F32)
     Fp32KFp16V = (F32, F16)
     Fp16KFp32V = (F16, F32)
     Fp16 = (F16, F16)
     Bf16 = (BF16, BF16)
+    Q4 = (Q4, Q4)
 
 
 @dataclass

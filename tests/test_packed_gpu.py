@@ -1,0 +1,269 @@
+"""Packed prompts: causal attention against 64 bits, and prompt, cache and
+decode as a serving step runs them.
+
+Tolerances. The weights of a key tile are rounded to the input type for their
+product with the values (half a step of it) and come from a base-2 exponential
+with a relative error of at most 2^-13; a logit error enters twice (numerator
+and sum); the sum of a row's weights in f32 adds its length in roundings.
+"""
+import numpy as np
+import pytest
+import torch
+
+import q4_reference as ref
+from qx_b200 import BF16, F16, F32, MODEL_GRANITE, MODEL_QWEN3, Q4, KvArena, QxError, _lib
+from qx_b200.runtime import model_shape
+from test_q4_gpu import check_decode, host, norms, stored, tensor
+
+pytestmark = pytest.mark.gpu
+MODELS = [MODEL_GRANITE, MODEL_QWEN3]
+
+
+def inputs(rng, model, total, dtype, fused=False):
+    hq, hkv, d = model_shape(model)
+    if fused:
+        joint = tensor(rng, (total, hq + 2 * hkv, d), dtype, 1.2)
+        return joint[:, :hq], joint[:, hq:hq + hkv], joint[:, hq + hkv:]
+    return tensor(rng, (total, hq, d), dtype, 1.5), tensor(rng, (total, hkv, d), dtype), tensor(rng, (total, hkv, d), dtype)
+
+
+def check(model, q, k, v, out, lengths, dtype, heads=None):
+    """Every row of `out` against 64 bits (on the GPU: prompts may be long)."""
+    hq, hkv, d = model_shape(model)
+    begin = 0
+    for n in lengths:
+        rows = slice(begin, begin + n)
+        begin += n
+        for h in heads or range(hq):
+            kd, vd = k[rows, h * hkv // hq].double(), v[rows, h * hkv // hq].double()
+            qd = q[rows, h].double()
+            for at in range(0, n, 1024):
+                part = qd[at:at + 1024]
+                seen = at + part.shape[0]
+                later = torch.arange(seen, device="cuda") > torch.arange(at, seen, device="cuda")[:, None]
+                logits = (part @ kd[:seen].T * ref.SCALE[model]).masked_fill(later, -torch.inf)
+                p = torch.softmax(logits, -1)
+                want, mean = p @ vd[:seen], p @ vd[:seen].abs()
+                # products are exact in f32, D of them summed in f32
+                size = (part.abs() @ kd[:seen].abs().T).masked_fill(later, 0).amax(-1, keepdim=True) * ref.SCALE[model]
+                rel = 2 * size * (d + 2) * 2.0 ** -24 + ref.HALF_STEP[dtype] + 2.0 ** -13 + seen * 2.0 ** -24
+                tol = ref.HALF_STEP[dtype] * want.abs() + rel * mean + 1e-30
+                got = out[rows, h][at:seen].double()
+                assert torch.isfinite(got).all()
+                assert float(((got - want).abs() / tol).max()) <= 1, (n, h, at)
+
+
+def attend(ctx, model, q, k, v, lengths, dtype, extra=0):
+    hq, _, d = model_shape(model)
+    out = torch.full((q.shape[0] + extra, hq, d), 5.0, device="cuda", dtype=ref.TORCH[dtype])
+    ctx.attend_packed(model, q, k, v, out, lengths, dtype=dtype)
+    ctx.sync()
+    assert (out[sum(lengths):] == 5.0).all()
+    return out
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 400])
+def test_one_prompt(gpu_ctx, model, n):
+    rng = np.random.default_rng([model, n])
+    for dtype in (BF16, F16):
+        q, k, v = inputs(rng, model, n, dtype)
+        check(model, q, k, v, attend(gpu_ctx, model, q, k, v, [n], dtype, 2), [n], dtype)
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths", [[3, 0, 1, 130, 64, 0, 257, 1], [0, 0, 5], [100, 28, 128, 128], [1] * 40])
+def test_packed_prompts(gpu_ctx, model, dtype, lengths):
+    rng = np.random.default_rng([model, dtype, len(lengths)])
+    q, k, v = inputs(rng, model, sum(lengths), dtype, fused=True)
+    check(model, q, k, v, attend(gpu_ctx, model, q, k, v, lengths, dtype, 3), lengths, dtype)
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_more_prompts_than_a_launch_holds(gpu_ctx, model):
+    rng = np.random.default_rng(3)
+    lengths = [int(x) for x in rng.integers(0, 9, 450)]
+    q, k, v = inputs(rng, model, sum(lengths), BF16)
+    check(model, q, k, v, attend(gpu_ctx, model, q, k, v, lengths, BF16), lengths, BF16)
+
+
+def test_no_tokens(gpu_ctx):
+    launches = gpu_ctx.launch_count
+    out = torch.full((2, 16, 64), 5.0, device="cuda", dtype=torch.bfloat16)
+    gpu_ctx.attend_packed(MODEL_GRANITE, None, None, None, out, [0, 0])
+    gpu_ctx.sync()
+    assert gpu_ctx.launch_count == launches and (out == 5.0).all()
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_a_row_does_not_attend_does_not_reach_it(gpu_ctx, model, bad):
+    """A bad key and value at token 90 of prompt 1: rows of other prompts and
+    the 90 rows before it are as without it, the rows from it on are not finite."""
+    rng = np.random.default_rng(4)
+    lengths = [70, 200, 50]
+    q, k, v = inputs(rng, model, sum(lengths), BF16)
+    clean = attend(gpu_ctx, model, q, k, v, lengths, BF16)
+    at = lengths[0] + 90
+    rest = torch.cat([torch.arange(at), torch.arange(270, 320)]).cuda()
+    for side in (k, v):
+        keep = side[at].clone()
+        side[at] = bad
+        out = torch.zeros_like(clean)
+        gpu_ctx.attend_packed(model, q, k, v, out, lengths, dtype=BF16)
+        with pytest.raises(QxError) as e:
+            gpu_ctx.sync()
+        assert e.value.status == _lib.ERR_NONFINITE
+        side[at] = keep
+        if side is v:
+            assert not torch.isfinite(out[at:270]).any()
+        check(model, q[:at], k[:at], v[:at], out[:at], [70, 90], BF16)
+        check(model, q[270:], k[270:], v[270:], out[270:], [50], BF16)
+        assert torch.equal(out[270:], clean[270:]) and torch.equal(out[:70], clean[:70]) and rest.numel() == at + 50
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("scale", [0.0, 30.0])
+def test_flat_and_peaked_scores(gpu_ctx, model, scale):
+    rng = np.random.default_rng(5)
+    q, k, v = inputs(rng, model, 300, F16)
+    q = q * scale
+    check(model, q, k, v, attend(gpu_ctx, model, q, k, v, [300], F16), [300], F16)
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_rising_scores(gpu_ctx, model):
+    """Each key scores higher than all before it: the running maximum moves in every tile."""
+    rng = np.random.default_rng(6)
+    q, k, v = inputs(rng, model, 700, F16)
+    q[:] = 1.0
+    k[:] = (torch.arange(700, device="cuda") / (25.0 if model == MODEL_GRANITE else 70.0))[:, None, None].half()
+    check(model, q, k, v, attend(gpu_ctx, model, q, k, v, [700], F16), [700], F16)
+
+
+@pytest.mark.parametrize("model,lengths", [(MODEL_GRANITE, [2500, 1100]), (MODEL_QWEN3, [3001])])
+def test_long_prompts(gpu_ctx, model, lengths):
+    rng = np.random.default_rng(7)
+    q, k, v = inputs(rng, model, sum(lengths), BF16, fused=True)
+    hq = model_shape(model)[0]
+    check(model, q, k, v, attend(gpu_ctx, model, q, k, v, lengths, BF16), lengths, BF16, heads=[0, hq // 2 + 1, hq - 1])
+
+
+def test_captured_and_replayed(gpu_ctx):
+    rng = np.random.default_rng(8)
+    lengths = [130, 1, 300]
+    q, k, v = inputs(rng, MODEL_QWEN3, sum(lengths), BF16, fused=True)
+    out = torch.zeros(sum(lengths), 32, 128, device="cuda", dtype=torch.bfloat16)
+    old, stream = gpu_ctx.stream, torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        gpu_ctx.set_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            gpu_ctx.attend_packed(MODEL_QWEN3, q, k, v, out, lengths)
+        for _ in range(2):
+            q.copy_(tensor(rng, q.shape, BF16, 1.5))
+            out.zero_()
+            graph.replay()
+            stream.synchronize()
+            check(MODEL_QWEN3, q, k, v, out, lengths, BF16, heads=[0, 17])
+    gpu_ctx.set_stream(old)
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("page", [0, 64])
+def test_prompt_then_decode(gpu_ctx, model, page):
+    """Packed prompts into two layers, then three decode steps over the rows they wrote."""
+    rng = np.random.default_rng([model, page, 9])
+    hq, hkv, d = model_shape(model)
+    qw, kw = norms(rng, model)
+    lengths, ids = [37, 0, 129, 1], [2, 0, 1, 3]
+    cap = max(lengths) + 3
+    arena = KvArena(gpu_ctx, model, 2, 4, cap, Q4, page_size=page, pool_pages=9 if page else 0)
+    for layer in range(2):
+        q, k, v = inputs(rng, model, sum(lengths), BF16, fused=True)
+        out = torch.zeros(sum(lengths), hq, d, device="cuda", dtype=torch.bfloat16)
+        arena.prefill_packed(q, k, v, out, lengths, seq_ids=ids, layer=layer, q_norm=qw, k_norm=kw,
+                             flags=_lib.DECODE_NO_ADVANCE if layer == 0 else 0)
+        gpu_ctx.sync()
+        begin = 0
+        for i, n in zip(ids, lengths):
+            rows = slice(begin, begin + n)
+            begin += n
+            if not n:
+                continue
+            qr, kr = (torch.from_numpy(ref.rotate64(model, host(x[rows]), range(n), None if w is None else host(w)))
+                      for x, w in ((q, qw), (k, kw)))
+            # the attention reads the rotated rows rounded to bf16
+            check_rounded(model, qr, kr, v[rows], out[rows])
+            (kc, ks), (vc, vs) = stored(arena, i, layer, 0, n)
+            want = ref.quantise(v[rows].float().cpu().numpy())
+            assert np.array_equal(vc, want[0]) and np.array_equal(vs, want[1])
+            # half a code step, and the two roundings a scale and the f32 row add to it
+            err = np.abs(ref.values(kc, ks) - kr.numpy()).reshape(*ks.shape, 32)
+            assert (err <= 0.5 * ks.astype(np.float64)[..., None] * (1 + 2.0 ** -7) + 1e-6).all()
+    assert [arena.len(i) for i in ids] == lengths
+    for step in range(3):
+        positions = [n + step for n in lengths]
+        q, k, v = (tensor(rng, (4, 2, h, d), BF16) for h in (hq, hkv, hkv))
+        out = torch.zeros(4, 2, hq, d, device="cuda")
+        arena.decode(q, k, v, out, positions, seq_ids=ids, q_dtype=BF16, in_dtype=BF16, q_norm=qw, k_norm=kw)
+        gpu_ctx.sync()
+        check_decode(gpu_ctx, arena, q, k, v, out, positions, F32, qw, kw, ids)
+    arena.close()
+
+
+def check_rounded(model, q, k, v, out):
+    """`out` of a prefill against 64 bits: its rotated queries and keys are
+    rounded to bf16 (one step of 2^-8 each), which moves a logit by at most
+    that share of |q|.|k|."""
+    hq, hkv, d = model_shape(model)
+    v, out, n = v.double().cpu(), out.double().cpu(), q.shape[0]
+    later = torch.arange(n) > torch.arange(n)[:, None]
+    for h in range(hq):
+        kd, vd = k[:, h * hkv // hq], v[:, h * hkv // hq]
+        p = torch.softmax((q[:, h] @ kd.T * ref.SCALE[model]).masked_fill(later, -torch.inf), -1)
+        want, mean = p @ vd, p @ vd.abs()
+        size = (q[:, h].abs() @ kd.abs().T).masked_fill(later, 0).amax(-1, keepdim=True) * ref.SCALE[model]
+        rel = torch.expm1(2 * size * (2 * 2.0 ** -8 + (d + 16) * 2.0 ** -24)) + 2.0 ** -8 + 2.0 ** -13 + n * 2.0 ** -24
+        assert float(((out[:, h] - want).abs() / (2.0 ** -8 * want.abs() + rel * mean + 1e-30)).max()) <= 1
+
+
+def test_refusals(gpu_ctx):
+    bad, unsupported = _lib.ERR_INVALID_ARG, _lib.ERR_UNSUPPORTED
+    q, k = (torch.zeros(64, h, 64, device="cuda", dtype=torch.bfloat16) for h in (16, 8))
+
+    def refused(status, call):
+        launches = gpu_ctx.launch_count
+        with pytest.raises(QxError) as e:
+            call()
+        assert e.value.status == status and gpu_ctx.launch_count == launches and str(e.value)
+    go = lambda *a, **kw: gpu_ctx.attend_packed(kw.pop("model", MODEL_GRANITE), *a, **kw)  # noqa: E731
+    refused(bad, lambda: go(q, k, k, q, []))
+    refused(bad, lambda: go(q, k, k, q, [3, -1]))
+    refused(bad, lambda: go(q, k, k, q, [2 ** 24, 1]))
+    refused(bad, lambda: go(q, k, None, q, [3]))
+    refused(bad, lambda: go(q, q, k, q, [3]))
+    refused(bad, lambda: go(q.transpose(0, 1), k, k, q, [3]))
+    refused(unsupported, lambda: go(q, k, k, q, [3], dtype=F32))
+    refused(unsupported, lambda: go(q, k, k, q, [3], dtype=Q4))
+    flat = torch.zeros(64 * 1024 + 8, device="cuda", dtype=torch.bfloat16)
+    refused(bad, lambda: go(flat[1:1 + 64 * 1024].view(64, 16, 64), k, k, q, [3]))
+    refused(bad, lambda: go(q, k, k, flat[1:1 + 64 * 1024].view(64, 16, 64), [3]))
+    odd = torch.as_strided(flat, (50, 16, 64), (1028, 64, 1))
+    refused(bad, lambda: go(odd, k, k, q, [3]))
+    arena = KvArena(gpu_ctx, MODEL_GRANITE, 1, 2, 16, Q4)
+    pre = lambda lengths, a=arena, **kw: a.prefill_packed(q, k, k, q.clone(), lengths, **kw)  # noqa: E731
+    refused(_lib.ERR_POSITION, lambda: pre([17]))
+    refused(bad, lambda: pre([1, 1], seq_ids=[0, 0]))
+    refused(bad, lambda: pre([1, 1, 1]))
+    refused(bad, lambda: pre([1], layer=1))
+    refused(unsupported, lambda: pre([1], dtype=F32))
+    plain = KvArena(gpu_ctx, MODEL_GRANITE, 1, 2, 16, BF16)
+    refused(unsupported, lambda: pre([1], plain))
+    pre([3, 2])
+    refused(_lib.ERR_POSITION, lambda: pre([3, 2]))
+    gpu_ctx.sync()
+    arena.close()
+    plain.close()

@@ -1,0 +1,84 @@
+"""Host-only checks of 4-bit arenas and packed prompts: memory plan, argument
+checks that need no device, the token strides the Python layer derives."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import q4_reference as ref
+from qx_b200 import MODEL_GRANITE, MODEL_QWEN3, KvPrecision, ExecutionPlan, QxError, _lib
+from qx_b200.runtime import _token_stride
+
+
+def kv_bytes(desc):
+    lib, kb, vb = _lib.load(), C.c_size_t(), C.c_size_t()
+    return lib.qxc_kv_bytes(C.byref(desc), C.byref(kb), C.byref(vb)), kb.value, vb.value
+
+
+@pytest.mark.parametrize("model,capacity", [(MODEL_GRANITE, 4096), (MODEL_QWEN3, 40960)])
+def test_a_4bit_row_is_288_bytes(model, capacity):
+    st, kb, vb = kv_bytes(_lib.KvDesc(model, 3, 5, capacity, _lib.Q4, _lib.Q4, 0))
+    assert st == _lib.OK and kb == vb == 3 * 5 * capacity * 288
+    lib, k2, v2 = _lib.load(), C.c_size_t(), C.c_size_t()
+    d, pg = _lib.KvDesc(model, 3, 5, capacity, _lib.Q4, _lib.Q4, 0), _lib.KvPaging(64, 11)
+    assert lib.qxc_kv_paged_bytes(C.byref(d), C.byref(pg), C.byref(k2), C.byref(v2)) == _lib.OK
+    assert k2.value == v2.value == 3 * 11 * 64 * 288
+
+
+def test_execution_plan_in_4_bits():
+    plan = ExecutionPlan.granite_with_kv_precision(512, KvPrecision.Q4)
+    assert plan.kv_bytes == 24 * 512 * 2 * 288
+
+
+@pytest.mark.parametrize("desc,status", [
+    (_lib.KvDesc(0, 1, 1, 16, _lib.Q4, _lib.F16, 0), _lib.ERR_UNSUPPORTED),
+    (_lib.KvDesc(0, 1, 1, 16, _lib.F32, _lib.Q4, 0), _lib.ERR_UNSUPPORTED),
+    (_lib.KvDesc(1, 1, 1, 16, _lib.BF16, _lib.Q4, 0), _lib.ERR_UNSUPPORTED),
+    (_lib.KvDesc(1, 1, 1, 16, _lib.Q4, _lib.Q4, 64), _lib.ERR_UNSUPPORTED),
+    (_lib.KvDesc(0, 1, 1, 4097, _lib.Q4, _lib.Q4, 0), _lib.ERR_INVALID_ARG),
+    (_lib.KvDesc(1, 1, 1, 40961, _lib.Q4, _lib.Q4, 0), _lib.ERR_INVALID_ARG),
+])
+def test_descriptors_refused(desc, status):
+    assert kv_bytes(desc)[0] == status
+
+
+def test_null_arguments():
+    lib = _lib.load()
+    assert lib.qxc_kv_append(None, None, None) == _lib.ERR_INVALID_ARG
+    assert lib.qxc_kv_read_rows(None, None, None) == _lib.ERR_INVALID_ARG
+    assert lib.qxc_attend_packed(None, None) == _lib.ERR_INVALID_ARG
+    assert lib.qxc_prefill_packed(None, None, None) == _lib.ERR_INVALID_ARG
+
+
+def test_token_strides():
+    x = torch.zeros(10, 24, 64)
+    assert _token_stride(x, 24 * 64) == 24 * 64
+    assert _token_stride(x[:, :16], 16 * 64) == 24 * 64  # part of a joint projection
+    assert _token_stride(x[::2], 24 * 64) == 2 * 24 * 64
+    assert _token_stride(x[:1, :16], 16 * 64) == 0       # one token: any stride
+    assert _token_stride(None, 5) == 0 and _token_stride(4096, 5) == 0
+    for bad, features in ((x[:, :, ::2], 24 * 32), (x.transpose(1, 2), 24 * 64), (x, 64),
+                          (x[:1].expand(10, 24, 64), 24 * 64), (x[:, ::2], 12 * 64)):
+        with pytest.raises(QxError):
+            _token_stride(bad, features)
+
+
+@pytest.mark.parametrize("model", [MODEL_GRANITE, MODEL_QWEN3])
+@pytest.mark.parametrize("key", [True, False])
+def test_the_stated_layout_uses_every_nibble_once(model, key):
+    rng = np.random.default_rng(1)
+    raw = rng.integers(0, 256, (3, 288), dtype=np.uint8)
+    codes, _ = ref.unpack_rows(model, raw, key)
+    nibbles = np.stack([raw[:, :256] & 15, raw[:, :256] >> 4], -1).reshape(3, -1)
+    assert np.array_equal(np.sort(codes.reshape(3, -1), 1), np.sort(nibbles, 1))
+
+
+def test_reference_quantiser_rounds_ties_to_even_and_keeps_the_largest():
+    x = np.zeros((1, 1, 64), np.float32)
+    x[..., 0] = 7.0
+    x[..., 1:5] = [0.5, 1.5, 2.5, -2.5]
+    codes, scales = ref.quantise(x)
+    assert scales[0, 0].tolist() == [1.0, 0.0]
+    assert codes[0, 0, :5].tolist() == [14, 7, 9, 9, 5]
+    assert (codes[0, 0, 32:] == 7).all()
