@@ -169,20 +169,26 @@ __device__ __forceinline__ void put_key(char* row, int head, int c, uint32_t cod
   if ((c & 3) == 0) *reinterpret_cast<__half*>(row + Q4Row<M>::scale(head, c >> 2)) = scale;
 }
 
-// Store this lane's codes and scale as part of a value row: nibble i of half
-// g comes from lane t = i of the group, which holds dims 8 i + g.
-template <class M>
-__device__ __forceinline__ void put_value(char* row, int head, int c, uint32_t codes, __half scale) {
-  const int t = c & 3, j = c >> 2, quad = (threadIdx.x & 31) & ~3;
-  uint32_t lo = 0u, hi = 0u;  // halves g = 2 t and 2 t + 1
+// The halves g = 2 t (low 16 bits) and 2 t + 1 of a value row's group that
+// lane t of a quad stores: nibble i of half g comes from lane i, which holds
+// dims 8 i + g. Every lane of the warp takes part.
+__device__ __forceinline__ uint32_t value_halves(uint32_t codes) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  uint32_t out = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t w = __shfl_sync(0xffffffffu, codes, quad + i) >> (8 * t);
-    lo |= (w & 15u) << (4 * i);
-    hi |= ((w >> 4) & 15u) << (4 * i);
+    const uint32_t w = __shfl_sync(0xffffffffu, codes, (lane & ~3) + i) >> (8 * t);
+    out |= (w & 15u) << (4 * i) | ((w >> 4) & 15u) << (16 + 4 * i);
   }
-  *reinterpret_cast<uint16_t*>(row + Q4Row<M>::value_half(head, j, 2 * t)) = (uint16_t)lo;
-  *reinterpret_cast<uint16_t*>(row + Q4Row<M>::value_half(head, j, 2 * t + 1)) = (uint16_t)hi;
+  return out;
+}
+
+// Store this lane's halves (value_halves) and scale as part of a value row.
+template <class M>
+__device__ __forceinline__ void put_value(char* row, int head, int c, uint32_t halves, __half scale) {
+  const int t = c & 3, j = c >> 2;
+  *reinterpret_cast<uint16_t*>(row + Q4Row<M>::value_half(head, j, 2 * t)) = (uint16_t)halves;
+  *reinterpret_cast<uint16_t*>(row + Q4Row<M>::value_half(head, j, 2 * t + 1)) = (uint16_t)(halves >> 16);
   if (t == 0) *reinterpret_cast<__half*>(row + Q4Row<M>::scale(head, j)) = scale;
 }
 

@@ -67,12 +67,27 @@ struct Q4DecodeParams {
   int layer_begin, layer_count;
   int n_seq;
   int seq_begin;  // index of seqs[0] among the call's sequences
-  const float* q;  // rotated queries [sequence][layer][HQ * D]
-  void* out;       // [sequence][layer][HQ * D]
-  int out_dtype;
+  int chunk;      // cache rows per split, a multiple of kQ4Tile
+  int items;      // (sequence, layer, split) of this launch
+  int split;      // some sequence has several splits: qx_q4_merge_kernel follows
+  const void* q;  // [sequence][layer][HQ * D]
+  const void* k;  // [sequence][layer][HKV * D]
+  const void* v;
+  void* out;         // [sequence][layer][HQ * D]
+  float* q_rot_out;  // rotated queries, or null
+  const float* q_norm;
+  const float* k_norm;
+  const float2* rope;
+  float* part_o;   // partials of split sequences: [item][HQ][D] sums
+  float2* part_ml;  // and [item][HQ] (m, l)
+  int q_dtype, in_dtype, out_dtype;
+  int vec;  // q, k and v allow 16-byte loads
   unsigned* err;
-  Q4Seq seqs[kQ4Seqs];
+  Q4Seq seqs[kQ4Seqs];  // begin: rows attended, the new token's among them; first: first work item
 };
+
+constexpr int kQ4Tile = 64;  // cache rows per pipeline stage; pages hold a multiple of it
+constexpr int kQ4MaxSplits = 1024;
 
 struct PackedParams {
   const void* q;
@@ -89,7 +104,10 @@ struct PackedParams {
 
 cudaError_t launch_q4_append(bool qwen, const Q4AppendParams& p, cudaStream_t stream);
 cudaError_t launch_q4_read(bool qwen, const Q4ReadParams& p, cudaStream_t stream);
-cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream);
+// The decode and, where p.split says so, the merge; the kernels launched.
+cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream, int* launched);
+// Decode CTAs resident on one SM.
+int q4_decode_blocks_per_sm();
 cudaError_t launch_packed(bool qwen, const PackedParams& p, cudaStream_t stream);
 
 }  // namespace qx

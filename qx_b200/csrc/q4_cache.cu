@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads) qx_q4_append_kernel(const __grid_con
       head -= M::HKV;
       load8(p.v, token * p.v_stride + ((long long)l * M::HKV + head) * M::D + 8 * c, p.in_dtype, p.vec, x);
       good = quantise8(x, &codes, &scale);
-      put_value<M>(p.arena.v + row * kQ4RowBytes, head, c, codes, scale);
+      put_value<M>(p.arena.v + row * kQ4RowBytes, head, c, value_halves(codes), scale);
     }
   }
   if (!good) flag_error(p.err, QX_ERR_BIT_NONFINITE);

@@ -1,78 +1,559 @@
-// q4_decode.cu — attention of new tokens over a 4-bit cache.
+// q4_decode.cu — one decode step over a 4-bit cache.
 //
-// First form: a warp takes one query head of one (sequence, layer), a lane
-// D / 32 neighbouring dims, row after row with a running maximum and sum.
+// qx_q4_decode_kernel: a CTA takes one (sequence, layer) and one split of its
+// cached rows, all kv heads at once, so a run of rows is one contiguous piece
+// of memory (288 bytes a row). Eight warps: Granite's eight kv heads, or
+// Qwen's four, two warps each taking half of every tile's rows.
+//   copies   tiles of 64 rows, keys and values, by bulk copies into a ring of
+//            three stages; the last warp to finish a tile refills its stage
+//   scores   S = [Q_hi; Q_lo] K^T by mma.m16n8k16: rows 0-7 are the kv head's
+//            query heads rounded to fp16, rows 8-15 what that rounding left,
+//            so a query counts with 22 bits at no extra product. K's codes
+//            become fp16 in registers and stay integers: each group of 32 dims
+//            has its own accumulator, multiplied by the row's scale in f32.
+//   softmax  in f32, base 2, a running reference m per head and warp
+//   output   O^T += V^T P'^T, V's codes again as integers; P' = P * scale of
+//            (row, group), rounded to fp16 (two fp16 terms when the output is
+//            f32), one operand per group. P falls out of the score
+//            accumulators in exactly the operand layout.
+// The tensor instructions take their operands from registers: 4-bit codes
+// would have to pass through shared memory a second time to reach tcgen05, and
+// the products are a small part of the work (a tile's codes are expanded by
+// more instructions than multiply them).
+//
+// The row order inside a block of 8 (kRow below) makes the quads' loads of
+// neighbouring MMA rows fall into different banks: a row is 72 words, 8 modulo
+// 32, and rows 0, 6, 1, 7, 2, 4, 3, 5 give every 128-byte phase of the key
+// loads, of the value loads and of the scale loads distinct banks.
 #include "q4.cuh"
 
 namespace qx {
 namespace {
 
-template <class M>
-__global__ void __launch_bounds__(128) qx_q4_decode_kernel(const __grid_constant__ Q4DecodeParams p) {
-  using R = Q4Row<M>;
-  constexpr int N = M::D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  pdl_wait();
-  if (w >= (long long)p.n_seq * p.layer_count * M::HQ) return;
-  const int qh = (int)(w % M::HQ), h = qh / M::G;
-  const long long unit = w / M::HQ;
-  const int l = (int)(unit % p.layer_count), i = (int)(unit / p.layer_count);
-  const Q4Seq s = p.seqs[i];
-  const long long base = (((long long)(p.seq_begin + i) * p.layer_count + l) * M::HQ + qh) * M::D;
-  float q[N], o[N], m = -INFINITY, sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    q[e] = p.q[base + N * lane + e];
-    o[e] = 0.0f;
-  }
-  for (int r = 0; r < s.begin; ++r) {
-    const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq, p.layer_begin + l, r);
-    const unsigned char* kr = reinterpret_cast<const unsigned char*>(p.arena.k) + row * kQ4RowBytes;
-    const unsigned char* vr = reinterpret_cast<const unsigned char*>(p.arena.v) + row * kQ4RowBytes;
-    float dot = 0.0f, v[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int d = N * lane + e, j = d >> 5, rr = d & 31;
-      const int kb = R::key_word(h, d >> 3) + ((rr & 7) >> 1);
-      const int kc = (kr[kb] >> (4 * (rr & 1))) & 15;
-      dot += q[e] * (float)(kc - 7) * __half2float(*reinterpret_cast<const __half*>(kr + R::scale(h, j)));
-      const int vb = R::value_half(h, j, rr & 7) + (rr >> 4);
-      const int vc = (vr[vb] >> (4 * ((rr >> 3) & 1))) & 15;
-      v[e] = (float)(vc - 7) * __half2float(*reinterpret_cast<const __half*>(vr + R::scale(h, j)));
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    const float x = dot * M::SCALE, top = fmaxf(m, x), keep = expf(m - top), e0 = expf(x - top);
-    m = top;
-    sum = sum * keep + e0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = o[e] * keep + e0 * v[e];
-  }
-  bool good = true;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float y = o[e] / sum;
-    good &= isfinite(y);
-    store_any(p.out, base + N * lane + e, p.out_dtype, y);
-  }
-  if (!good) flag_error(p.err, QX_ERR_BIT_NONFINITE);
+constexpr int kThreads = 256;
+constexpr int kStages = 3;
+constexpr int kSide = kQ4Tile * kQ4RowBytes;  // bytes of a tile's keys, or values
+constexpr int kStage = 2 * kSide;
+constexpr int kOffBar = kStages * kStage;
+constexpr int kSmem = kOffBar + 8 * kStages + 4 * kStages + 4;
+
+// The largest P' = 2^(x - m) * scale of a step is set to about 2^kTop when the
+// reference m moves, and m moves when it would pass 2^(kTop + kSlack), below
+// fp16's largest: the smaller weights and the groups of smaller scale then keep
+// as much of fp16's range below it as there is.
+constexpr float kTop = 7.0f, kSlack = 8.0f;
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-}  // namespace
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream) {
+// Nibbles 0 and 4 of w (low: bits 0 and 16) as fp16 c - 7: 0x6400 | c is 1024 + c.
+__device__ __forceinline__ uint32_t codes_low(uint32_t w) {
+  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1031.0f));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Nibbles 1 and 5: 0x6400 | 16 c is 1024 + 16 c.
+__device__ __forceinline__ uint32_t codes_high(uint32_t w) {
+  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0.0625f), __float2half2_rn(-71.0f));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Add one to a shared counter; the caller's reads of the stage are ordered
+// before it, those of the others' before the last caller's return.
+__device__ __forceinline__ unsigned count_up(unsigned* counter) {
+  unsigned old;
+  asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;" : "=r"(old) : "r"(smem_addr(counter)) : "memory");
+  return old;
+}
+
+template <int N>
+struct Words {  // N 16-bit halves per row and lane
+  uint32_t w[N / 2];
+  __device__ __forceinline__ void load(const unsigned char* p) {
+    if constexpr (N == 4) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x;
+      w[1] = u.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
+};
+
+template <class M>
+struct Dec {
+  static constexpr int NG = M::D / 32;
+  static constexpr int WPH = 8 / M::HKV;          // warps per kv head
+  static constexpr int ROWS = kQ4Tile / WPH;      // rows of a tile per warp
+  static constexpr int PITCH = M::D + 8;          // floats per head in the closing exchange
+  static constexpr int OFF_STAT = 8 * M::G * PITCH * 4;
+  static_assert(OFF_STAT + 8 * M::G * 8 <= kStages * kStage, "the closing exchange fits the stages");
+};
+
+// The rotated queries of a warp's kv head as MMA operands.
+template <class M, bool PRECISE>
+struct Query {
+  static constexpr int NG = M::D / 32;
+  uint32_t a[NG][2][4];
+  float unit;       // base-2 logit of an accumulator
+};
+
+// Lane (g, t) holds dims 32 j + 8 t .. + 7 of query head g: rotation pairs are
+// in the lane, norms in the quad.
+template <class M, bool PRECISE>
+__device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long unit, int h, int position, bool emit,
+                                           Query<M, PRECISE>* out) {
+  constexpr int NG = M::D / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const bool mine = g < M::G;
+  const long long base = (unit * M::HQ + h * M::G + (mine ? g : 0)) * M::D + 8 * t;
+  float x[NG * 8];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) load8(p.q, base + 32 * j, p.q_dtype, p.vec, x + 8 * j);
+  if constexpr (M::QWEN) {
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < NG * 8; ++e) sum = fma((double)x[e], (double)x[e], sum);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    const float inv = (float)rsqrt(sum * (1.0 / M::D) + 1.0e-6);
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[8 * j + e] = __fmul_rn(__fmul_rn(x[8 * j + e], inv), p.q_norm ? p.q_norm[32 * j + 8 * t + e] : 1.0f);
+  }
+  const float2* tab = p.rope + (long long)position * (M::D / 2) + 8 * t;
+  bool good = true;
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NG / 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float l = x[8 * j + e], r = x[8 * (j + NG / 2) + e];
+      const float2 c = tab[32 * j + e];
+      float a, b;
+      if constexpr (M::QWEN) {
+        a = __fsub_rn(__fmul_rn(l, c.x), __fmul_rn(r, c.y));
+        b = __fadd_rn(__fmul_rn(r, c.x), __fmul_rn(l, c.y));
+      } else {
+        a = __fmaf_rn(-r, c.x, __fmul_rn(l, c.y));
+        b = __fmaf_rn(r, c.y, __fmul_rn(l, c.x));
+      }
+      x[8 * j + e] = a;
+      x[8 * (j + NG / 2) + e] = b;
+      good &= isfinite(a) && isfinite(b);
+      top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
+    }
+  if (emit && mine) {
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p.q_rot_out[base + 32 * j + e] = x[8 * j + e];
+  }
+  // largest element of the head to [2^14, 2^15): fp16 then holds the leading
+  // 11 bits of every element that matters, a second fp16 the next 11
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int ex = max((int)(__float_as_uint(top) >> 23), 15);
+  const float up = __int_as_float((268 - ex) << 23), down = __int_as_float((ex - 14) << 23);
+  out->unit = M::SCALE * 1.4426950408889634f * down;
+#pragma unroll
+  for (int j = 0; j < NG; ++j)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float y0 = mine ? x[8 * j + 2 * u + s] * up : 0.0f, y1 = mine ? x[8 * j + 2 * u + s + 4] * up : 0.0f;
+        const uint32_t hi = pack_half(y0, y1);
+        const float2 back = unpack_half(hi);
+        out->a[j][u][2 * s] = hi;
+        out->a[j][u][2 * s + 1] = pack_half(y0 - back.x, y1 - back.y);
+      }
+  return good;
+}
+
+template <class M, bool PRECISE>
+__global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_constant__ Q4DecodeParams p) {
+  using C = Dec<M>;
+  using R = Q4Row<M>;
+  constexpr int NG = C::NG;
+  extern __shared__ __align__(128) unsigned char sm[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + kOffBar);
+  unsigned* done = reinterpret_cast<unsigned*>(full + kStages);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int h = warp / C::WPH, half = warp % C::WPH;
+  const int i = find_seq(p.seqs, p.n_seq, blockIdx.x);
+  const Q4Seq seq = p.seqs[i];
+  const int attend = seq.begin, nsplit = (attend + p.chunk - 1) / p.chunk;
+  const int layer = (blockIdx.x - seq.first) / nsplit, split = (blockIdx.x - seq.first) - layer * nsplit;
+  const long long unit = (long long)(p.seq_begin + i) * p.layer_count + layer;
+  const int row0 = split * p.chunk, row1 = min(row0 + p.chunk, attend), tiles = (row1 - row0 + kQ4Tile - 1) / kQ4Tile;
+  const bool last = row1 == attend;
+  const int held = last ? attend - 1 : row1;  // rows the cache holds before this call
+  bool ok = true;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      done[s] = 0u;
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  // where tile `k`'s rows are in the arena
+  auto tile_row = [&](int k) {
+    return kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, row0 + k * kQ4Tile);
+  };
+  auto issue = [&](int k, long long row) {
+    const int s = k % kStages, n = min(kQ4Tile, held - (row0 + k * kQ4Tile));
+    if (n <= 0) {  // only the new token's row, which is written below
+      mbar_arrive(&full[s]);
+      return;
+    }
+    mbar_arrive_expect_tx(&full[s], 2u * n * kQ4RowBytes);
+    bulk_load(sm + s * kStage, p.arena.k + row * kQ4RowBytes, n * kQ4RowBytes, &full[s]);
+    bulk_load(sm + s * kStage + kSide, p.arena.v + row * kQ4RowBytes, n * kQ4RowBytes, &full[s]);
+  };
+  if (tid == 0)
+    for (int k = 0; k < min(kStages, tiles); ++k) issue(k, tile_row(k));
+
+  Query<M, PRECISE> query;
+  bool good = load_query<M, PRECISE>(p, unit, h, attend - 1, p.q_rot_out && split == 0 && half == 0, &query);
+
+  // The new token's row of this head: lanes 0 .. LPH-1 its key, the next LPH
+  // its value. The warp whose rows it falls among quantises it and puts it
+  // into its tile and the arena; no other warp reads it.
+  const int new_row = (attend - 1 - row0) & (kQ4Tile - 1);
+  const bool owner = last && new_row / C::ROWS == half;
+  uint32_t new_codes = 0u;
+  __half new_scale = __float2half_rn(0.0f);
+  if (owner) {
+    const int c = lane & (R::LPH - 1);
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+    if (lane < 2 * R::LPH)
+      load8(lane < R::LPH ? p.k : p.v, (unit * M::HKV + h) * M::D + 8 * c, p.in_dtype, p.vec, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e];
+    const bool rotated = rotate_head<M>(y, c, attend - 1, p.k_norm, p.rope);
+    if (lane < R::LPH) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = y[e];
+      good &= rotated;
+    }
+    good &= quantise8(x, &new_codes, &new_scale);
+    const uint32_t halves = value_halves(new_codes);
+    if (lane >= R::LPH) new_codes = halves;
+  }
+
+  float o[2 * NG][4];
+#pragma unroll
+  for (int m = 0; m < 2 * NG; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[m][e] = 0.0f;
+  float m = -INFINITY, sum = 0.0f;  // of query head g, this lane's rows
+  // the cache row that MMA row (or column) g stands for, and those of 2 t and 2 t + 1
+  const int row_g = (g & 1) ? 4 + ((g >> 1) ^ 2) : g >> 1, row_a = t, row_b = 4 + (t ^ 2);
+
+  for (int k = 0; k < tiles; ++k) {
+    const int s = k % kStages;
+    unsigned char* tile = sm + s * kStage;
+    const int valid = min(kQ4Tile, row1 - (row0 + k * kQ4Tile));
+    const bool refill = k + kStages < tiles;
+    const long long next = refill && lane == 0 ? tile_row(k + kStages) : 0;
+    ok &= mbar_wait_bounded(&full[s], (uint32_t)(k / kStages) & 1u, p.err);
+    __syncwarp();
+    if (owner && k == tiles - 1) {
+      const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, attend - 1);
+      const int c = lane & (R::LPH - 1);
+      if (lane < R::LPH) {
+        put_key<M>(reinterpret_cast<char*>(tile) + new_row * kQ4RowBytes, h, c, new_codes, new_scale);
+        put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, new_codes, new_scale);
+      } else if (lane < 2 * R::LPH) {
+        put_value<M>(reinterpret_cast<char*>(tile) + kSide + new_row * kQ4RowBytes, h, c, new_codes, new_scale);
+        put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, new_codes, new_scale);
+      }
+      __syncwarp();
+    }
+#pragma unroll 1
+    for (int r0 = half * C::ROWS; r0 < min(valid, (half + 1) * C::ROWS); r0 += 32) {
+      const unsigned char* ks = tile + r0 * kQ4RowBytes;
+      const unsigned char* vs = ks + kSide;
+      // ---- scores of 32 rows: x[n] = rows 8 n + row_a, 8 n + row_b of head g
+      float2 x[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        uint32_t w[NG];
+        const unsigned char* kr = ks + (8 * n + row_g) * kQ4RowBytes + h * R::HEAD + 4 * NG * t;
+        if constexpr (NG == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(kr);
+          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(kr);
+          w[0] = u.x, w[1] = u.y;
+        }
+        Words<NG> sa, sb;
+        sa.load(ks + (8 * n + row_a) * kQ4RowBytes + R::scale(h, 0));
+        sb.load(ks + (8 * n + row_b) * kQ4RowBytes + R::scale(h, 0));
+        float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint32_t* a = query.a[j][0];
+          mma_f16(c, a[0], a[1], a[2], a[3], codes_low(w[j]), codes_high(w[j]));
+          a = query.a[j][1];
+          mma_f16(c, a[0], a[1], a[2], a[3], codes_low(w[j] >> 8), codes_high(w[j] >> 8));
+          const float2 fa = unpack_half(sa.w[j / 2]), fb = unpack_half(sb.w[j / 2]);
+          acc = __ffma2_rn(make_float2(j & 1 ? fa.y : fa.x, j & 1 ? fb.y : fb.x),
+                           __fadd2_rn(make_float2(c[0], c[1]), make_float2(c[2], c[3])), acc);
+        }
+        x[n] = __fmul2_rn(acc, make_float2(query.unit, query.unit));
+      }
+      Words<NG> va[4], vb[4];  // scales of the values
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        va[n].load(vs + (8 * n + row_a) * kQ4RowBytes + R::scale(h, 0));
+        vb[n].load(vs + (8 * n + row_b) * kQ4RowBytes + R::scale(h, 0));
+      }
+      if (r0 + 32 > valid) {  // rows past the last: no weight, and no garbage for a scale
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          if (r0 + 8 * n + row_a >= valid) {
+            x[n].x = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < NG / 2; ++e) va[n].w[e] = 0u;
+          }
+          if (r0 + 8 * n + row_b >= valid) {
+            x[n].y = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < NG / 2; ++e) vb[n].w[e] = 0u;
+          }
+        }
+      }
+      // ---- reference m, from the largest score plus the exponent of the
+      // largest scale
+      float top = fmax3f(x[0].x, x[0].y, x[1].x);
+      top = fmax3f(top, x[1].y, x[2].x);
+      top = fmax3f(top, x[2].y, x[3].x);
+      top = fmaxf(top, x[3].y);
+      uint32_t most = 0u;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < NG / 2; ++e) most = __vimax3_u16x2(most, va[n].w[e], vb[n].w[e]);
+      top += (float)(int)(max(most & 0xffffu, most >> 16) >> 10) - 14.0f;
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - kTop;
+      const bool raise = top > m + kSlack;  // always in the first step (m = -inf)
+      if (__any_sync(0xffffffffu, raise)) {
+        const float keep = raise ? fast_exp2(m - top) : 1.0f;
+        if (raise) m = top;
+        sum *= keep;
+        const float k0 = __shfl_sync(0xffffffffu, keep, 8 * t), k1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
+#pragma unroll
+        for (int e = 0; e < 2 * NG; ++e) {
+          o[e][0] *= k0;
+          o[e][1] *= k1;
+          o[e][2] *= k0;
+          o[e][3] *= k1;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        x[n] = make_float2(fast_exp2(x[n].x - m), fast_exp2(x[n].y - m));
+        sum += x[n].x + x[n].y;
+      }
+      // ---- O^T += V^T P'^T, 16 rows at a time
+#pragma unroll
+      for (int n = 0; n < 4; n += 2) {
+        Words<NG> ca0, cb0, ca1, cb1;
+        const unsigned char* vr = vs + 8 * n * kQ4RowBytes + h * R::HEAD + 2 * NG * g;
+        ca0.load(vr + row_a * kQ4RowBytes);
+        cb0.load(vr + row_b * kQ4RowBytes);
+        ca1.load(vr + (8 + row_a) * kQ4RowBytes);
+        cb1.load(vr + (8 + row_b) * kQ4RowBytes);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          const float2 a0 = unpack_half(va[n].w[j / 2]), b0 = unpack_half(vb[n].w[j / 2]);
+          const float2 a1 = unpack_half(va[n + 1].w[j / 2]), b1 = unpack_half(vb[n + 1].w[j / 2]);
+          const float2 p0 = __fmul2_rn(x[n], make_float2(j & 1 ? a0.y : a0.x, j & 1 ? b0.y : b0.x));
+          const float2 p1 = __fmul2_rn(x[n + 1], make_float2(j & 1 ? a1.y : a1.x, j & 1 ? b1.y : b1.x));
+          const uint32_t h0 = pack_half(p0.x, p0.y), h1 = pack_half(p1.x, p1.y);
+          // half j of the rows: low 16 bits row a, high 16 bits row b
+          const uint32_t pick = j & 1 ? 0x7632u : 0x5410u;
+          const uint32_t z0 = __byte_perm(ca0.w[j / 2], cb0.w[j / 2], pick);
+          const uint32_t z1 = __byte_perm(ca1.w[j / 2], cb1.w[j / 2], pick);
+          const uint32_t c00 = codes_low(z0), c01 = codes_high(z0), c02 = codes_low(z0 >> 8), c03 = codes_high(z0 >> 8);
+          const uint32_t c10 = codes_low(z1), c11 = codes_high(z1), c12 = codes_low(z1 >> 8), c13 = codes_high(z1 >> 8);
+          mma_f16(o[2 * j], c00, c01, c10, c11, h0, h1);
+          mma_f16(o[2 * j + 1], c02, c03, c12, c13, h0, h1);
+          if constexpr (PRECISE) {
+            const float2 q0 = unpack_half(h0), q1 = unpack_half(h1);
+            const uint32_t l0 = pack_half(p0.x - q0.x, p0.y - q0.y), l1 = pack_half(p1.x - q1.x, p1.y - q1.y);
+            mma_f16(o[2 * j], c00, c01, c10, c11, l0, l1);
+            mma_f16(o[2 * j + 1], c02, c03, c12, c13, l0, l1);
+          }
+        }
+      }
+    }
+    // the last warp to finish a tile refills its stage
+    __syncwarp();
+    if (refill && lane == 0 && count_up(&done[s]) == 7u) {
+      done[s] = 0u;
+      issue(k + kStages, next);
+    }
+  }
+
+  // ---- the warps' sums meet in shared memory ------------------------------------
+  __syncthreads();  // every stage was read
+  float* red = reinterpret_cast<float*>(sm);
+  float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  if (t == 0 && g < M::G) stat[warp * M::G + g] = make_float2(m, sum);
+#pragma unroll
+  for (int e = 0; e < 2 * NG; ++e)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int head = 2 * t + (c & 1), dim = 16 * e + 8 * (c >> 1) + g;
+      if (head < M::G) red[(warp * M::G + head) * C::PITCH + dim] = o[e][c];
+    }
+  __syncthreads();
+  for (int e = tid; e < M::HQ * M::D; e += kThreads) {
+    const int qh = e / M::D, d = e - qh * M::D;
+    const int w0 = qh / M::G * C::WPH, head = qh - qh / M::G * M::G;
+    float top = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < C::WPH; ++w) top = fmaxf(top, stat[(w0 + w) * M::G + head].x);
+#pragma unroll
+    for (int w = 0; w < C::WPH; ++w) {
+      const float2 ml = stat[(w0 + w) * M::G + head];
+      const float weight = C::WPH == 1 ? 1.0f : fast_exp2(ml.x - top);
+      num = fmaf(weight, red[((w0 + w) * M::G + head) * C::PITCH + d], num);
+      den = fmaf(weight, ml.y, den);
+    }
+    if (nsplit > 1) {
+      p.part_o[(long long)blockIdx.x * M::HQ * M::D + e] = num;
+      if (d == 0) p.part_ml[(long long)blockIdx.x * M::HQ + qh] = make_float2(top, den);
+    } else {
+      const float y = num / den;
+      good &= isfinite(y);
+      store_any(p.out, unit * M::HQ * M::D + e, p.out_dtype, y);
+    }
+  }
+  if (!good && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
+}
+
+// The partials of a split (sequence, layer): a CTA joins 32 dims of one query
+// head, eight lanes of four dims for each of 32 shares of the splits.
+template <class M>
+__global__ void __launch_bounds__(256) qx_q4_merge_kernel(const __grid_constant__ Q4DecodeParams p) {
+  constexpr int SLICES = M::D / 32;
+  __shared__ float red[32][33];
+  __shared__ float tops[8], dens[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int slice = blockIdx.x % SLICES, qh = blockIdx.x / SLICES % M::HQ, rel = blockIdx.x / (SLICES * M::HQ);
+  const int i = rel / p.layer_count, layer = rel - i * p.layer_count;
+  const Q4Seq seq = p.seqs[i];
+  const int nsplit = (seq.begin + p.chunk - 1) / p.chunk;
+  if (nsplit == 1) return;
+  pdl_wait();
+  const long long item0 = seq.first + (long long)layer * nsplit;
+  const float2* ml = p.part_ml + item0 * M::HQ + qh;
+  float top = -INFINITY;
+  for (int s = tid; s < nsplit; s += 256) top = fmaxf(top, ml[(long long)s * M::HQ].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, tops[w]);
+  const int share = tid >> 3, c = tid & 7;
+  const float* po = p.part_o + (item0 * M::HQ + qh) * M::D + 32 * slice + 4 * c;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float den = 0.0f;
+#pragma unroll 4
+  for (int s = share; s < nsplit; s += 32) {
+    const float2 x = ml[(long long)s * M::HQ];
+    const float4 v = *reinterpret_cast<const float4*>(po + (long long)s * M::HQ * M::D);
+    const float w = fast_exp2(x.x - top);
+    den = fmaf(w, x.y, den);
+    acc.x = fmaf(w, v.x, acc.x);
+    acc.y = fmaf(w, v.y, acc.y);
+    acc.z = fmaf(w, v.z, acc.z);
+    acc.w = fmaf(w, v.w, acc.w);
+  }
+  red[share][4 * c] = acc.x;
+  red[share][4 * c + 1] = acc.y;
+  red[share][4 * c + 2] = acc.z;
+  red[share][4 * c + 3] = acc.w;
+  if (c == 0) dens[share] = den;
+  __syncthreads();
+  if (warp == 0) {
+    float num = 0.0f, all = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 32; ++s) {
+      num += red[s][lane];
+      all += dens[s];
+    }
+    const float y = num / all;
+    if (!isfinite(y)) flag_error(p.err, QX_ERR_BIT_NONFINITE);
+    const long long unit = (long long)(p.seq_begin + i) * p.layer_count + layer;
+    store_any(p.out, (unit * M::HQ + qh) * M::D + 32 * slice + lane, p.out_dtype, y);
+  }
+}
+
+cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int smem, cudaStream_t stream, const Q4DecodeParams& p) {
   cudaLaunchConfig_t cfg = {};
-  const long long warps = (long long)p.n_seq * p.layer_count * (qwen ? Qwen3Heads::HQ : GraniteHeads::HQ);
-  cfg.gridDim = dim3((unsigned)((warps + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, qwen ? qx_q4_decode_kernel<Qwen3Heads> : qx_q4_decode_kernel<GraniteHeads>, p);
+  return cudaLaunchKernelEx(&cfg, fn, p);
 }
+
+template <class M>
+cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
+  void (*fn)(Q4DecodeParams) = p.out_dtype == 0 ? qx_q4_decode_kernel<M, true> : qx_q4_decode_kernel<M, false>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  *launched = 0;
+  e = launch_dependent(fn, p.items, kSmem, stream, p);
+  if (e != cudaSuccess) return e;
+  ++*launched;
+  if (!p.split) return e;
+  e = launch_dependent(qx_q4_merge_kernel<M>, p.n_seq * p.layer_count * M::HQ * (M::D / 32), 0, stream, p);
+  if (e == cudaSuccess) ++*launched;
+  return e;
+}
+
+}  // namespace
+
+cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
+  return qwen ? decode<Qwen3Heads>(p, stream, launched) : decode<GraniteHeads>(p, stream, launched);
+}
+
+int q4_decode_blocks_per_sm() { return 2; }
 
 }  // namespace qx

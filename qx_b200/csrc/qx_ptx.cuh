@@ -191,6 +191,15 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, 
       : "memory");
 }
 
+// Bulk copy of `bytes` neighbouring bytes global -> this CTA's shared memory;
+// both addresses and the size are multiples of 16.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
+
 // Prefetch of a TMA tile into L2 only: nothing lands in shared memory and
 // no barrier completes (a plain copy for this CTA). L2 stays coherent with later
 // writes, so any rows may be prefetched, settled or not.

@@ -98,7 +98,7 @@ struct qxc_ctx {
   // 4-bit decode's and packed prefill's workspaces; the buffers they have
   // outgrown are kept until the context goes, since a captured graph may
   // still name them
-  Workspace q4_q, packed_rot;
+  Workspace q4_parts, packed_rot;
   std::vector<void*> outgrown;
   // prefill's rotated-query scratch (bf16 elements)
   unsigned short* prefill_q = nullptr;
@@ -1164,49 +1164,59 @@ qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a, int q_d
   });
 }
 
-// One decode step on a 4-bit arena, its arguments checked and its pages
-// mapped: the new rows and rotated queries, then the attention.
+// One decode step on a 4-bit arena, its arguments checked and its pages mapped.
 qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
-  const size_t heads = (size_t)a->seq_count * a->layer_count * kv->hq * kv->d;
-  float* q = a->q_rot_out;
-  if (!q) {
-    qxc_status st = reserve(ctx, &ctx->q4_q, heads * sizeof(float));
-    if (st != QXC_OK) return st;
-    q = reinterpret_cast<float*>(ctx->q4_q.ptr);
-  }
-  std::vector<int32_t> ones(a->seq_count, 1), attend(a->seq_count);
+  std::vector<int32_t> attend(a->seq_count), ones(a->seq_count, 1);
   for (int i = 0; i < a->seq_count; ++i) attend[i] = a->positions[i] + 1;
-  qxc_append_args ap;
-  memset(&ap, 0, sizeof(ap));
-  ap.layer_begin = a->layer_begin;
-  ap.layer_count = a->layer_count;
-  ap.seq_count = a->seq_count;
-  ap.seq_ids = a->seq_ids;
-  ap.positions = a->positions;
-  ap.counts = ones.data();
-  ap.q = a->q;
-  ap.k = a->k;
-  ap.v = a->v;
-  ap.q_rot = q;
-  ap.q_norm = a->q_norm;
-  ap.k_norm = a->k_norm;
-  ap.in_dtype = a->in_dtype;
-  qxc_status st = q4_append(ctx, kv, &ap, a->q_dtype, QXC_F32);
-  if (st != QXC_OK) return st;
+  int chunk = a->split;
+  if (chunk == 0)
+    chunk = auto_chunk(ctx->sm_count * q4_decode_blocks_per_sm(), attend.data(), a->seq_count, a->layer_count,
+                       kQ4MaxSplits, kQ4Tile);
+  ctx->last_split = chunk;
   Q4DecodeParams p;
   p.arena = q4_arena(kv);
   p.layer_begin = a->layer_begin;
   p.layer_count = a->layer_count;
-  p.q = q;
+  p.chunk = chunk;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
   p.out = a->out;
+  p.q_rot_out = a->q_rot_out;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.rope = rope_of(ctx, kv);
+  p.q_dtype = a->q_dtype;
+  p.in_dtype = a->in_dtype;
   p.out_dtype = a->out_dtype;
+  p.vec = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16);
   p.err = ctx->err_dev;
   return each_part(a->seq_count, a->seq_ids, attend.data(), ones.data(), [&](const Q4Seq* seqs, int n, int first, int) {
     memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
     p.n_seq = n;
     p.seq_begin = first;
-    QXC_CUDA(ctx, launch_q4_decode(is_qwen(kv), p, ctx->stream));
-    ctx->launches++;
+    p.split = 0;
+    long long items = 0;
+    for (int i = 0; i < n; ++i) {
+      const int nsplit = (seqs[i].begin + chunk - 1) / chunk;
+      p.seqs[i].first = (int)items;
+      items += (long long)nsplit * a->layer_count;
+      if (nsplit > 1) p.split = 1;
+    }
+    if (items > 0x7fffffffLL) return fail(ctx, QXC_ERR_INVALID_ARG, "too much work in one call");
+    p.items = (int)items;
+    if (p.split) {
+      // partials of every item: [HQ][D] sums, then [HQ] (m, l)
+      const size_t heads = (size_t)items * kv->hq;
+      qxc_status st = reserve(ctx, &ctx->q4_parts, heads * (kv->d * sizeof(float) + sizeof(float2)));
+      if (st != QXC_OK) return st;
+      p.part_o = reinterpret_cast<float*>(ctx->q4_parts.ptr);
+      p.part_ml = reinterpret_cast<float2*>(ctx->q4_parts.ptr + heads * kv->d * sizeof(float));
+    }
+    int launched = 0;
+    QXC_CUDA(ctx, launch_q4_decode(is_qwen(kv), p, ctx->stream, &launched));
+    ctx->launches += launched;
+    note_rows_written(ctx, kv, -1, 0);
     return QXC_OK;
   });
 }
@@ -1330,7 +1340,7 @@ void qxc_destroy(qxc_ctx* ctx) {
   cudaFree(ctx->stack_f);
   cudaFree(ctx->stack_words);
   cudaFree(ctx->prefill_q);
-  cudaFree(ctx->q4_q.ptr);
+  cudaFree(ctx->q4_parts.ptr);
   cudaFree(ctx->packed_rot.ptr);
   for (void* p : ctx->outgrown) cudaFree(p);
   if (ctx->err_host) cudaFreeHost(ctx->err_host);

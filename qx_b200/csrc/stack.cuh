@@ -126,15 +126,6 @@ struct StackCfg {
 };
 static_assert(StackCfg::SMEM <= 227 * 1024, "the stack kernel's shared memory must fit one SM");
 
-// 1-D bulk copy global -> shared (16-byte aligned addresses, size a
-// multiple of 16), completing on `bar`'s transaction count.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_addr(dst)),
-               "l"(src), "r"(bytes), "r"(smem_addr(bar))
-               : "memory");
-}
-
 // Poll state of one thread: when it first had to wait, and how often.
 struct StackPoll {
   unsigned long long t0 = 0;
