@@ -1,65 +1,378 @@
-// packed.cu — causal attention of whole prompts packed one after another.
+// packed.cu — causal attention of whole prompts packed one after another, on
+// tcgen05 tensor cores.
 //
-// First form: a warp takes one query head of one token, a lane D / 32
-// neighbouring dims, key after key with a running maximum and sum.
+// A work item is a block of a prompt's tokens and one kv head: two query tiles
+// of 128 rows, each 128 / G tokens x the kv head's G query heads, so the heads
+// of a group share every key and value tile. One CTA per item, longest first:
+//   warp 9      TMA producer, one thread: both query tiles, then the key and
+//               value tiles of 128 tokens through one ring in the order of
+//               their use
+//   warp 8      MMA issuer, one thread: for each tile in turn O += P V, then the
+//               next scores S = Q K^T, so one tile's products run while the
+//               other's softmax does
+//   warps 0-3, 4-7  the softmax of the first, the second tile: a thread owns a
+//               row, reads its 128 scores from TMEM, writes 128 weights over
+//               them as 16-bit pairs (the A operand of P V). The row's
+//               reference moves only when its maximum passes it by 2^8; then
+//               the thread rescales its row of O in TMEM, which no product
+//               uses while the tile's scores are being read.
+// S of a tile is issued after its P V, and tensor instructions of one thread
+// complete in order: once S is there, P may be overwritten and O is settled.
+//
+// A key tile may hold tokens its rows do not attend: later ones of the prompt,
+// the next prompt's. Their scores are replaced by -inf, so their weights are
+// zero, but a zero weight times an infinite or NaN value is NaN: a row whose
+// sums are finite and whose output is not is recomputed token by token
+// (careful_row), over what it attends only.
+#include <type_traits>
+
 #include "q4.cuh"
+#include "qx_tc.cuh"
 
 namespace qx {
 namespace {
 
-template <class M>
-__global__ void __launch_bounds__(128) qx_packed_kernel(const __grid_constant__ PackedParams p) {
-  constexpr int N = M::D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  pdl_wait();
-  if (w >= (long long)p.token_count * M::HQ) return;
-  const int qh = (int)(w % M::HQ), h = qh / M::G;
-  const int token = p.token_begin + (int)(w / M::HQ);
-  const Q4Seq s = p.seqs[find_seq(p.seqs, p.n_seq, token)];
-  float q[N], o[N], m = -INFINITY, sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    q[e] = load_any(p.q, token * p.q_stride + qh * M::D + N * lane + e, p.dtype);
-    o[e] = 0.0f;
+template <class M, typename T>
+struct Packed {
+  static constexpr int NT = 320;
+  static constexpr int HALVES = M::D / 64;          // 64-dim column blocks of a row
+  static constexpr int TOKENS = 128 / M::G;         // tokens of a query tile
+  static constexpr int BLK = 128 * 128;             // [128 rows][128 B]
+  static constexpr int TILE = HALVES * BLK;
+  static constexpr int STAGES = M::D == 128 ? 5 : 8;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_RING = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_RING + STAGES * TILE;
+  // qfull, ring full/empty, per tile: scores there, weights there, output done
+  static constexpr int NBAR = 1 + 2 * STAGES + 6;
+  static constexpr int SMEM = OFF_BAR + 8 * NBAR + 16 + 1024;  // + TMEM slot, + slack to align the base
+  static constexpr uint32_t COL_S = 0, COL_O = 256;            // tile u: scores at 128 u, output at 256 + D u
+  static constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  static constexpr float TAU = 8.0f;
+  static constexpr float UNIT = M::SCALE * 1.4426950408889634f;  // base-2 logit of a score
+  // of every POLY pairs of exponentials the last runs on the FMA pipe
+  static constexpr int POLY = 4;
+  static_assert(SMEM <= 227 * 1024, "fits one SM");
+  static_assert(packed_block(M::QWEN) == 2 * TOKENS, "two tiles a block");
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float2 x) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x.x, x.y);
+    return *reinterpret_cast<const uint32_t*>(&b);
+  } else {
+    const __half2 h = __floats2half2_rn(x.x, x.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  for (int t = s.first; t <= token; ++t) {
-    float dot = 0.0f;
+}
+
+// One output row by a whole warp, over tokens first .. token only, against the
+// row's own reference m and sum.
+template <class M, typename T>
+__device__ __noinline__ bool careful_row(const PackedParams& p, int first, int token, int qh, float m, float sum) {
+  constexpr int N = M::D / 32;
+  using P = Packed<M, T>;
+  const int lane = threadIdx.x & 31, h = qh / M::G;
+  const T* q = static_cast<const T*>(p.q) + token * p.q_stride + qh * M::D;
+  float o[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) dot += q[e] * load_any(p.k, t * p.k_stride + h * M::D + N * lane + e, p.dtype);
+  for (int e = 0; e < N; ++e) o[e] = 0.0f;
+  for (int t0 = first; t0 <= token; t0 += 32) {
+    float weight = 0.0f;
+    if (t0 + lane <= token) {
+      const T* k = static_cast<const T*>(p.k) + (t0 + lane) * p.k_stride + h * M::D;
+      float dot = 0.0f;
+      for (int d = 0; d < M::D; ++d) dot = fmaf(Elem<T>::to_f32(q[d]), Elem<T>::to_f32(k[d]), dot);
+      weight = fast_exp2(fmaf(dot, P::UNIT, -m));
+    }
+    for (int u = 0; u < 32 && t0 + u <= token; ++u) {
+      const float w = __shfl_sync(0xffffffffu, weight, u);
+      const T* v = static_cast<const T*>(p.v) + (t0 + u) * p.v_stride + h * M::D;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    const float x = dot * M::SCALE, top = fmaxf(m, x), keep = expf(m - top), e0 = expf(x - top);
-    m = top;
-    sum = sum * keep + e0;
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      o[e] = o[e] * keep + e0 * load_any(p.v, t * p.v_stride + h * M::D + N * lane + e, p.dtype);
+      for (int e = 0; e < N; ++e) o[e] = fmaf(w, Elem<T>::to_f32(v[32 * e + lane]), o[e]);
+    }
   }
   bool good = true;
+  T* out = static_cast<T*>(p.out) + ((long long)token * M::HQ + qh) * M::D;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const float y = o[e] / sum;
     good &= isfinite(y);
-    store_any(p.out, ((long long)token * M::HQ + qh) * M::D + N * lane + e, p.dtype, y);
+    out[32 * e + lane] = Elem<T>::from_f32(y);
   }
-  if (!good) flag_error(p.err, QX_ERR_BIT_NONFINITE);
+  return good;
 }
 
-}  // namespace
+template <class M, typename T>
+__global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __grid_constant__ PackedParams p) {
+  using C = Packed<M, T>;
+  constexpr int NS = C::STAGES;
+  extern __shared__ __align__(1024) unsigned char sm_raw[];
+  unsigned char* sm = sm_raw + ((1024u - (smem_addr(sm_raw) & 1023u)) & 1023u);
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+  uint64_t* full = qfull + 1;      // [NS] a key or value tile landed
+  uint64_t* empty = full + NS;     // [NS] its products completed
+  uint64_t* sfull = empty + NS;    // [tile] scores in TMEM (and everything issued before them done)
+  uint64_t* pfull = sfull + 2;     // [tile] weights in TMEM
+  uint64_t* odone = pfull + 2;     // [tile] output in TMEM
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(odone + 2);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-cudaError_t launch_packed(bool qwen, const PackedParams& p, cudaStream_t stream) {
+  // the item's prompt, kv head and block
+  int lo = 0, hi = p.n_seq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.seqs[mid].item <= (int)blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const PackedSeq seq = p.seqs[lo];
+  const int rel = blockIdx.x - seq.item, h = rel % M::HKV;
+  const int blocks = (seq.length + 2 * C::TOKENS - 1) / (2 * C::TOKENS);
+  const int q0 = (blocks - 1 - rel / M::HKV) * 2 * C::TOKENS;  // first token of the block, within the prompt
+  // key tiles each query tile attends (0: past the prompt's end)
+  int tiles[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int begin = q0 + u * C::TOKENS, end = min(begin + C::TOKENS, seq.length);
+    tiles[u] = begin < seq.length ? (end + kPackedKeys - 1) / kPackedKeys : 0;
+  }
+  const int n = max(tiles[0], tiles[1]);
+
+  if (tid == 0) {
+    mbar_init(qfull, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(&sfull[u], 1);
+      mbar_init(&pfull[u], 4);
+      mbar_init(&odone[u], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tslot;
+  pdl_wait();
+  pdl_launch_dependents();
+  bool ok = true;
+
+  if (warp == 9) {
+    // ---- TMA producer: keys of tile i are load 2 i, its values load 2 i + 1 ------
+    if (lane == 0) {
+      prefetch_tmap(&p.tmq);
+      prefetch_tmap(&p.tmk);
+      prefetch_tmap(&p.tmv);
+      const int used = tiles[1] ? 2 : 1;
+      mbar_arrive_expect_tx(qfull, used * C::TILE);
+      for (int u = 0; u < used; ++u)
+#pragma unroll
+        for (int b = 0; b < C::HALVES; ++b)
+          tma_load_3d(sm + C::OFF_Q + u * C::TILE + b * C::BLK, &p.tmq, 64 * b, h * M::G,
+                      seq.token + q0 + u * C::TOKENS, qfull);
+      for (int i = 0; i < 2 * n; ++i) {
+        const int s = i % NS;
+        if (i >= NS) ok &= mbar_wait_bounded(&empty[s], (uint32_t)(i / NS - 1) & 1u, p.err);
+        mbar_arrive_expect_tx(&full[s], C::TILE);
+#pragma unroll
+        for (int b = 0; b < C::HALVES; ++b)
+          tma_load_3d(sm + C::OFF_RING + s * C::TILE + b * C::BLK, i & 1 ? &p.tmv : &p.tmk, 64 * b, h,
+                      seq.token + (i >> 1) * kPackedKeys, &full[s]);
+      }
+      // no copy may still be landing when the CTA exits
+      for (int i = max(0, 2 * n - NS); i < 2 * n; ++i)
+        ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
+    }
+  } else if (warp == 8) {
+    // ---- MMA issuer ---------------------------------------------------------------
+    if (lane == 0) {
+      constexpr uint32_t IDESC_S = umma_idesc_16bit(128, kPackedKeys, C::FMT, false, false);
+      constexpr uint32_t IDESC_PV = umma_idesc_16bit(128, M::D, C::FMT, false, true);
+      const uint32_t sq = smem_addr(sm + C::OFF_Q), ring = smem_addr(sm + C::OFF_RING);
+      auto landed = [&](int i) {
+        ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
+        tc_fence_after();
+      };
+      auto scores = [&](int u, int i) {  // S of query tile u and key tile i
+        const uint32_t q = sq + u * C::TILE, k = ring + (2 * i % NS) * C::TILE;
+#pragma unroll
+        for (int kk = 0; kk < M::D / 16; ++kk)
+          tc_mma_bf16(tbase + C::COL_S + 128 * u, umma_desc_sw128(q + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024),
+                      umma_desc_sw128(k + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024), IDESC_S, kk > 0);
+        tc_commit(&sfull[u]);
+      };
+      auto output = [&](int u, int i) {  // O += P V of query tile u and key tile i
+        ok &= mbar_wait_bounded(&pfull[u], (uint32_t)i & 1u, p.err);
+        tc_fence_after();
+        const uint32_t v = ring + ((2 * i + 1) % NS) * C::TILE;
+#pragma unroll
+        for (int kk = 0; kk < kPackedKeys / 16; ++kk)
+          tc_mma_ts_bf16(tbase + C::COL_O + M::D * u, tbase + C::COL_S + 128 * u + 8 * kk,
+                         umma_desc_sw128(v + kk * 2048, C::BLK, 1024), IDESC_PV, (i > 0 ? 1u : 0u) | (kk > 0 ? 1u : 0u));
+      };
+      ok &= mbar_wait_bounded(qfull, 0, p.err);
+      landed(0);
+      for (int u = 0; u < 2; ++u)
+        if (tiles[u]) scores(u, 0);
+      tc_commit(&empty[0]);
+      for (int i = 0; i < n; ++i) {
+        landed(2 * i + 1);
+        if (i + 1 < n) landed(2 * i + 2);
+        for (int u = 0; u < 2; ++u) {
+          if (i < tiles[u]) output(u, i);
+          if (i + 1 < tiles[u]) scores(u, i + 1);
+          else if (i + 1 == tiles[u]) tc_commit(&odone[u]);
+        }
+        tc_commit(&empty[(2 * i + 1) % NS]);
+        if (i + 1 < n) tc_commit(&empty[(2 * i + 2) % NS]);
+      }
+      // TMEM and the ring are released only after every product completed
+      for (int u = 0; u < 2; ++u)
+        if (tiles[u]) ok &= mbar_wait_bounded(&odone[u], 0, p.err);
+    }
+  } else {
+    // ---- softmax of tile u: thread owns row r (token r / G of the tile, head r % G)
+    const int u = warp >> 2, r = tid & 127;
+    const int pos = q0 + u * C::TOKENS + r / M::G;  // within the prompt
+    const uint32_t trow = tbase + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = trow + C::COL_S + 128 * u, to = trow + C::COL_O + M::D * u;
+    float m = -INFINITY;
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    for (int i = 0; i < tiles[u]; ++i) {
+      ok &= mbar_wait_bounded(&sfull[u], (uint32_t)i & 1u, p.err);
+      __syncwarp();
+      tc_fence_after();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_ld32_sync(ts + c, s + c);
+      if (i == tiles[u] - 1 || (i + 1) * kPackedKeys > q0 + u * C::TOKENS) {  // some key is later than some row
+        const int limit = pos - i * kPackedKeys;
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c > limit) s[c] = -INFINITY;
+      }
+      float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 124; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m4[e] = fmax3f(m4[e], s[c + 2 * e], s[c + 2 * e + 1]);
+      }
+      m4[0] = fmax3f(m4[0], s[124], s[125]);
+      m4[1] = fmax3f(m4[1], s[126], s[127]);
+      const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * C::UNIT;
+      const bool raise = top > m + C::TAU;  // true on the first tile (m = -inf)
+      if (__any_sync(0xffffffffu, raise)) {
+        const float keep = raise ? fast_exp2(m - top) : 1.0f;
+        if (i > 0) {
+#pragma unroll
+          for (int c = 0; c < M::D; c += 16) {
+            float o[16];
+            uint32_t b[16];
+            tmem_ld16_sync(to + c, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) b[e] = __float_as_uint(o[e] * keep);
+            tmem_st16u(to + c, b);
+          }
+        }
+        sum[0] = __fmul2_rn(sum[0], make_float2(keep, keep));
+        sum[1] = __fmul2_rn(sum[1], make_float2(keep, keep));
+        if (raise) m = top;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int c = 32 * q + 2 * j;
+          const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), make_float2(C::UNIT, C::UNIT), make_float2(-m, -m));
+          const float2 e = j % C::POLY == C::POLY - 1 ? exp2_poly2(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          w[j] = pack_pair<T>(e);
+          sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+        }
+        tmem_st16u(ts + 16 * q, w);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pfull[u]);
+    }
+    // ---- output ---------------------------------------------------------------------
+    if (tiles[u]) {
+      ok &= mbar_wait_bounded(&odone[u], 0, p.err);
+      __syncwarp();
+      tc_fence_after();
+      const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), inv = 1.0f / all;
+      const bool real = pos < seq.length;
+      const int token = seq.token + pos, qh = h * M::G + r % M::G;
+      bool good = true;
+      T* out = static_cast<T*>(p.out) + ((long long)token * M::HQ + qh) * M::D;
+#pragma unroll
+      for (int c = 0; c < M::D; c += 32) {
+        float o[32];
+        tmem_ld32_sync(to + c, o);
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 y = make_float2(o[2 * e] * inv, o[2 * e + 1] * inv);
+          good &= isfinite(y.x) && isfinite(y.y);
+          w[e] = pack_pair<T>(y);
+        }
+        if (real) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            reinterpret_cast<uint4*>(out + c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        }
+      }
+      unsigned redo = __ballot_sync(0xffffffffu, real && ok && !good && isfinite(m) && isfinite(all));
+      bool bad = real && !good && !(isfinite(m) && isfinite(all));
+      while (redo) {
+        const int src = __ffs(redo) - 1;
+        redo &= redo - 1;
+        bad |= !careful_row<M, T>(p, seq.token, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, qh, src),
+                                  __shfl_sync(0xffffffffu, m, src), __shfl_sync(0xffffffffu, all, src));
+      }
+      if (bad && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+template <class M, typename T>
+cudaError_t packed(const PackedParams& p, cudaStream_t stream) {
+  using C = Packed<M, T>;
+  cudaError_t e = cudaFuncSetAttribute(qx_packed_kernel<M, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  const long long warps = (long long)p.token_count * (qwen ? Qwen3Heads::HQ : GraniteHeads::HQ);
-  cfg.gridDim = dim3((unsigned)((warps + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(p.items);
+  cfg.blockDim = dim3(C::NT);
+  cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, qwen ? qx_packed_kernel<Qwen3Heads> : qx_packed_kernel<GraniteHeads>, p);
+  return cudaLaunchKernelEx(&cfg, qx_packed_kernel<M, T>, p);
+}
+
+}  // namespace
+
+cudaError_t launch_packed(bool qwen, const PackedParams& p, cudaStream_t stream) {
+  if (p.dtype == 1)
+    return qwen ? packed<Qwen3Heads, __nv_bfloat16>(p, stream) : packed<GraniteHeads, __nv_bfloat16>(p, stream);
+  return qwen ? packed<Qwen3Heads, __half>(p, stream) : packed<GraniteHeads, __half>(p, stream);
 }
 
 }  // namespace qx

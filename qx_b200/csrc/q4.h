@@ -89,7 +89,16 @@ struct Q4DecodeParams {
 constexpr int kQ4Tile = 64;  // cache rows per pipeline stage; pages hold a multiple of it
 constexpr int kQ4MaxSplits = 1024;
 
+// One prompt of a packed call: its first packed token, its length, its first
+// work item in the launch.
+struct PackedSeq {
+  int token, length, item;
+};
+
 struct PackedParams {
+  // tokens x heads x head_dim: boxes of 64 dims, of a query tile's heads and
+  // tokens and of 128 keys, 128-byte swizzle
+  CUtensorMap tmq, tmk, tmv;
   const void* q;
   const void* k;
   const void* v;
@@ -97,10 +106,14 @@ struct PackedParams {
   long long q_stride, k_stride, v_stride;  // elements between tokens
   int dtype;
   int n_seq;
-  int token_begin, token_count;
+  int items;
   unsigned* err;
-  Q4Seq seqs[kQ4Seqs];  // begin: tokens of the sequence; first: its first packed token
+  PackedSeq seqs[kQ4Seqs];  // longest first
 };
+
+// Tokens of a query block (two tiles of 128 query rows).
+constexpr int packed_block(bool qwen) { return qwen ? 32 : 128; }
+constexpr int kPackedKeys = 128;  // keys of a tile
 
 cudaError_t launch_q4_append(bool qwen, const Q4AppendParams& p, cudaStream_t stream);
 cudaError_t launch_q4_read(bool qwen, const Q4ReadParams& p, cudaStream_t stream);

@@ -1233,6 +1233,24 @@ qxc_status check_lengths(qxc_ctx* ctx, int seq_count, const int32_t* lengths, lo
   return QXC_OK;
 }
 
+// 3-D map of a packed tensor {head_dim, heads, tokens} with the given token
+// stride: boxes of 64 dims (128 bytes) x box_heads x box_tokens, 128-byte
+// swizzle. Tokens past the last read as zero.
+qxc_status encode_token_map(qxc_ctx* ctx, CUtensorMap* map, const void* base, int dtype, int d, int heads, int tokens,
+                            long long stride, int box_heads, int box_tokens) {
+  auto fn = encode_fn();
+  if (!fn) return fail(ctx, QXC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, dtype == QXC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ctx, QXC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return QXC_OK;
+}
+
 qxc_status attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
   int hq, hkv, d;
   model_shape(a->model, &hq, &hkv, &d);
@@ -1251,15 +1269,34 @@ qxc_status attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
     return fail(ctx, QXC_ERR_INVALID_ARG, "packed tensors must be 16-byte aligned, their token strides multiples of 8");
   if (p.q_stride < (long long)hq * d || p.k_stride < (long long)hkv * d || p.v_stride < (long long)hkv * d)
     return fail(ctx, QXC_ERR_INVALID_ARG, "a token stride is shorter than a token's heads");
-  return each_part(a->seq_count, nullptr, a->lengths, a->lengths, [&](const Q4Seq* seqs, int n, int first, int tokens) {
-    memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
-    p.n_seq = n;
-    p.token_begin = first;
-    p.token_count = tokens;
-    QXC_CUDA(ctx, launch_packed(a->model == QXC_MODEL_QWEN3, p, ctx->stream));
+  std::vector<PackedSeq> prompts;
+  int token = 0;
+  for (int i = 0; i < a->seq_count; ++i) {
+    if (a->lengths[i]) prompts.push_back({token, a->lengths[i], 0});
+    token += a->lengths[i];
+  }
+  // the longest work items first: what is left at the end of a launch is short
+  std::stable_sort(prompts.begin(), prompts.end(),
+                   [](const PackedSeq& x, const PackedSeq& y) { return x.length > y.length; });
+  const bool qwen = a->model == QXC_MODEL_QWEN3;
+  const int block = packed_block(qwen), group = hq / hkv;
+  qxc_status st = encode_token_map(ctx, &p.tmq, a->q, a->dtype, d, hq, token, p.q_stride, group, 128 / group);
+  if (st == QXC_OK) st = encode_token_map(ctx, &p.tmk, a->k, a->dtype, d, hkv, token, p.k_stride, 1, kPackedKeys);
+  if (st == QXC_OK) st = encode_token_map(ctx, &p.tmv, a->v, a->dtype, d, hkv, token, p.v_stride, 1, kPackedKeys);
+  if (st != QXC_OK) return st;
+  for (size_t at = 0; at < prompts.size(); at += kQ4Seqs) {
+    p.n_seq = (int)std::min<size_t>(kQ4Seqs, prompts.size() - at);
+    p.items = 0;
+    for (int i = 0; i < p.n_seq; ++i) {
+      p.seqs[i] = prompts[at + i];
+      p.seqs[i].item = p.items;
+      p.items += (prompts[at + i].length + block - 1) / block * hkv;
+    }
+    QXC_CUDA(ctx, launch_packed(qwen, p, ctx->stream));
     ctx->launches++;
-    return QXC_OK;
-  });
+    note_rows_written(ctx, nullptr, -1, 0);
+  }
+  return QXC_OK;
 }
 
 // No C++ exception leaves a C entry point.

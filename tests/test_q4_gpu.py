@@ -260,7 +260,8 @@ def check_decode(ctx, arena, q, k, v, out, positions, out_dtype, qw=None, kw=Non
             # a dot product of D terms in chains of at most 64, the query's own rotation (8) and split (4)
             weights = 2 * ref.logit_error(model, qr, keys, 76) + 2.0 ** -20 + (0 if out_dtype == F32 else 2.0 ** -11)
             floor = (pos + 1) * 2.0 ** -31 * 7 * vs.astype(np.float64).max()
-            tol = ref.HALF_STEP[out_dtype] * np.abs(want) + weights * mean + floor + 1e-30
+            floor += 2.0 ** -25 if out_dtype == F16 else 1e-30  # half of an fp16 output's smallest step
+            tol = ref.HALF_STEP[out_dtype] * np.abs(want) + weights * mean + floor
             assert ref.close(host(out[i, l]), want, tol) <= 1, (i, l, pos)
 
 
