@@ -136,14 +136,15 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
 /* key_dtype = value_dtype = QXC_Q4 (new; the reference keeps caches in f32 or
  * f16): keys and values are quantised as they are written, per kv head and
  * group of 32 dims, by the value rule of the Q4 weights below: an FP16 scale
- * s = fp16(max |x| / 7) and codes c = clamp(rint(x / s), -7, 7) + 7 that stand
- * for (c - 7) * s (all zero when s rounds to zero). Keys are rotated first and
+ * s = fp16(max |x| / 7) and codes c = clamp(rint(x / s), -7, 7) that stand for
+ * c * s (all zero when s rounds to zero). Keys are rotated first and
  * rounded to f32. A row, one position's keys or values of all kv heads, is 288
  * bytes for either model: the kv heads' codes, head_dim / 2 bytes each, then
  * the scales [kv_heads][head_dim / 32]. With NG = head_dim / 32, dim 32 j + r
  * of a head is
- *   keys    nibble r % 8 (low first) of its 32-bit word (r / 8) * NG + j
- *   values  nibble r / 8 (low first) of its 16-bit half (r % 8) * NG + j
+ *   keys    c in two's complement in byte r % 4 of its 32-bit word (r / 8) * NG + j,
+ *           in the high nibble when r % 8 < 4, else in the low one
+ *   values  c + 7 in nibble r / 8 (low first) of its 16-bit half (r % 8) * NG + j
  * Contiguous or paged, any input type of either model; first_position must be
  * 0. Cursors, paging, views (bytes), qxc_kv_read / write (raw rows) work as on
  * any arena, qxc_decode reads and writes it, qxc_attention_layer and

@@ -3,15 +3,17 @@
 // A row (one position, all kv heads) is 288 bytes for both models:
 //   [0, 256)    codes, kv head after kv head, D / 2 bytes each
 //   [256, 288)  fp16 scales [kv head][D / 32]
-// A code c in 0..14 of a group of 32 dims stands for (c - 7) * scale, the
-// value rule of the framework's Q4 weights. Within a head the codes are laid
-// out for the lane that reads them in the attention kernel (group j of
-// D / 32, dim 32 j + r):
-//   keys    32-bit word t * (D / 32) + j holds dims r = 8 t .. 8 t + 7, low
-//           nibble first: lane t of a quad reads its words of all groups at
-//           once
-//   values  16-bit half g * (D / 32) + j holds dims r = 8 i + g in nibble i
-//           (i = 0..3): lane group g reads its halves of all groups at once
+// A code c in -7..7 of a group of 32 dims stands for c * scale, the values of
+// the framework's Q4 weights. Within a head the codes are laid out for the lane
+// that reads them in the attention kernel, and in the form that costs it the
+// fewest instructions (group j of D / 32, dim 32 j + r):
+//   keys    32-bit word t * (D / 32) + j holds dims r = 8 t .. 8 t + 7: lane t of
+//           a quad reads its words of all groups at once. Byte i has c of dim
+//           8 t + i in its high nibble and c of dim 8 t + 4 + i in its low one, in
+//           two's complement, so that w and w << 4, masked with 0xf0 in each byte,
+//           are eight 8-bit integers 16 c.
+//   values  16-bit half g * (D / 32) + j holds c + 7 of dims r = 8 i + g in nibble
+//           i (i = 0..3): lane group g reads its halves of all groups at once
 //
 // A head is D / 8 neighbouring lanes of eight dims each: lane `c` of a head
 // holds dims 8 c .. 8 c + 7, group c / 4, t = c % 4. Rotation pairs dim d with
@@ -133,10 +135,9 @@ __device__ __forceinline__ bool rotate_head(float* x, int c, int position, const
   return good;
 }
 
-// Codes of this lane's eight dims (nibble e: dim 8 c + e) and its group's
-// scale. False when the scale is not finite: a value above 7 * 65504, an
+// Codes -7..7 of this lane's eight dims and its group's scale. False when the scale is not finite: a value above 7 * 65504, an
 // infinity, or a NaN (which fmaxf alone would drop).
-__device__ __forceinline__ bool quantise8(const float* x, uint32_t* codes, __half* scale) {
+__device__ __forceinline__ bool quantise8(const float* x, int* codes, __half* scale) {
   float top = 0.0f;
   bool good = true;
 #pragma unroll
@@ -148,21 +149,24 @@ __device__ __forceinline__ bool quantise8(const float* x, uint32_t* codes, __hal
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const __half h = __float2half_rn(__fdiv_rn(top, 7.0f));
   const float s = __half2float(h);
-  uint32_t w = 0x77777777u;  // a scale that rounds to zero: every value is zero
-  if (s > 0.0f) {
-    w = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int code = __float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f)) + 7;
-      w |= (uint32_t)code << (4 * e);
-    }
-  }
-  *codes = w;
+  for (int e = 0; e < 8; ++e)  // a scale that rounds to zero: every value is zero
+    codes[e] = s > 0.0f ? __float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f)) : 0;
   *scale = h;
   return good && isfinite(s);
 }
 
-// Store this lane's codes and scale as part of a key row.
+// This lane's eight codes as a word of a key row.
+__device__ __forceinline__ uint32_t key_codes(const int* c) {
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w |= ((uint32_t)c[i] & 15u) << (8 * i + 4) | ((uint32_t)c[4 + i] & 15u) << (8 * i);
+  }
+  return w;
+}
+
+// Store this lane's word and scale as part of a key row.
 template <class M>
 __device__ __forceinline__ void put_key(char* row, int head, int c, uint32_t codes, __half scale) {
   *reinterpret_cast<uint32_t*>(row + Q4Row<M>::key_word(head, c)) = codes;
@@ -172,9 +176,11 @@ __device__ __forceinline__ void put_key(char* row, int head, int c, uint32_t cod
 // The halves g = 2 t (low 16 bits) and 2 t + 1 of a value row's group that
 // lane t of a quad stores: nibble i of half g comes from lane i, which holds
 // dims 8 i + g. Every lane of the warp takes part.
-__device__ __forceinline__ uint32_t value_halves(uint32_t codes) {
+__device__ __forceinline__ uint32_t value_halves(const int* c) {
   const int lane = threadIdx.x & 31, t = lane & 3;
-  uint32_t out = 0u;
+  uint32_t codes = 0u, out = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) codes |= (uint32_t)(c[e] + 7) << (4 * e);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = __shfl_sync(0xffffffffu, codes, (lane & ~3) + i) >> (8 * t);

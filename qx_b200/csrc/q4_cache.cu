@@ -38,19 +38,19 @@ __global__ void __launch_bounds__(kThreads) qx_q4_append_kernel(const __grid_con
   } else {
     head -= q_heads;
     const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq, p.layer_begin + l, position);
-    uint32_t codes;
+    int codes[8];
     __half scale;
     if (head < M::HKV) {
       load8(p.k, token * p.k_stride + ((long long)l * M::HKV + head) * M::D + 8 * c, p.in_dtype, p.vec, x);
       good = rotate_head<M>(x, c, position, p.k_norm, p.rope);
       if (p.k_rot)
         store8(p.k_rot, (((long long)token * p.layer_count + l) * M::HKV + head) * M::D + 8 * c, p.rot_dtype, p.vec, x);
-      good &= quantise8(x, &codes, &scale);
-      put_key<M>(p.arena.k + row * kQ4RowBytes, head, c, codes, scale);
+      good &= quantise8(x, codes, &scale);
+      put_key<M>(p.arena.k + row * kQ4RowBytes, head, c, key_codes(codes), scale);
     } else {
       head -= M::HKV;
       load8(p.v, token * p.v_stride + ((long long)l * M::HKV + head) * M::D + 8 * c, p.in_dtype, p.vec, x);
-      good = quantise8(x, &codes, &scale);
+      good = quantise8(x, codes, &scale);
       put_value<M>(p.arena.v + row * kQ4RowBytes, head, c, value_halves(codes), scale);
     }
   }
@@ -74,20 +74,25 @@ __global__ void __launch_bounds__(kThreads) qx_q4_read_kernel(const __grid_const
   const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq, p.layer_begin + l,
                                s.begin + token - s.first);
   const char* src = (side ? p.arena.v : p.arena.k) + row * kQ4RowBytes;
-  uint32_t codes = 0u;
+  int codes[8];
   if (side == 0) {
-    codes = *reinterpret_cast<const uint32_t*>(src + R::key_word(head, c));
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(src + R::key_word(head, c));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      codes[i] = (int)(w << (24 - 8 * i)) >> 28;
+      codes[4 + i] = (int)(w << (28 - 8 * i)) >> 28;
+    }
   } else {
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
       const uint32_t half = *reinterpret_cast<const uint16_t*>(src + R::value_half(head, c >> 2, g));
-      codes |= ((half >> (4 * (c & 3))) & 15u) << (4 * g);
+      codes[g] = (int)((half >> (4 * (c & 3))) & 15u) - 7;
     }
   }
   const float scale = __half2float(*reinterpret_cast<const __half*>(src + R::scale(head, c >> 2)));
   float x[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)((int)((codes >> (4 * e)) & 15u) - 7), scale);
+  for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)codes[e], scale);
   store8(out, (((long long)token * p.layer_count + l) * M::HKV + head) * M::D + 8 * c, p.out_dtype, p.vec, x);
 }
 

@@ -2,29 +2,37 @@
 //
 // qx_q4_decode_kernel: a CTA takes one (sequence, layer) and one split of its
 // cached rows, all kv heads at once, so a run of rows is one contiguous piece
-// of memory (288 bytes a row). Eight warps: Granite's eight kv heads, or
-// Qwen's four, two warps each taking half of every tile's rows.
+// of memory (288 bytes a row). A warp takes a unit of eight query heads, one kv
+// head of Qwen or four of Granite, and a half (Granite: a quarter) of every
+// tile's rows:
 //   copies   tiles of 64 rows, keys and values, by bulk copies into a ring of
 //            three stages; the last warp to finish a tile refills its stage
-//   scores   S = [Q_hi; Q_lo] K^T by mma.m16n8k16: rows 0-7 are the kv head's
-//            query heads rounded to fp16, rows 8-15 what that rounding left,
-//            so a query counts with 22 bits at no extra product. K's codes
-//            become fp16 in registers and stay integers: each group of 32 dims
-//            has its own accumulator, multiplied by the row's scale in f32.
+//   scores   S = Q K^T by mma.m16n8k32 on 8-bit integers, exact: K's codes are
+//            8-bit integers as they lie in the row but for a mask, a query is
+//            rounded once to an integer of 15 bits (29 unless the output is bf16)
+//            against its head's largest element, cut into terms of 7 bits: rows
+//            0-7 of an operand hold one term of the unit's heads, rows 8-15 the
+//            next. Each group of 32 dims has its own accumulator, multiplied by
+//            the row's scale in f32.
 //   softmax  in f32, base 2, a running reference m per head and warp
-//   output   O^T += V^T P'^T, V's codes again as integers; P' = P * scale of
-//            (row, group), rounded to fp16 (two fp16 terms when the output is
-//            f32), one operand per group. P falls out of the score
+//   output   O^T += V^T P'^T by mma.m16n8k16, V's codes as fp16 integers; P' =
+//            P * scale of (row, group), rounded to fp16 (two fp16 terms when the
+//            output is f32), one operand per group. P falls out of the score
 //            accumulators in exactly the operand layout.
+// Granite's four kv heads of a unit share accumulators: a head's operand is
+// zero in the rows (columns) of the other heads, so a lane's scores, weights and
+// outputs are those of its own query head whichever kv head it has, and the
+// softmax runs on full lanes.
+//
 // The tensor instructions take their operands from registers: 4-bit codes
 // would have to pass through shared memory a second time to reach tcgen05, and
-// the products are a small part of the work (a tile's codes are expanded by
-// more instructions than multiply them).
+// the products are a small part of the work (expanding a tile's codes takes
+// more instructions than multiplying them).
 //
-// The row order inside a block of 8 (kRow below) makes the quads' loads of
-// neighbouring MMA rows fall into different banks: a row is 72 words, 8 modulo
-// 32, and rows 0, 6, 1, 7, 2, 4, 3, 5 give every 128-byte phase of the key
-// loads, of the value loads and of the scale loads distinct banks.
+// The row order inside a block of 8 (row_g, row_a, row_b below) makes the
+// quads' loads of neighbouring MMA rows fall into different banks: a row is 72
+// words, 8 modulo 32, and rows 0, 6, 1, 7, 2, 4, 3, 5 give every 128-byte phase
+// of the key loads, of the value loads and of the scale loads distinct banks.
 #include "q4.cuh"
 
 namespace qx {
@@ -34,7 +42,8 @@ constexpr int kThreads = 256;
 constexpr int kStages = 3;
 constexpr int kSide = kQ4Tile * kQ4RowBytes;  // bytes of a tile's keys, or values
 constexpr int kStage = 2 * kSide;
-constexpr int kOffBar = kStages * kStage;
+constexpr int kOffNew = kStages * kStage;               // a word and a scale per thread and pass: the new rows
+constexpr int kOffBar = kOffNew + 2 * kThreads * 8;
 constexpr int kSmem = kOffBar + 8 * kStages + 4 * kStages + 4;
 
 // The largest P' = 2^(x - m) * scale of a step is set to about 2^kTop when the
@@ -45,10 +54,23 @@ constexpr float kTop = 7.0f, kSlack = 8.0f;
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1, const int* c) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+
+// Integer accumulators start at the bits of 1.5 * 2^23: read as f32, they are
+// that number plus the sum (|sum| <= 127 * 112 * 32 < 2^22).
+constexpr int kZeroBits = 0x4b400000;
+constexpr float kZero = 12582912.0f;
+__device__ __forceinline__ float2 sums(int a, int b) {
+  return __fadd2_rn(make_float2(__int_as_float(a), __int_as_float(b)), make_float2(-kZero, -kZero));
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
@@ -57,15 +79,29 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// Nibbles 0 and 4 of w (low: bits 0 and 16) as fp16 c - 7: 0x6400 | c is 1024 + c.
-__device__ __forceinline__ uint32_t codes_low(uint32_t w) {
-  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+// Four integers' parts of `shift` bits and up, rounded, as bytes; y becomes the
+// rest.
+__device__ __forceinline__ uint32_t take_bytes(int* y, int shift) {
+  uint32_t w = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int part = shift ? (y[e] + (1 << shift >> 1)) >> shift : y[e];
+    y[e] -= part << shift;
+    w |= ((uint32_t)part & 255u) << (8 * e);
+  }
+  return w;
+}
+
+// Nibbles 0 and 4 of w (low: bits 0 and 16) as fp16 c - 7: 0x6400 | c is 1024 +
+// c. `magic` is 0x64006400 in a register: two constants would take two instructions.
+__device__ __forceinline__ uint32_t codes_low(uint32_t w, uint32_t magic) {
+  const uint32_t x = (w & 0x000f000fu) | magic;
   const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1031.0f));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 // Nibbles 1 and 5: 0x6400 | 16 c is 1024 + 16 c.
-__device__ __forceinline__ uint32_t codes_high(uint32_t w) {
-  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
+__device__ __forceinline__ uint32_t codes_high(uint32_t w, uint32_t magic) {
+  const uint32_t x = (w & 0x00f000f0u) | magic;
   const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0.0625f), __float2half2_rn(-71.0f));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
@@ -95,30 +131,39 @@ struct Words {  // N 16-bit halves per row and lane
 template <class M>
 struct Dec {
   static constexpr int NG = M::D / 32;
-  static constexpr int WPH = 8 / M::HKV;          // warps per kv head
-  static constexpr int ROWS = kQ4Tile / WPH;      // rows of a tile per warp
+  static constexpr int KVU = 8 / M::G;            // kv heads of a unit of eight query heads
+  static constexpr int UNITS = M::HKV / KVU;
+  static constexpr int PARTS = 8 / UNITS;         // of a tile's rows, a warp each
+  static constexpr int ROWS = kQ4Tile / PARTS, BLOCKS = ROWS / 8;
+  static constexpr int PASSES = KVU * M::D / 128;  // of 32 lanes over the unit's new keys and values
   static constexpr int PITCH = M::D + 8;          // floats per head in the closing exchange
-  static constexpr int OFF_STAT = 8 * M::G * PITCH * 4;
-  static_assert(OFF_STAT + 8 * M::G * 8 <= kStages * kStage, "the closing exchange fits the stages");
+  static constexpr int OFF_STAT = 8 * 8 * PITCH * 4;
+  static_assert(OFF_STAT + 8 * 8 * 8 <= kStages * kStage, "the closing exchange fits the stages");
 };
 
-// The rotated queries of a warp's kv head as MMA operands.
-template <class M, bool PRECISE>
+// What an output type asks for: queries of four terms of 7 bits (else two),
+// weights of two fp16 terms (else one).
+template <int OUT>
+struct Need {
+  static constexpr bool QUERY = OUT != 1, WEIGHT = OUT == 0;
+  static constexpr int PAIRS = QUERY ? 2 : 1;
+};
+
+// The rotated queries of a unit as MMA operands: pairs of terms.
+template <class M, int PAIRS>
 struct Query {
-  static constexpr int NG = M::D / 32;
-  uint32_t a[NG][2][4];
-  float unit;       // base-2 logit of an accumulator
+  uint32_t a[M::D / 32][PAIRS][4];
+  float unit;  // base-2 logit of the first pair's sum
 };
 
-// Lane (g, t) holds dims 32 j + 8 t .. + 7 of query head g: rotation pairs are
-// in the lane, norms in the quad.
-template <class M, bool PRECISE>
-__device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long unit, int h, int position, bool emit,
-                                           Query<M, PRECISE>* out) {
+// Lane (g, t) holds dims 32 j + 8 t .. + 7 of query head g of the unit:
+// rotation pairs are in the lane, norms in the quad.
+template <class M, int PAIRS>
+__device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long first_head, int position, bool emit,
+                                           Query<M, PAIRS>* out) {
   constexpr int NG = M::D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const bool mine = g < M::G;
-  const long long base = (unit * M::HQ + h * M::G + (mine ? g : 0)) * M::D + 8 * t;
+  const long long base = (first_head + g) * M::D + 8 * t;
   float x[NG * 8];
 #pragma unroll
   for (int j = 0; j < NG; ++j) load8(p.q, base + 32 * j, p.q_dtype, p.vec, x + 8 * j);
@@ -157,49 +202,52 @@ __device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long un
       good &= isfinite(a) && isfinite(b);
       top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
     }
-  if (emit && mine) {
+  if (emit) {
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) p.q_rot_out[base + 32 * j + e] = x[8 * j + e];
   }
-  // largest element of the head to [2^14, 2^15): fp16 then holds the leading
-  // 11 bits of every element that matters, a second fp16 the next 11
+  // the head's largest element to 126 * 2^7 (126 * 2^21): its first term, rounded,
+  // then stays within a byte; a code counts 16
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const int ex = max((int)(__float_as_uint(top) >> 23), 15);
-  const float up = __int_as_float((268 - ex) << 23), down = __int_as_float((ex - 14) << 23);
-  out->unit = M::SCALE * 1.4426950408889634f * down;
+  top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), 1e-30f);
+  constexpr float MOST = PAIRS == 2 ? 126.0f * 2097152.0f : 126.0f * 128.0f;
+  const float up = MOST / top;
+  out->unit = M::SCALE * 1.4426950408889634f / 16.0f * (top / (126.0f * 128.0f));
 #pragma unroll
   for (int j = 0; j < NG; ++j)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int s = 0; s < 2; ++s) {  // dims 8 t .. + 3, 8 t + 4 .. + 7
+      int y[4];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const float y0 = mine ? x[8 * j + 2 * u + s] * up : 0.0f, y1 = mine ? x[8 * j + 2 * u + s + 4] * up : 0.0f;
-        const uint32_t hi = pack_half(y0, y1);
-        const float2 back = unpack_half(hi);
-        out->a[j][u][2 * s] = hi;
-        out->a[j][u][2 * s + 1] = pack_half(y0 - back.x, y1 - back.y);
+      for (int e = 0; e < 4; ++e) y[e] = __float2int_rn(x[8 * j + 4 * s + e] * up);
+      if constexpr (PAIRS == 2) {
+        out->a[j][0][2 * s] = take_bytes(y, 21);
+        out->a[j][0][2 * s + 1] = take_bytes(y, 14);
       }
+      out->a[j][PAIRS - 1][2 * s] = take_bytes(y, 7);
+      out->a[j][PAIRS - 1][2 * s + 1] = take_bytes(y, 0);
+    }
   return good;
 }
 
-template <class M, bool PRECISE>
+template <class M, int OUT>
 __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_constant__ Q4DecodeParams p) {
   using C = Dec<M>;
   using R = Q4Row<M>;
-  constexpr int NG = C::NG;
+  constexpr int NG = C::NG, KVU = C::KVU, PAIRS = Need<OUT>::PAIRS;
+  constexpr bool PRECISE = Need<OUT>::WEIGHT;
   extern __shared__ __align__(128) unsigned char sm[];
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + kOffBar);
   unsigned* done = reinterpret_cast<unsigned*>(full + kStages);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int h = warp / C::WPH, half = warp % C::WPH;
+  const int part = warp % C::PARTS, unit = warp / C::PARTS;
   const int i = find_seq(p.seqs, p.n_seq, blockIdx.x);
   const Q4Seq seq = p.seqs[i];
   const int attend = seq.begin, nsplit = (attend + p.chunk - 1) / p.chunk;
   const int layer = (blockIdx.x - seq.first) / nsplit, split = (blockIdx.x - seq.first) - layer * nsplit;
-  const long long unit = (long long)(p.seq_begin + i) * p.layer_count + layer;
+  const long long cell = (long long)(p.seq_begin + i) * p.layer_count + layer;  // (sequence, layer) of the call
   const int row0 = split * p.chunk, row1 = min(row0 + p.chunk, attend), tiles = (row1 - row0 + kQ4Tile - 1) / kQ4Tile;
   const bool last = row1 == attend;
   const int held = last ? attend - 1 : row1;  // rows the cache holds before this call
@@ -232,34 +280,36 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   if (tid == 0)
     for (int k = 0; k < min(kStages, tiles); ++k) issue(k, tile_row(k));
 
-  Query<M, PRECISE> query;
-  bool good = load_query<M, PRECISE>(p, unit, h, attend - 1, p.q_rot_out && split == 0 && half == 0, &query);
+  Query<M, PAIRS> query;
+  bool good = load_query<M, PAIRS>(p, cell * M::HQ + 8 * unit, attend - 1,
+                                     p.q_rot_out && split == 0 && part == 0, &query);
 
-  // The new token's row of this head: lanes 0 .. LPH-1 its key, the next LPH
-  // its value. The warp whose rows it falls among quantises it and puts it
-  // into its tile and the arena; no other warp reads it.
+  // The new token's rows of this unit's kv heads, D / 8 lanes each: the keys,
+  // then the values. The warp whose rows they fall among quantises them and puts
+  // them into its tile and the arena; no other warp reads them.
   const int new_row = (attend - 1 - row0) & (kQ4Tile - 1);
-  const bool owner = last && new_row / C::ROWS == half;
-  uint32_t new_codes = 0u;
-  __half new_scale = __float2half_rn(0.0f);
+  const bool owner = last && new_row / C::ROWS == part;
+  uint2* fresh = reinterpret_cast<uint2*>(sm + kOffNew) + tid;
   if (owner) {
-    const int c = lane & (R::LPH - 1);
-    float x[8], y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    if (lane < 2 * R::LPH)
-      load8(lane < R::LPH ? p.k : p.v, (unit * M::HKV + h) * M::D + 8 * c, p.in_dtype, p.vec, x);
+    for (int a = 0; a < C::PASSES; ++a) {
+      const int at = 32 * a + lane, c = at & (R::LPH - 1);
+      const bool value = at >= KVU * R::LPH;
+      const int h = unit * KVU + at / R::LPH % KVU;
+      float x[8], y[8];
+      load8(value ? p.v : p.k, (cell * M::HKV + h) * M::D + 8 * c, p.in_dtype, p.vec, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = x[e];
-    const bool rotated = rotate_head<M>(y, c, attend - 1, p.k_norm, p.rope);
-    if (lane < R::LPH) {
+      for (int e = 0; e < 8; ++e) y[e] = x[e];
+      const bool rotated = rotate_head<M>(y, c, attend - 1, p.k_norm, p.rope);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = y[e];
-      good &= rotated;
+      for (int e = 0; e < 8; ++e) x[e] = value ? x[e] : y[e];
+      good &= value || rotated;
+      int codes[8];
+      __half scale;
+      good &= quantise8(x, codes, &scale);
+      const uint32_t halves = value_halves(codes);
+      fresh[a * kThreads] = make_uint2(value ? halves : key_codes(codes), __half_as_ushort(scale));
     }
-    good &= quantise8(x, &new_codes, &new_scale);
-    const uint32_t halves = value_halves(new_codes);
-    if (lane >= R::LPH) new_codes = halves;
   }
 
   float o[2 * NG][4];
@@ -270,6 +320,11 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   float m = -INFINITY, sum = 0.0f;  // of query head g, this lane's rows
   // the cache row that MMA row (or column) g stands for, and those of 2 t and 2 t + 1
   const int row_g = (g & 1) ? 4 + ((g >> 1) ^ 2) : g >> 1, row_a = t, row_b = 4 + (t ^ 2);
+  const int own = KVU == 1 ? 0 : g / M::G;  // kv head of query head g within the unit
+  const int scale_at = R::scale(unit * KVU + own, 0);
+  uint32_t magic;
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));  // opaque: kept in a register
+  const int zero[4] = {kZeroBits, kZeroBits, kZeroBits, kZeroBits};
 
   for (int k = 0; k < tiles; ++k) {
     const int s = k % kStages;
@@ -281,59 +336,92 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     __syncwarp();
     if (owner && k == tiles - 1) {
       const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, attend - 1);
-      const int c = lane & (R::LPH - 1);
-      if (lane < R::LPH) {
-        put_key<M>(reinterpret_cast<char*>(tile) + new_row * kQ4RowBytes, h, c, new_codes, new_scale);
-        put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, new_codes, new_scale);
-      } else if (lane < 2 * R::LPH) {
-        put_value<M>(reinterpret_cast<char*>(tile) + kSide + new_row * kQ4RowBytes, h, c, new_codes, new_scale);
-        put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, new_codes, new_scale);
+#pragma unroll
+      for (int a = 0; a < C::PASSES; ++a) {
+        const int at = 32 * a + lane, c = at & (R::LPH - 1), h = unit * KVU + at / R::LPH % KVU;
+        char* into = reinterpret_cast<char*>(tile) + new_row * kQ4RowBytes;
+        const uint2 x = fresh[a * kThreads];
+        const __half scale = __ushort_as_half((unsigned short)x.y);
+        if (at < KVU * R::LPH) {
+          put_key<M>(into, h, c, x.x, scale);
+          put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, x.x, scale);
+        } else {
+          put_value<M>(into + kSide, h, c, x.x, scale);
+          put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, x.x, scale);
+        }
       }
       __syncwarp();
     }
-#pragma unroll 1
-    for (int r0 = half * C::ROWS; r0 < min(valid, (half + 1) * C::ROWS); r0 += 32) {
+    const int r0 = C::ROWS * part;
+    if (r0 < valid) {
       const unsigned char* ks = tile + r0 * kQ4RowBytes;
       const unsigned char* vs = ks + kSide;
-      // ---- scores of 32 rows: x[n] = rows 8 n + row_a, 8 n + row_b of head g
-      float2 x[4];
+      // ---- scores: x[n] = rows 8 n + row_a, 8 n + row_b of head g, Granite's two
+      // blocks at a time so that its masked operands serve both
+      constexpr int NB = KVU == 1 ? 1 : 2;
+      float2 x[C::BLOCKS];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        uint32_t w[NG];
-        const unsigned char* kr = ks + (8 * n + row_g) * kQ4RowBytes + h * R::HEAD + 4 * NG * t;
-        if constexpr (NG == 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(kr);
-          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(kr);
-          w[0] = u.x, w[1] = u.y;
+      for (int n0 = 0; n0 < C::BLOCKS; n0 += NB) {
+        int c[NB][NG][PAIRS][4];
+#pragma unroll
+        for (int kv = 0; kv < KVU; ++kv) {
+          uint32_t w[NB][NG];
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const unsigned char* kr = ks + (8 * (n0 + n) + row_g) * kQ4RowBytes + (unit * KVU + kv) * R::HEAD + 4 * NG * t;
+            if constexpr (NG == 4) {
+              const uint4 u = *reinterpret_cast<const uint4*>(kr);
+              w[n][0] = u.x, w[n][1] = u.y, w[n][2] = u.z, w[n][3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(kr);
+              w[n][0] = u.x, w[n][1] = u.y;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            uint32_t a[PAIRS][4];
+#pragma unroll
+            for (int i2 = 0; i2 < PAIRS; ++i2)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[i2][e] = KVU == 1 || own == kv ? query.a[j][i2][e] : 0u;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const uint32_t b0 = w[n][j] & 0xf0f0f0f0u, b1 = (w[n][j] << 4) & 0xf0f0f0f0u;
+#pragma unroll
+              for (int i2 = 0; i2 < PAIRS; ++i2) mma_s8(c[n][j][i2], a[i2], b0, b1, kv == 0 ? zero : c[n][j][i2]);
+            }
+          }
         }
-        Words<NG> sa, sb;
-        sa.load(ks + (8 * n + row_a) * kQ4RowBytes + R::scale(h, 0));
-        sb.load(ks + (8 * n + row_b) * kQ4RowBytes + R::scale(h, 0));
-        float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const uint32_t* a = query.a[j][0];
-          mma_f16(c, a[0], a[1], a[2], a[3], codes_low(w[j]), codes_high(w[j]));
-          a = query.a[j][1];
-          mma_f16(c, a[0], a[1], a[2], a[3], codes_low(w[j] >> 8), codes_high(w[j] >> 8));
-          const float2 fa = unpack_half(sa.w[j / 2]), fb = unpack_half(sb.w[j / 2]);
-          acc = __ffma2_rn(make_float2(j & 1 ? fa.y : fa.x, j & 1 ? fb.y : fb.x),
-                           __fadd2_rn(make_float2(c[0], c[1]), make_float2(c[2], c[3])), acc);
+        for (int n = 0; n < NB; ++n) {
+          Words<NG> sa, sb;
+          sa.load(ks + (8 * (n0 + n) + row_a) * kQ4RowBytes + scale_at);
+          sb.load(ks + (8 * (n0 + n) + row_b) * kQ4RowBytes + scale_at);
+          float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const float2 fa = unpack_half(sa.w[j / 2]), fb = unpack_half(sb.w[j / 2]);
+            float2 dot = __ffma2_rn(sums(c[n][j][0][0], c[n][j][0][1]), make_float2(128.0f, 128.0f),
+                                    sums(c[n][j][0][2], c[n][j][0][3]));
+            if constexpr (PAIRS == 2) {
+              const float2 low = __ffma2_rn(sums(c[n][j][1][0], c[n][j][1][1]), make_float2(128.0f, 128.0f),
+                                            sums(c[n][j][1][2], c[n][j][1][3]));
+              dot = __ffma2_rn(low, make_float2(1.0f / 16384.0f, 1.0f / 16384.0f), dot);
+            }
+            acc = __ffma2_rn(make_float2(j & 1 ? fa.y : fa.x, j & 1 ? fb.y : fb.x), dot, acc);
+          }
+          x[n0 + n] = __fmul2_rn(acc, make_float2(query.unit, query.unit));
         }
-        x[n] = __fmul2_rn(acc, make_float2(query.unit, query.unit));
       }
-      Words<NG> va[4], vb[4];  // scales of the values
+      Words<NG> va[C::BLOCKS], vb[C::BLOCKS];  // scales of the values
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        va[n].load(vs + (8 * n + row_a) * kQ4RowBytes + R::scale(h, 0));
-        vb[n].load(vs + (8 * n + row_b) * kQ4RowBytes + R::scale(h, 0));
+      for (int n = 0; n < C::BLOCKS; ++n) {
+        va[n].load(vs + (8 * n + row_a) * kQ4RowBytes + scale_at);
+        vb[n].load(vs + (8 * n + row_b) * kQ4RowBytes + scale_at);
       }
-      if (r0 + 32 > valid) {  // rows past the last: no weight, and no garbage for a scale
+      if (r0 + C::ROWS > valid) {  // rows past the last: no weight, and no garbage for a scale
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < C::BLOCKS; ++n) {
           if (r0 + 8 * n + row_a >= valid) {
             x[n].x = -INFINITY;
 #pragma unroll
@@ -348,13 +436,12 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
       }
       // ---- reference m, from the largest score plus the exponent of the
       // largest scale
-      float top = fmax3f(x[0].x, x[0].y, x[1].x);
-      top = fmax3f(top, x[1].y, x[2].x);
-      top = fmax3f(top, x[2].y, x[3].x);
-      top = fmaxf(top, x[3].y);
+      float top = fmaxf(x[0].x, x[0].y);
       uint32_t most = 0u;
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 1; n < C::BLOCKS; ++n) top = fmax3f(top, x[n].x, x[n].y);
+#pragma unroll
+      for (int n = 0; n < C::BLOCKS; ++n)
 #pragma unroll
         for (int e = 0; e < NG / 2; ++e) most = __vimax3_u16x2(most, va[n].w[e], vb[n].w[e]);
       top += (float)(int)(max(most & 0xffffu, most >> 16) >> 10) - 14.0f;
@@ -375,39 +462,58 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
         }
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int n = 0; n < C::BLOCKS; ++n) {
         x[n] = make_float2(fast_exp2(x[n].x - m), fast_exp2(x[n].y - m));
         sum += x[n].x + x[n].y;
       }
       // ---- O^T += V^T P'^T, 16 rows at a time
 #pragma unroll
-      for (int n = 0; n < 4; n += 2) {
-        Words<NG> ca0, cb0, ca1, cb1;
-        const unsigned char* vr = vs + 8 * n * kQ4RowBytes + h * R::HEAD + 2 * NG * g;
-        ca0.load(vr + row_a * kQ4RowBytes);
-        cb0.load(vr + row_b * kQ4RowBytes);
-        ca1.load(vr + (8 + row_a) * kQ4RowBytes);
-        cb1.load(vr + (8 + row_b) * kQ4RowBytes);
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
+      for (int n = 0; n < C::BLOCKS; n += 2) {
+        // the operand of group j: rows 2 t, 2 t + 1 of both blocks, head g
+        uint32_t h0[NG], h1[NG], l0[NG], l1[NG];
+        auto weights = [&](int j) {
           const float2 a0 = unpack_half(va[n].w[j / 2]), b0 = unpack_half(vb[n].w[j / 2]);
           const float2 a1 = unpack_half(va[n + 1].w[j / 2]), b1 = unpack_half(vb[n + 1].w[j / 2]);
           const float2 p0 = __fmul2_rn(x[n], make_float2(j & 1 ? a0.y : a0.x, j & 1 ? b0.y : b0.x));
           const float2 p1 = __fmul2_rn(x[n + 1], make_float2(j & 1 ? a1.y : a1.x, j & 1 ? b1.y : b1.x));
-          const uint32_t h0 = pack_half(p0.x, p0.y), h1 = pack_half(p1.x, p1.y);
-          // half j of the rows: low 16 bits row a, high 16 bits row b
-          const uint32_t pick = j & 1 ? 0x7632u : 0x5410u;
-          const uint32_t z0 = __byte_perm(ca0.w[j / 2], cb0.w[j / 2], pick);
-          const uint32_t z1 = __byte_perm(ca1.w[j / 2], cb1.w[j / 2], pick);
-          const uint32_t c00 = codes_low(z0), c01 = codes_high(z0), c02 = codes_low(z0 >> 8), c03 = codes_high(z0 >> 8);
-          const uint32_t c10 = codes_low(z1), c11 = codes_high(z1), c12 = codes_low(z1 >> 8), c13 = codes_high(z1 >> 8);
-          mma_f16(o[2 * j], c00, c01, c10, c11, h0, h1);
-          mma_f16(o[2 * j + 1], c02, c03, c12, c13, h0, h1);
+          h0[j] = pack_half(p0.x, p0.y), h1[j] = pack_half(p1.x, p1.y);
           if constexpr (PRECISE) {
-            const float2 q0 = unpack_half(h0), q1 = unpack_half(h1);
-            const uint32_t l0 = pack_half(p0.x - q0.x, p0.y - q0.y), l1 = pack_half(p1.x - q1.x, p1.y - q1.y);
-            mma_f16(o[2 * j], c00, c01, c10, c11, l0, l1);
-            mma_f16(o[2 * j + 1], c02, c03, c12, c13, l0, l1);
+            const float2 q0 = unpack_half(h0[j]), q1 = unpack_half(h1[j]);
+            l0[j] = pack_half(p0.x - q0.x, p0.y - q0.y), l1[j] = pack_half(p1.x - q1.x, p1.y - q1.y);
+          }
+        };
+        if constexpr (KVU > 1) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) weights(j);
+        }
+#pragma unroll
+        for (int kv = 0; kv < KVU; ++kv) {
+          const bool mine = KVU == 1 || own == kv;
+          Words<NG> ca0, cb0, ca1, cb1;
+          const unsigned char* vr = vs + 8 * n * kQ4RowBytes + (unit * KVU + kv) * R::HEAD + 2 * NG * g;
+          ca0.load(vr + row_a * kQ4RowBytes);
+          cb0.load(vr + row_b * kQ4RowBytes);
+          ca1.load(vr + (8 + row_a) * kQ4RowBytes);
+          cb1.load(vr + (8 + row_b) * kQ4RowBytes);
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            if constexpr (KVU == 1) weights(j);
+            // half j of the rows: low 16 bits row a, high 16 bits row b
+            const uint32_t pick = j & 1 ? 0x7632u : 0x5410u;
+            const uint32_t z0 = __byte_perm(ca0.w[j / 2], cb0.w[j / 2], pick);
+            const uint32_t z1 = __byte_perm(ca1.w[j / 2], cb1.w[j / 2], pick);
+            const uint32_t c00 = codes_low(z0, magic), c01 = codes_high(z0, magic);
+            const uint32_t c02 = codes_low(z0 >> 8, magic), c03 = codes_high(z0 >> 8, magic);
+            const uint32_t c10 = codes_low(z1, magic), c11 = codes_high(z1, magic);
+            const uint32_t c12 = codes_low(z1 >> 8, magic), c13 = codes_high(z1 >> 8, magic);
+            const uint32_t p0 = mine ? h0[j] : 0u, p1 = mine ? h1[j] : 0u;
+            mma_f16(o[2 * j], c00, c01, c10, c11, p0, p1);
+            mma_f16(o[2 * j + 1], c02, c03, c12, c13, p0, p1);
+            if constexpr (PRECISE) {
+              const uint32_t q0 = mine ? l0[j] : 0u, q1 = mine ? l1[j] : 0u;
+              mma_f16(o[2 * j], c00, c01, c10, c11, q0, q1);
+              mma_f16(o[2 * j + 1], c02, c03, c12, c13, q0, q1);
+            }
           }
         }
       }
@@ -426,26 +532,25 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);
   sum += __shfl_xor_sync(0xffffffffu, sum, 1);
   sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-  if (t == 0 && g < M::G) stat[warp * M::G + g] = make_float2(m, sum);
+  if (t == 0) stat[warp * 8 + g] = make_float2(m, sum);
 #pragma unroll
   for (int e = 0; e < 2 * NG; ++e)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int head = 2 * t + (c & 1), dim = 16 * e + 8 * (c >> 1) + g;
-      if (head < M::G) red[(warp * M::G + head) * C::PITCH + dim] = o[e][c];
-    }
+    for (int c = 0; c < 4; ++c)
+      red[(warp * 8 + 2 * t + (c & 1)) * C::PITCH + 16 * e + 8 * (c >> 1) + g] = o[e][c];
   __syncthreads();
   for (int e = tid; e < M::HQ * M::D; e += kThreads) {
     const int qh = e / M::D, d = e - qh * M::D;
-    const int w0 = qh / M::G * C::WPH, head = qh - qh / M::G * M::G;
     float top = -INFINITY, num = 0.0f, den = 0.0f;
+    // the warps of this head's unit
 #pragma unroll
-    for (int w = 0; w < C::WPH; ++w) top = fmaxf(top, stat[(w0 + w) * M::G + head].x);
+    for (int w = 0; w < C::PARTS; ++w) top = fmaxf(top, stat[((qh >> 3) * C::PARTS + w) * 8 + (qh & 7)].x);
 #pragma unroll
-    for (int w = 0; w < C::WPH; ++w) {
-      const float2 ml = stat[(w0 + w) * M::G + head];
-      const float weight = C::WPH == 1 ? 1.0f : fast_exp2(ml.x - top);
-      num = fmaf(weight, red[((w0 + w) * M::G + head) * C::PITCH + d], num);
+    for (int w = 0; w < C::PARTS; ++w) {
+      const int at = ((qh >> 3) * C::PARTS + w) * 8 + (qh & 7);
+      const float2 ml = stat[at];
+      const float weight = fast_exp2(ml.x - top);
+      num = fmaf(weight, red[at * C::PITCH + d], num);
       den = fmaf(weight, ml.y, den);
     }
     if (nsplit > 1) {
@@ -454,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     } else {
       const float y = num / den;
       good &= isfinite(y);
-      store_any(p.out, unit * M::HQ * M::D + e, p.out_dtype, y);
+      store_any(p.out, cell * M::HQ * M::D + e, p.out_dtype, y);
     }
   }
   if (!good && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
@@ -535,7 +640,9 @@ cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int smem, c
 
 template <class M>
 cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
-  void (*fn)(Q4DecodeParams) = p.out_dtype == 0 ? qx_q4_decode_kernel<M, true> : qx_q4_decode_kernel<M, false>;
+  void (*fn)(Q4DecodeParams) = p.out_dtype == 0   ? qx_q4_decode_kernel<M, 0>
+                               : p.out_dtype == 1 ? qx_q4_decode_kernel<M, 1>
+                                                  : qx_q4_decode_kernel<M, 2>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   *launched = 0;

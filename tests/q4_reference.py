@@ -79,21 +79,24 @@ def values(codes, scales):
 
 
 def unpack_rows(model, raw, key):
-    """Codes [rows, heads, D] and scales [rows, heads, D / 32] of raw 288-byte
-    rows, by the layout include/qxcuda.h states."""
+    """Codes [rows, heads, D] (the value's code plus 7: 0..14) and scales
+    [rows, heads, D / 32] of raw 288-byte rows, by the layout include/qxcuda.h
+    states."""
     hkv, d = model_shape(model)[1:]
     ng = d // 32
     n = raw.shape[0]
     scales = np.ascontiguousarray(raw[:, 256:]).view(np.float16).reshape(n, hkv, ng)
     body = np.ascontiguousarray(raw[:, :256]).reshape(n, hkv, d // 2)
     codes = np.zeros((n, hkv, d), np.uint8)
+    words = body.view(np.uint32).astype(np.int64)
     for dim in range(d):
         j, r = dim // 32, dim % 32
         if key:
-            nibble = 8 * ((r // 8) * ng + j) + r % 8
+            w = words[:, :, (r // 8) * ng + j] >> (8 * (r % 4) + (4 if r % 8 < 4 else 0))
+            codes[:, :, dim] = ((w & 15) ^ 8) - 1  # two's complement plus 7
         else:
             nibble = 4 * ((r % 8) * ng + j) + r // 8
-        codes[:, :, dim] = (body[:, :, nibble // 2] >> (4 * (nibble % 2))) & 15
+            codes[:, :, dim] = (body[:, :, nibble // 2] >> (4 * (nibble % 2))) & 15
     return codes, scales
 
 

@@ -66,12 +66,20 @@ def test_token_strides():
 
 @pytest.mark.parametrize("model", [MODEL_GRANITE, MODEL_QWEN3])
 @pytest.mark.parametrize("key", [True, False])
-def test_the_stated_layout_uses_every_nibble_once(model, key):
-    rng = np.random.default_rng(1)
-    raw = rng.integers(0, 256, (3, 288), dtype=np.uint8)
-    codes, _ = ref.unpack_rows(model, raw, key)
-    nibbles = np.stack([raw[:, :256] & 15, raw[:, :256] >> 4], -1).reshape(3, -1)
-    assert np.array_equal(np.sort(codes.reshape(3, -1), 1), np.sort(nibbles, 1))
+def test_the_stated_layout_uses_every_bit_once(model, key):
+    """Each bit of the code bytes belongs to exactly one dim."""
+    base = np.zeros((1, 288), np.uint8)
+    owners = np.zeros((256, 8), np.int64)
+    start, _ = ref.unpack_rows(model, base, key)
+    for byte in range(256):
+        for bit in range(8):
+            raw = base.copy()
+            raw[0, byte] ^= 1 << bit
+            codes, _ = ref.unpack_rows(model, raw, key)
+            changed = np.flatnonzero(codes != start)
+            assert changed.size == 1
+            owners[byte, bit] = changed[0]
+    assert (np.bincount(owners.flatten(), minlength=512) == 4).all()
 
 
 def test_reference_quantiser_rounds_ties_to_even_and_keeps_the_largest():
