@@ -44,7 +44,8 @@ constexpr int kSide = kQ4Tile * kQ4RowBytes;  // bytes of a tile's keys, or valu
 constexpr int kStage = 2 * kSide;
 constexpr int kOffNew = kStages * kStage;               // a word and a scale per thread and pass: the new rows
 constexpr int kOffBar = kOffNew + 2 * kThreads * 8;
-constexpr int kSmem = kOffBar + 8 * kStages + 4 * kStages + 4;
+constexpr int kOffMagic = kOffBar + 8 * kStages + 4 * kStages;
+constexpr int kSmem = kOffMagic + 4;
 
 // The largest P' = 2^(x - m) * scale of a step is set to about 2^kTop when the
 // reference m moves, and m moves when it would pass 2^(kTop + kSlack), below
@@ -93,7 +94,8 @@ __device__ __forceinline__ uint32_t take_bytes(int* y, int shift) {
 }
 
 // Nibbles 0 and 4 of w (low: bits 0 and 16) as fp16 c - 7: 0x6400 | c is 1024 +
-// c. `magic` is 0x64006400 in a register: two constants would take two instructions.
+// c. `magic` is 0x64006400 in a register, read from memory so that it stays there:
+// with two constants the mask and the or are two instructions.
 __device__ __forceinline__ uint32_t codes_low(uint32_t w, uint32_t magic) {
   const uint32_t x = (w & 0x000f000fu) | magic;
   const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1031.0f));
@@ -258,9 +260,11 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
       mbar_init(&full[s], 1);
       done[s] = 0u;
     }
+    *reinterpret_cast<volatile uint32_t*>(sm + kOffMagic) = 0x64006400u;
     fence_barrier_init();
   }
   __syncthreads();
+  const uint32_t magic = *reinterpret_cast<volatile uint32_t*>(sm + kOffMagic);
   pdl_wait();
   pdl_launch_dependents();
   // where tile `k`'s rows are in the arena
@@ -317,13 +321,12 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   for (int m = 0; m < 2 * NG; ++m)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[m][e] = 0.0f;
-  float m = -INFINITY, sum = 0.0f;  // of query head g, this lane's rows
+  float m = -INFINITY;  // of query head g, this lane's rows
+  float2 sum = make_float2(0.0f, 0.0f);
   // the cache row that MMA row (or column) g stands for, and those of 2 t and 2 t + 1
   const int row_g = (g & 1) ? 4 + ((g >> 1) ^ 2) : g >> 1, row_a = t, row_b = 4 + (t ^ 2);
   const int own = KVU == 1 ? 0 : g / M::G;  // kv head of query head g within the unit
   const int scale_at = R::scale(unit * KVU + own, 0);
-  uint32_t magic;
-  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));  // opaque: kept in a register
   const int zero[4] = {kZeroBits, kZeroBits, kZeroBits, kZeroBits};
 
   for (int k = 0; k < tiles; ++k) {
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
       if (__any_sync(0xffffffffu, raise)) {
         const float keep = raise ? fast_exp2(m - top) : 1.0f;
         if (raise) m = top;
-        sum *= keep;
+        sum = __fmul2_rn(sum, make_float2(keep, keep));
         const float k0 = __shfl_sync(0xffffffffu, keep, 8 * t), k1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
 #pragma unroll
         for (int e = 0; e < 2 * NG; ++e) {
@@ -463,8 +466,9 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
       }
 #pragma unroll
       for (int n = 0; n < C::BLOCKS; ++n) {
-        x[n] = make_float2(fast_exp2(x[n].x - m), fast_exp2(x[n].y - m));
-        sum += x[n].x + x[n].y;
+        x[n] = __fadd2_rn(x[n], make_float2(-m, -m));
+        x[n] = make_float2(fast_exp2(x[n].x), fast_exp2(x[n].y));
+        sum = __fadd2_rn(sum, x[n]);
       }
       // ---- O^T += V^T P'^T, 16 rows at a time
 #pragma unroll
@@ -502,11 +506,11 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
             const uint32_t pick = j & 1 ? 0x7632u : 0x5410u;
             const uint32_t z0 = __byte_perm(ca0.w[j / 2], cb0.w[j / 2], pick);
             const uint32_t z1 = __byte_perm(ca1.w[j / 2], cb1.w[j / 2], pick);
+            const uint32_t p0 = mine ? h0[j] : 0u, p1 = mine ? h1[j] : 0u;
             const uint32_t c00 = codes_low(z0, magic), c01 = codes_high(z0, magic);
             const uint32_t c02 = codes_low(z0 >> 8, magic), c03 = codes_high(z0 >> 8, magic);
             const uint32_t c10 = codes_low(z1, magic), c11 = codes_high(z1, magic);
             const uint32_t c12 = codes_low(z1 >> 8, magic), c13 = codes_high(z1 >> 8, magic);
-            const uint32_t p0 = mine ? h0[j] : 0u, p1 = mine ? h1[j] : 0u;
             mma_f16(o[2 * j], c00, c01, c10, c11, p0, p1);
             mma_f16(o[2 * j + 1], c02, c03, c12, c13, p0, p1);
             if constexpr (PRECISE) {
@@ -530,9 +534,10 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   __syncthreads();  // every stage was read
   float* red = reinterpret_cast<float*>(sm);
   float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);
-  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-  if (t == 0) stat[warp * 8 + g] = make_float2(m, sum);
+  float all = sum.x + sum.y;
+  all += __shfl_xor_sync(0xffffffffu, all, 1);
+  all += __shfl_xor_sync(0xffffffffu, all, 2);
+  if (t == 0) stat[warp * 8 + g] = make_float2(m, all);
 #pragma unroll
   for (int e = 0; e < 2 * NG; ++e)
 #pragma unroll
