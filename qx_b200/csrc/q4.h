@@ -78,6 +78,8 @@ struct Q4DecodeParams {
   const float* q_norm;
   const float* k_norm;
   const float2* rope;
+  uint4* operands;  // rotated queries as MMA operands, per (sequence, layer) of the launch: see q4_operand_bytes
+  float* units;     // and [HQ] base-2 logits of their sums
   float* part_o;   // partials of split sequences: [item][HQ][D] sums
   float2* part_ml;  // and [item][HQ] (m, l)
   int q_dtype, in_dtype, out_dtype;
@@ -121,6 +123,9 @@ cudaError_t launch_q4_read(bool qwen, const Q4ReadParams& p, cudaStream_t stream
 cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream, int* launched);
 // Decode CTAs resident on one SM.
 int q4_decode_blocks_per_sm();
+// Bytes of the operands of one (sequence, layer): two 7-bit terms of every
+// element, four unless the output is bf16.
+constexpr size_t q4_operand_bytes(int heads, int d, int out_dtype) { return (size_t)heads * d * (out_dtype == 1 ? 2 : 4); }
 cudaError_t launch_packed(bool qwen, const PackedParams& p, cudaStream_t stream);
 
 }  // namespace qx

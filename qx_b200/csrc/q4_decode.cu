@@ -1,5 +1,10 @@
 // q4_decode.cu — one decode step over a 4-bit cache.
 //
+// qx_q4_prepare_kernel writes the new token's rows and the rotated queries as
+// MMA operands; qx_q4_decode_kernel attends; where a sequence was split,
+// qx_q4_merge_kernel joins the parts. Each is a programmatic dependent of the one
+// before.
+//
 // qx_q4_decode_kernel: a CTA takes one (sequence, layer) and one split of its
 // cached rows, all kv heads at once, so a run of rows is one contiguous piece
 // of memory (288 bytes a row). A warp takes a unit of eight query heads, one kv
@@ -42,8 +47,7 @@ constexpr int kThreads = 256;
 constexpr int kStages = 3;
 constexpr int kSide = kQ4Tile * kQ4RowBytes;  // bytes of a tile's keys, or values
 constexpr int kStage = 2 * kSide;
-constexpr int kOffNew = kStages * kStage;               // a word and a scale per thread and pass: the new rows
-constexpr int kOffBar = kOffNew + 2 * kThreads * 8;
+constexpr int kOffBar = kStages * kStage;
 constexpr int kOffMagic = kOffBar + 8 * kStages + 4 * kStages;
 constexpr int kSmem = kOffMagic + 4;
 
@@ -137,7 +141,6 @@ struct Dec {
   static constexpr int UNITS = M::HKV / KVU;
   static constexpr int PARTS = 8 / UNITS;         // of a tile's rows, a warp each
   static constexpr int ROWS = kQ4Tile / PARTS, BLOCKS = ROWS / 8;
-  static constexpr int PASSES = KVU * M::D / 128;  // of 32 lanes over the unit's new keys and values
   static constexpr int PITCH = M::D + 8;          // floats per head in the closing exchange
   static constexpr int OFF_STAT = 8 * 8 * PITCH * 4;
   static_assert(OFF_STAT + 8 * 8 * 8 <= kStages * kStage, "the closing exchange fits the stages");
@@ -161,7 +164,7 @@ struct Query {
 // Lane (g, t) holds dims 32 j + 8 t .. + 7 of query head g of the unit:
 // rotation pairs are in the lane, norms in the quad.
 template <class M, int PAIRS>
-__device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long first_head, int position, bool emit,
+__device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long first_head, int position,
                                            Query<M, PAIRS>* out) {
   constexpr int NG = M::D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -204,7 +207,7 @@ __device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long fi
       good &= isfinite(a) && isfinite(b);
       top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
     }
-  if (emit) {
+  if (p.q_rot_out) {
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
@@ -234,6 +237,54 @@ __device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long fi
   return good;
 }
 
+// Before the attention: per (sequence, layer) the queries normed (Qwen), rotated
+// and cut into operands, the new token's rows quantised into the arena. A warp
+// per unit of eight query heads, four for the keys' and values' heads.
+template <class M, int PAIRS>
+__global__ void __launch_bounds__(256) qx_q4_prepare_kernel(const __grid_constant__ Q4DecodeParams p) {
+  using C = Dec<M>;
+  using R = Q4Row<M>;
+  constexpr int NG = C::NG;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i = blockIdx.x / p.layer_count, layer = blockIdx.x - i * p.layer_count;
+  const Q4Seq seq = p.seqs[i];
+  const int position = seq.begin - 1;
+  const long long cell = (long long)p.seq_begin * p.layer_count + blockIdx.x;  // of the call
+  pdl_wait();
+  // The attention grid may start: every grid before this one has completed, so it
+  // may read all rows but the new ones, for which it waits.
+  pdl_launch_dependents();
+  bool good;
+  if (warp < C::UNITS) {
+    Query<M, PAIRS> query;
+    good = load_query<M, PAIRS>(p, cell * M::HQ + 8 * warp, position, &query);
+    uint4* out = p.operands + ((long long)blockIdx.x * C::UNITS + warp) * NG * PAIRS * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int a = 0; a < PAIRS; ++a)
+        out[(j * PAIRS + a) * 32] = make_uint4(query.a[j][a][0], query.a[j][a][1], query.a[j][a][2], query.a[j][a][3]);
+    if ((lane & 3) == 0) p.units[(long long)blockIdx.x * M::HQ + 8 * warp + (lane >> 2)] = query.unit;
+  } else {
+    const int at = 32 * (warp - C::UNITS) + lane, c = at & (R::LPH - 1), h = at / R::LPH % M::HKV;
+    const bool value = at >= M::HKV * R::LPH;  // the same for a whole warp
+    const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, position);
+    float x[8];
+    load8(value ? p.v : p.k, (cell * M::HKV + h) * M::D + 8 * c, p.in_dtype, p.vec, x);
+    int codes[8];
+    __half scale;
+    if (value) {
+      good = quantise8(x, codes, &scale);
+      put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, value_halves(codes), scale);
+    } else {
+      good = rotate_head<M>(x, c, position, p.k_norm, p.rope);
+      good &= quantise8(x, codes, &scale);
+      put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, key_codes(codes), scale);
+    }
+  }
+  if (!good) flag_error(p.err, QX_ERR_BIT_NONFINITE);
+}
+
 template <class M, int OUT>
 __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_constant__ Q4DecodeParams p) {
   using C = Dec<M>;
@@ -251,8 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   const int layer = (blockIdx.x - seq.first) / nsplit, split = (blockIdx.x - seq.first) - layer * nsplit;
   const long long cell = (long long)(p.seq_begin + i) * p.layer_count + layer;  // (sequence, layer) of the call
   const int row0 = split * p.chunk, row1 = min(row0 + p.chunk, attend), tiles = (row1 - row0 + kQ4Tile - 1) / kQ4Tile;
-  const bool last = row1 == attend;
-  const int held = last ? attend - 1 : row1;  // rows the cache holds before this call
+  const bool last = row1 == attend;  // this split's last tile has the new token's row
   bool ok = true;
 
   if (tid == 0) {
@@ -265,55 +315,38 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   }
   __syncthreads();
   const uint32_t magic = *reinterpret_cast<volatile uint32_t*>(sm + kOffMagic);
-  pdl_wait();
-  pdl_launch_dependents();
   // where tile `k`'s rows are in the arena
   auto tile_row = [&](int k) {
     return kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, row0 + k * kQ4Tile);
   };
   auto issue = [&](int k, long long row) {
-    const int s = k % kStages, n = min(kQ4Tile, held - (row0 + k * kQ4Tile));
-    if (n <= 0) {  // only the new token's row, which is written below
-      mbar_arrive(&full[s]);
-      return;
-    }
-    mbar_arrive_expect_tx(&full[s], 2u * n * kQ4RowBytes);
-    bulk_load(sm + s * kStage, p.arena.k + row * kQ4RowBytes, n * kQ4RowBytes, &full[s]);
-    bulk_load(sm + s * kStage + kSide, p.arena.v + row * kQ4RowBytes, n * kQ4RowBytes, &full[s]);
+    const int s = k % kStages;
+    const uint32_t bytes = min(kQ4Tile, row1 - (row0 + k * kQ4Tile)) * kQ4RowBytes;
+    mbar_arrive_expect_tx(&full[s], 2u * bytes);
+    bulk_load(sm + s * kStage, p.arena.k + row * kQ4RowBytes, bytes, &full[s]);
+    bulk_load(sm + s * kStage + kSide, p.arena.v + row * kQ4RowBytes, bytes, &full[s]);
   };
+  // Rows of earlier calls may be read before the wait: qx_q4_prepare_kernel, the
+  // grid before this one, lets this one start only when all before it are complete.
+  const int early = min(kStages, last ? tiles - 1 : tiles);
   if (tid == 0)
-    for (int k = 0; k < min(kStages, tiles); ++k) issue(k, tile_row(k));
+    for (int k = 0; k < early; ++k) issue(k, tile_row(k));
+  pdl_wait();
+  pdl_launch_dependents();
+  if (tid == 0 && early < min(kStages, tiles)) issue(early, tile_row(early));
 
   Query<M, PAIRS> query;
-  bool good = load_query<M, PAIRS>(p, cell * M::HQ + 8 * unit, attend - 1,
-                                     p.q_rot_out && split == 0 && part == 0, &query);
-
-  // The new token's rows of this unit's kv heads, D / 8 lanes each: the keys,
-  // then the values. The warp whose rows they fall among quantises them and puts
-  // them into its tile and the arena; no other warp reads them.
-  const int new_row = (attend - 1 - row0) & (kQ4Tile - 1);
-  const bool owner = last && new_row / C::ROWS == part;
-  uint2* fresh = reinterpret_cast<uint2*>(sm + kOffNew) + tid;
-  if (owner) {
+  {
+    const long long here = cell - (long long)p.seq_begin * p.layer_count;  // within the launch
+    const uint4* in = p.operands + (here * C::UNITS + unit) * NG * PAIRS * 32 + lane;
 #pragma unroll
-    for (int a = 0; a < C::PASSES; ++a) {
-      const int at = 32 * a + lane, c = at & (R::LPH - 1);
-      const bool value = at >= KVU * R::LPH;
-      const int h = unit * KVU + at / R::LPH % KVU;
-      float x[8], y[8];
-      load8(value ? p.v : p.k, (cell * M::HKV + h) * M::D + 8 * c, p.in_dtype, p.vec, x);
+    for (int j = 0; j < NG; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e];
-      const bool rotated = rotate_head<M>(y, c, attend - 1, p.k_norm, p.rope);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = value ? x[e] : y[e];
-      good &= value || rotated;
-      int codes[8];
-      __half scale;
-      good &= quantise8(x, codes, &scale);
-      const uint32_t halves = value_halves(codes);
-      fresh[a * kThreads] = make_uint2(value ? halves : key_codes(codes), __half_as_ushort(scale));
-    }
+      for (int a = 0; a < PAIRS; ++a) {
+        const uint4 w = in[(j * PAIRS + a) * 32];
+        query.a[j][a][0] = w.x, query.a[j][a][1] = w.y, query.a[j][a][2] = w.z, query.a[j][a][3] = w.w;
+      }
+    query.unit = p.units[here * M::HQ + 8 * unit + g];
   }
 
   float o[2 * NG][4];
@@ -337,24 +370,6 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     const long long next = refill && lane == 0 ? tile_row(k + kStages) : 0;
     ok &= mbar_wait_bounded(&full[s], (uint32_t)(k / kStages) & 1u, p.err);
     __syncwarp();
-    if (owner && k == tiles - 1) {
-      const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, attend - 1);
-#pragma unroll
-      for (int a = 0; a < C::PASSES; ++a) {
-        const int at = 32 * a + lane, c = at & (R::LPH - 1), h = unit * KVU + at / R::LPH % KVU;
-        char* into = reinterpret_cast<char*>(tile) + new_row * kQ4RowBytes;
-        const uint2 x = fresh[a * kThreads];
-        const __half scale = __ushort_as_half((unsigned short)x.y);
-        if (at < KVU * R::LPH) {
-          put_key<M>(into, h, c, x.x, scale);
-          put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, x.x, scale);
-        } else {
-          put_value<M>(into + kSide, h, c, x.x, scale);
-          put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, x.x, scale);
-        }
-      }
-      __syncwarp();
-    }
     const int r0 = C::ROWS * part;
     if (r0 < valid) {
       const unsigned char* ks = tile + r0 * kQ4RowBytes;
@@ -533,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   // ---- the warps' sums meet in shared memory ------------------------------------
   __syncthreads();  // every stage was read
   float* red = reinterpret_cast<float*>(sm);
-  float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);
+  float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);  // [warp][8]: (m, l), then the weight in .x
   float all = sum.x + sum.y;
   all += __shfl_xor_sync(0xffffffffu, all, 1);
   all += __shfl_xor_sync(0xffffffffu, all, 2);
@@ -544,27 +559,49 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     for (int c = 0; c < 4; ++c)
       red[(warp * 8 + 2 * t + (c & 1)) * C::PITCH + 16 * e + 8 * (c >> 1) + g] = o[e][c];
   __syncthreads();
-  for (int e = tid; e < M::HQ * M::D; e += kThreads) {
-    const int qh = e / M::D, d = e - qh * M::D;
-    float top = -INFINITY, num = 0.0f, den = 0.0f;
-    // the warps of this head's unit
-#pragma unroll
-    for (int w = 0; w < C::PARTS; ++w) top = fmaxf(top, stat[((qh >> 3) * C::PARTS + w) * 8 + (qh & 7)].x);
+  if (tid < M::HQ) {  // each head: what the warps of its unit count for
+    float2* mine = stat + (tid >> 3) * C::PARTS * 8 + (tid & 7);
+    float2 ml[C::PARTS];
+    float top = -INFINITY, den = 0.0f;
 #pragma unroll
     for (int w = 0; w < C::PARTS; ++w) {
-      const int at = ((qh >> 3) * C::PARTS + w) * 8 + (qh & 7);
-      const float2 ml = stat[at];
-      const float weight = fast_exp2(ml.x - top);
-      num = fmaf(weight, red[at * C::PITCH + d], num);
-      den = fmaf(weight, ml.y, den);
+      ml[w] = mine[w * 8];
+      top = fmaxf(top, ml[w].x);
+    }
+#pragma unroll
+    for (int w = 0; w < C::PARTS; ++w) {
+      ml[w].x = fast_exp2(ml[w].x - top);
+      den = fmaf(ml[w].x, ml[w].y, den);
+    }
+    if (nsplit > 1) p.part_ml[(long long)blockIdx.x * M::HQ + tid] = make_float2(top, den);
+    const float unit_weight = nsplit > 1 ? 1.0f : 1.0f / den;
+#pragma unroll
+    for (int w = 0; w < C::PARTS; ++w) mine[w * 8].x = ml[w].x * unit_weight;
+  }
+  __syncthreads();
+  bool good = true;
+#pragma unroll
+  for (int e = 4 * tid; e < M::HQ * M::D; e += 4 * kThreads) {
+    const int qh = e / M::D, d = e - qh * M::D;
+    const int at = (qh >> 3) * C::PARTS * 8 + (qh & 7);
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < C::PARTS; ++w) {
+      const float weight = stat[at + w * 8].x;
+      const float4 v = *reinterpret_cast<const float4*>(red + (at + w * 8) * C::PITCH + d);
+      y.x = fmaf(weight, v.x, y.x);
+      y.y = fmaf(weight, v.y, y.y);
+      y.z = fmaf(weight, v.z, y.z);
+      y.w = fmaf(weight, v.w, y.w);
     }
     if (nsplit > 1) {
-      p.part_o[(long long)blockIdx.x * M::HQ * M::D + e] = num;
-      if (d == 0) p.part_ml[(long long)blockIdx.x * M::HQ + qh] = make_float2(top, den);
+      *reinterpret_cast<float4*>(p.part_o + (long long)blockIdx.x * M::HQ * M::D + e) = y;
     } else {
-      const float y = num / den;
-      good &= isfinite(y);
-      store_any(p.out, cell * M::HQ * M::D + e, p.out_dtype, y);
+      good &= isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w);
+      store_any(p.out, cell * M::HQ * M::D + e, OUT, y.x);
+      store_any(p.out, cell * M::HQ * M::D + e + 1, OUT, y.y);
+      store_any(p.out, cell * M::HQ * M::D + e + 2, OUT, y.z);
+      store_any(p.out, cell * M::HQ * M::D + e + 3, OUT, y.w);
     }
   }
   if (!good && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
@@ -629,10 +666,11 @@ __global__ void __launch_bounds__(256) qx_q4_merge_kernel(const __grid_constant_
   }
 }
 
-cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int smem, cudaStream_t stream, const Q4DecodeParams& p) {
+cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int threads, int smem, cudaStream_t stream,
+                             const Q4DecodeParams& p, int* launched) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -640,30 +678,30 @@ cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int smem, c
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p);
+  if (e == cudaSuccess) ++*launched;
+  return e;
 }
 
-template <class M>
+template <class M, int OUT>
 cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
-  void (*fn)(Q4DecodeParams) = p.out_dtype == 0   ? qx_q4_decode_kernel<M, 0>
-                               : p.out_dtype == 1 ? qx_q4_decode_kernel<M, 1>
-                                                  : qx_q4_decode_kernel<M, 2>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  cudaError_t e = cudaFuncSetAttribute(qx_q4_decode_kernel<M, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  *launched = 0;
-  e = launch_dependent(fn, p.items, kSmem, stream, p);
-  if (e != cudaSuccess) return e;
-  ++*launched;
-  if (!p.split) return e;
-  e = launch_dependent(qx_q4_merge_kernel<M>, p.n_seq * p.layer_count * M::HQ * (M::D / 32), 0, stream, p);
-  if (e == cudaSuccess) ++*launched;
+  const int cells = p.n_seq * p.layer_count;
+  e = launch_dependent(qx_q4_prepare_kernel<M, Need<OUT>::PAIRS>, cells, 32 * (Dec<M>::UNITS + 4), 0, stream, p, launched);
+  if (e == cudaSuccess) e = launch_dependent(qx_q4_decode_kernel<M, OUT>, p.items, kThreads, kSmem, stream, p, launched);
+  if (e == cudaSuccess && p.split)
+    e = launch_dependent(qx_q4_merge_kernel<M>, cells * M::HQ * (M::D / 32), kThreads, 0, stream, p, launched);
   return e;
 }
 
 }  // namespace
 
 cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
-  return qwen ? decode<Qwen3Heads>(p, stream, launched) : decode<GraniteHeads>(p, stream, launched);
+  *launched = 0;
+  if (p.out_dtype == 0) return qwen ? decode<Qwen3Heads, 0>(p, stream, launched) : decode<GraniteHeads, 0>(p, stream, launched);
+  if (p.out_dtype == 1) return qwen ? decode<Qwen3Heads, 1>(p, stream, launched) : decode<GraniteHeads, 1>(p, stream, launched);
+  return qwen ? decode<Qwen3Heads, 2>(p, stream, launched) : decode<GraniteHeads, 2>(p, stream, launched);
 }
 
 int q4_decode_blocks_per_sm() { return 2; }

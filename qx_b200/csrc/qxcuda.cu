@@ -98,7 +98,7 @@ struct qxc_ctx {
   // 4-bit decode's and packed prefill's workspaces; the buffers they have
   // outgrown are kept until the context goes, since a captured graph may
   // still name them
-  Workspace q4_parts, packed_rot;
+  Workspace q4_work, packed_rot;
   std::vector<void*> outgrown;
   // prefill's rotated-query scratch (bf16 elements)
   unsigned short* prefill_q = nullptr;
@@ -1205,14 +1205,17 @@ qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
     }
     if (items > 0x7fffffffLL) return fail(ctx, QXC_ERR_INVALID_ARG, "too much work in one call");
     p.items = (int)items;
-    if (p.split) {
-      // partials of every item: [HQ][D] sums, then [HQ] (m, l)
-      const size_t heads = (size_t)items * kv->hq;
-      qxc_status st = reserve(ctx, &ctx->q4_parts, heads * (kv->d * sizeof(float) + sizeof(float2)));
-      if (st != QXC_OK) return st;
-      p.part_o = reinterpret_cast<float*>(ctx->q4_parts.ptr);
-      p.part_ml = reinterpret_cast<float2*>(ctx->q4_parts.ptr + heads * kv->d * sizeof(float));
-    }
+    // workspace: the queries' operands and their units, then, where a sequence is
+    // split, the partials of every item: [HQ][D] sums, then [HQ] (m, l)
+    const size_t cells = (size_t)n * a->layer_count, heads = p.split ? (size_t)items * kv->hq : 0;
+    const size_t operands = cells * q4_operand_bytes(kv->hq, kv->d, a->out_dtype);
+    const size_t units = (cells * kv->hq * sizeof(float) + 15) / 16 * 16, sums = heads * kv->d * sizeof(float);
+    qxc_status st = reserve(ctx, &ctx->q4_work, operands + units + sums + heads * sizeof(float2));
+    if (st != QXC_OK) return st;
+    p.operands = reinterpret_cast<uint4*>(ctx->q4_work.ptr);
+    p.units = reinterpret_cast<float*>(ctx->q4_work.ptr + operands);
+    p.part_o = reinterpret_cast<float*>(ctx->q4_work.ptr + operands + units);
+    p.part_ml = reinterpret_cast<float2*>(ctx->q4_work.ptr + operands + units + sums);
     int launched = 0;
     QXC_CUDA(ctx, launch_q4_decode(is_qwen(kv), p, ctx->stream, &launched));
     ctx->launches += launched;
@@ -1377,7 +1380,7 @@ void qxc_destroy(qxc_ctx* ctx) {
   cudaFree(ctx->stack_f);
   cudaFree(ctx->stack_words);
   cudaFree(ctx->prefill_q);
-  cudaFree(ctx->q4_parts.ptr);
+  cudaFree(ctx->q4_work.ptr);
   cudaFree(ctx->packed_rot.ptr);
   for (void* p : ctx->outgrown) cudaFree(p);
   if (ctx->err_host) cudaFreeHost(ctx->err_host);
