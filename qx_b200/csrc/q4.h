@@ -67,9 +67,12 @@ struct Q4DecodeParams {
   int layer_begin, layer_count;
   int n_seq;
   int seq_begin;  // index of seqs[0] among the call's sequences
-  int chunk;      // cache rows per split, a multiple of kQ4Tile
-  int items;      // (sequence, layer, split) of this launch
-  int split;      // some sequence has several splits: qx_q4_merge_kernel follows
+  // The launch's cells, (sequence, layer) in order, lie one after another on a
+  // line of tiles; CTA b attends tiles [b * per_cta, (b + 1) * per_cta) of it.
+  int per_cta;
+  int total;      // tiles of the line
+  int padded;     // a cell's place is rounded up to whole CTAs (a split the caller asked for)
+  int max_parts;  // CTAs that share a cell, at most; above 1 qx_q4_merge_kernel follows
   const void* q;  // [sequence][layer][HQ * D]
   const void* k;  // [sequence][layer][HKV * D]
   const void* v;
@@ -80,16 +83,15 @@ struct Q4DecodeParams {
   const float2* rope;
   uint4* operands;  // rotated queries as MMA operands, per (sequence, layer) of the launch: see q4_operand_bytes
   float* units;     // and [HQ] base-2 logits of their sums
-  float* part_o;   // partials of split sequences: [item][HQ][D] sums
-  float2* part_ml;  // and [item][HQ] (m, l)
+  float* part_o;    // of cells shared by CTAs: [CTA][2][HQ][D] sums (slot 0: the CTA's first cell, 1: its last)
+  float2* part_ml;  // and [CTA][2][HQ] (m, l)
   int q_dtype, in_dtype, out_dtype;
   int vec;  // q, k and v allow 16-byte loads
   unsigned* err;
-  Q4Seq seqs[kQ4Seqs];  // begin: rows attended, the new token's among them; first: first work item
+  Q4Seq seqs[kQ4Seqs];  // begin: rows attended, the new token's among them; first: its place on the line
 };
 
-constexpr int kQ4Tile = 64;  // cache rows per pipeline stage; pages hold a multiple of it
-constexpr int kQ4MaxSplits = 1024;
+constexpr int kQ4Tile = 32;  // cache rows per pipeline stage; pages hold a multiple of it
 
 // One prompt of a packed call: its first packed token, its length, its first
 // work item in the launch.

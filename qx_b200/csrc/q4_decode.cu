@@ -5,13 +5,17 @@
 // qx_q4_merge_kernel joins the parts. Each is a programmatic dependent of the one
 // before.
 //
-// qx_q4_decode_kernel: a CTA takes one (sequence, layer) and one split of its
-// cached rows, all kv heads at once, so a run of rows is one contiguous piece
-// of memory (288 bytes a row). A warp takes a unit of eight query heads, one kv
-// head of Qwen or four of Granite, and a half (Granite: a quarter) of every
-// tile's rows:
-//   copies   tiles of 64 rows, keys and values, by bulk copies into a ring of
-//            three stages; the last warp to finish a tile refills its stage
+// qx_q4_decode_kernel: all (sequence, layer) cells of a launch lie on one line of
+// tiles of 32 rows, and every CTA, two an SM, takes the same length of it: the
+// stream of rows never stops between cells, and no CTA has more rows than
+// another. A CTA attends all kv heads, so a tile is one contiguous piece of
+// memory a side (288 bytes a row). Two groups of four warps take alternate tiles;
+// a warp takes a unit of eight query heads, one kv head of Qwen or four of
+// Granite (and then half of the tile's rows):
+//   copies   by bulk copies into a ring of four stages, two a group; the last
+//            warp of a group to finish a tile refills its stage. (A stage belongs
+//            to one group: a warp is then never two phases ahead of a barrier,
+//            which its parity could not tell from none.)
 //   scores   S = Q K^T by mma.m16n8k32 on 8-bit integers, exact: K's codes are
 //            8-bit integers as they lie in the row but for a mask, a query is
 //            rounded once to an integer of 15 bits (29 unless the output is bf16)
@@ -44,12 +48,14 @@ namespace qx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kStages = 3;
+constexpr int kStages = 4;
 constexpr int kSide = kQ4Tile * kQ4RowBytes;  // bytes of a tile's keys, or values
 constexpr int kStage = 2 * kSide;
-constexpr int kOffBar = kStages * kStage;
-constexpr int kOffMagic = kOffBar + 8 * kStages + 4 * kStages;
-constexpr int kSmem = kOffMagic + 4;
+
+// The next tile a group's stages take: its place on the line and its cell.
+struct Cursor {
+  int at, seq, layer, tile, tiles;
+};
 
 // The largest P' = 2^(x - m) * scale of a step is set to about 2^kTop when the
 // reference m moves, and m moves when it would pass 2^(kTop + kSlack), below
@@ -139,11 +145,18 @@ struct Dec {
   static constexpr int NG = M::D / 32;
   static constexpr int KVU = 8 / M::G;            // kv heads of a unit of eight query heads
   static constexpr int UNITS = M::HKV / KVU;
-  static constexpr int PARTS = 8 / UNITS;         // of a tile's rows, a warp each
+  static constexpr int PARTS = 4 / UNITS;         // of a tile's rows, a warp each
   static constexpr int ROWS = kQ4Tile / PARTS, BLOCKS = ROWS / 8;
+  static constexpr int WARPS = 2 * PARTS;         // of a unit, both groups
   static constexpr int PITCH = M::D + 8;          // floats per head in the closing exchange
-  static constexpr int OFF_STAT = 8 * 8 * PITCH * 4;
-  static_assert(OFF_STAT + 8 * 8 * 8 <= kStages * kStage, "the closing exchange fits the stages");
+  static constexpr int OFF_RED = kStages * kStage;
+  static constexpr int OFF_STAT = OFF_RED + 8 * 8 * PITCH * 4;
+  static constexpr int OFF_BAR = OFF_STAT + 8 * 8 * 8;
+  static constexpr int OFF_DONE = OFF_BAR + 8 * kStages;
+  static constexpr int OFF_CURSOR = OFF_DONE + 4 * kStages;
+  static constexpr int OFF_MAGIC = OFF_CURSOR + 2 * (int)sizeof(Cursor);
+  static constexpr int SMEM = OFF_MAGIC + 4;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
 // What an output type asks for: queries of four terms of 7 bits (else two),
@@ -292,52 +305,81 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
   constexpr int NG = C::NG, KVU = C::KVU, PAIRS = Need<OUT>::PAIRS;
   constexpr bool PRECISE = Need<OUT>::WEIGHT;
   extern __shared__ __align__(128) unsigned char sm[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm + kOffBar);
-  unsigned* done = reinterpret_cast<unsigned*>(full + kStages);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+  unsigned* done = reinterpret_cast<unsigned*>(sm + C::OFF_DONE);
+  Cursor* cursor = reinterpret_cast<Cursor*>(sm + C::OFF_CURSOR);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int part = warp % C::PARTS, unit = warp / C::PARTS;
-  const int i = find_seq(p.seqs, p.n_seq, blockIdx.x);
-  const Q4Seq seq = p.seqs[i];
-  const int attend = seq.begin, nsplit = (attend + p.chunk - 1) / p.chunk;
-  const int layer = (blockIdx.x - seq.first) / nsplit, split = (blockIdx.x - seq.first) - layer * nsplit;
-  const long long cell = (long long)(p.seq_begin + i) * p.layer_count + layer;  // (sequence, layer) of the call
-  const int row0 = split * p.chunk, row1 = min(row0 + p.chunk, attend), tiles = (row1 - row0 + kQ4Tile - 1) / kQ4Tile;
-  const bool last = row1 == attend;  // this split's last tile has the new token's row
+  const int group = warp >> 2, unit = (warp & 3) / C::PARTS, part = warp & (C::PARTS - 1);
+  // this CTA's stretch of the line, and the cell it starts in
+  const int start = blockIdx.x * p.per_cta;
+  auto tiles_of = [&](int i) { return (p.seqs[i].begin + kQ4Tile - 1) / kQ4Tile; };
+  int seq = find_seq(p.seqs, p.n_seq, start), tiles = tiles_of(seq);
+  const int place = p.padded ? (tiles + p.per_cta - 1) / p.per_cta * p.per_cta : tiles;
+  int layer = (start - p.seqs[seq].first) / place, tile = (start - p.seqs[seq].first) - layer * place;
+  const int end = p.padded ? start + min(p.per_cta, tiles - tile) : min(start + p.per_cta, p.total);
   bool ok = true;
 
+  // one tile further
+  auto advance = [&](Cursor& c) {
+    ++c.at;
+    if (++c.tile < c.tiles) return;
+    c.tile = 0;
+    if (++c.layer == p.layer_count) {
+      c.layer = 0;
+      if (++c.seq < p.n_seq) c.tiles = tiles_of(c.seq);
+    }
+  };
+  auto issue = [&](const Cursor& c) {
+    const int s = (c.at - start) % kStages, begin = c.tile * kQ4Tile;
+    const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, p.seqs[c.seq].seq,
+                                 p.layer_begin + c.layer, begin);
+    const uint32_t bytes = min(kQ4Tile, p.seqs[c.seq].begin - begin) * kQ4RowBytes;
+    mbar_arrive_expect_tx(&full[s], 2u * bytes);
+    bulk_load(sm + s * kStage, p.arena.k + row * kQ4RowBytes, bytes, &full[s]);
+    bulk_load(sm + s * kStage + kSide, p.arena.v + row * kQ4RowBytes, bytes, &full[s]);
+  };
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       done[s] = 0u;
     }
-    *reinterpret_cast<volatile uint32_t*>(sm + kOffMagic) = 0x64006400u;
+    *reinterpret_cast<volatile uint32_t*>(sm + C::OFF_MAGIC) = 0x64006400u;
     fence_barrier_init();
+    // Rows of earlier calls may be read before the wait: qx_q4_prepare_kernel, the
+    // grid before this one, lets this one start only when all before it are
+    // complete. A cell's last tile has the row which that grid writes.
+    Cursor c = {start, seq, layer, tile, tiles};
+    bool waited = false;
+    for (int k = 0; k < kStages && c.at < end; ++k) {
+      if (c.tile == c.tiles - 1 && !waited) {
+        pdl_wait();
+        waited = true;
+      }
+      issue(c);
+      advance(c);
+    }
+    cursor[c.at & 1 ^ start & 1] = c;
+    advance(c);
+    cursor[c.at & 1 ^ start & 1] = c;
   }
   __syncthreads();
-  const uint32_t magic = *reinterpret_cast<volatile uint32_t*>(sm + kOffMagic);
-  // where tile `k`'s rows are in the arena
-  auto tile_row = [&](int k) {
-    return kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, row0 + k * kQ4Tile);
-  };
-  auto issue = [&](int k, long long row) {
-    const int s = k % kStages;
-    const uint32_t bytes = min(kQ4Tile, row1 - (row0 + k * kQ4Tile)) * kQ4RowBytes;
-    mbar_arrive_expect_tx(&full[s], 2u * bytes);
-    bulk_load(sm + s * kStage, p.arena.k + row * kQ4RowBytes, bytes, &full[s]);
-    bulk_load(sm + s * kStage + kSide, p.arena.v + row * kQ4RowBytes, bytes, &full[s]);
-  };
-  // Rows of earlier calls may be read before the wait: qx_q4_prepare_kernel, the
-  // grid before this one, lets this one start only when all before it are complete.
-  const int early = min(kStages, last ? tiles - 1 : tiles);
-  if (tid == 0)
-    for (int k = 0; k < early; ++k) issue(k, tile_row(k));
+  const uint32_t magic = *reinterpret_cast<volatile uint32_t*>(sm + C::OFF_MAGIC);
   pdl_wait();
   pdl_launch_dependents();
-  if (tid == 0 && early < min(kStages, tiles)) issue(early, tile_row(early));
 
+  // the cache row that MMA row (or column) g stands for, and those of 2 t and 2 t + 1
+  const int row_g = (g & 1) ? 4 + ((g >> 1) ^ 2) : g >> 1, row_a = t, row_b = 4 + (t ^ 2);
+  const int own = KVU == 1 ? 0 : g / M::G;  // kv head of query head g within the unit
+  const int scale_at = R::scale(unit * KVU + own, 0);
+  const int zero[4] = {kZeroBits, kZeroBits, kZeroBits, kZeroBits};
+  bool good = true;
+
+  for (int at = start; at < end;) {  // cell by cell
+  const int n_tiles = min(end - at, tiles - tile);  // of this cell in this CTA
+  const int attend = p.seqs[seq].begin;
+  const long long here = (long long)seq * p.layer_count + layer;  // the cell within the launch
   Query<M, PAIRS> query;
   {
-    const long long here = cell - (long long)p.seq_begin * p.layer_count;  // within the launch
     const uint4* in = p.operands + (here * C::UNITS + unit) * NG * PAIRS * 32 + lane;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
@@ -356,23 +398,16 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     for (int e = 0; e < 4; ++e) o[m][e] = 0.0f;
   float m = -INFINITY;  // of query head g, this lane's rows
   float2 sum = make_float2(0.0f, 0.0f);
-  // the cache row that MMA row (or column) g stands for, and those of 2 t and 2 t + 1
-  const int row_g = (g & 1) ? 4 + ((g >> 1) ^ 2) : g >> 1, row_a = t, row_b = 4 + (t ^ 2);
-  const int own = KVU == 1 ? 0 : g / M::G;  // kv head of query head g within the unit
-  const int scale_at = R::scale(unit * KVU + own, 0);
-  const int zero[4] = {kZeroBits, kZeroBits, kZeroBits, kZeroBits};
 
-  for (int k = 0; k < tiles; ++k) {
-    const int s = k % kStages;
-    unsigned char* tile = sm + s * kStage;
-    const int valid = min(kQ4Tile, row1 - (row0 + k * kQ4Tile));
-    const bool refill = k + kStages < tiles;
-    const long long next = refill && lane == 0 ? tile_row(k + kStages) : 0;
-    ok &= mbar_wait_bounded(&full[s], (uint32_t)(k / kStages) & 1u, p.err);
+  for (int k = (at - start + group) & 1; k < n_tiles; k += 2) {  // this group's tiles
+    const int kk = at - start + k, s = kk % kStages;
+    unsigned char* data = sm + s * kStage;
+    const int valid = min(kQ4Tile, attend - (tile + k) * kQ4Tile);
+    ok &= mbar_wait_bounded(&full[s], (uint32_t)(kk / kStages) & 1u, p.err);
     __syncwarp();
     const int r0 = C::ROWS * part;
     if (r0 < valid) {
-      const unsigned char* ks = tile + r0 * kQ4RowBytes;
+      const unsigned char* ks = data + r0 * kQ4RowBytes;
       const unsigned char* vs = ks + kSide;
       // ---- scores: x[n] = rows 8 n + row_a, 8 n + row_b of head g, Granite's two
       // blocks at a time so that its masked operands serve both
@@ -537,17 +572,25 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
         }
       }
     }
-    // the last warp to finish a tile refills its stage
+    // the last warp of the group to finish a tile refills its stage
     __syncwarp();
-    if (refill && lane == 0 && count_up(&done[s]) == 7u) {
+    if (lane == 0 && count_up(&done[s]) == 3u) {
       done[s] = 0u;
-      issue(k + kStages, next);
+      Cursor c = cursor[group];
+      if (c.at < end) {
+        issue(c);
+        advance(c);
+        advance(c);
+        cursor[group] = c;
+      }
     }
   }
 
   // ---- the warps' sums meet in shared memory ------------------------------------
-  __syncthreads();  // every stage was read
-  float* red = reinterpret_cast<float*>(sm);
+  const bool whole = n_tiles == tiles;
+  const long long slot = 2ll * blockIdx.x + (at == start ? 0 : 1);
+  __syncthreads();  // the last cell's sums were read
+  float* red = reinterpret_cast<float*>(sm + C::OFF_RED);
   float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);  // [warp][8]: (m, l), then the weight in .x
   float all = sum.x + sum.y;
   all += __shfl_xor_sync(0xffffffffu, all, 1);
@@ -559,111 +602,126 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     for (int c = 0; c < 4; ++c)
       red[(warp * 8 + 2 * t + (c & 1)) * C::PITCH + 16 * e + 8 * (c >> 1) + g] = o[e][c];
   __syncthreads();
+  // warp w of unit u
+  auto warp_of = [](int u, int w) { return w / C::PARTS * 4 + u * C::PARTS + w % C::PARTS; };
   if (tid < M::HQ) {  // each head: what the warps of its unit count for
-    float2* mine = stat + (tid >> 3) * C::PARTS * 8 + (tid & 7);
-    float2 ml[C::PARTS];
+    float2 ml[C::WARPS];
     float top = -INFINITY, den = 0.0f;
 #pragma unroll
-    for (int w = 0; w < C::PARTS; ++w) {
-      ml[w] = mine[w * 8];
+    for (int w = 0; w < C::WARPS; ++w) {
+      ml[w] = stat[warp_of(tid >> 3, w) * 8 + (tid & 7)];
       top = fmaxf(top, ml[w].x);
     }
 #pragma unroll
-    for (int w = 0; w < C::PARTS; ++w) {
+    for (int w = 0; w < C::WARPS; ++w) {
       ml[w].x = fast_exp2(ml[w].x - top);
       den = fmaf(ml[w].x, ml[w].y, den);
     }
-    if (nsplit > 1) p.part_ml[(long long)blockIdx.x * M::HQ + tid] = make_float2(top, den);
-    const float unit_weight = nsplit > 1 ? 1.0f : 1.0f / den;
+    if (!whole) p.part_ml[slot * M::HQ + tid] = make_float2(top, den);
+    const float scale = whole ? 1.0f / den : 1.0f;
 #pragma unroll
-    for (int w = 0; w < C::PARTS; ++w) mine[w * 8].x = ml[w].x * unit_weight;
+    for (int w = 0; w < C::WARPS; ++w) stat[warp_of(tid >> 3, w) * 8 + (tid & 7)].x = ml[w].x * scale;
   }
   __syncthreads();
-  bool good = true;
 #pragma unroll
   for (int e = 4 * tid; e < M::HQ * M::D; e += 4 * kThreads) {
     const int qh = e / M::D, d = e - qh * M::D;
-    const int at = (qh >> 3) * C::PARTS * 8 + (qh & 7);
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < C::PARTS; ++w) {
-      const float weight = stat[at + w * 8].x;
-      const float4 v = *reinterpret_cast<const float4*>(red + (at + w * 8) * C::PITCH + d);
+    for (int w = 0; w < C::WARPS; ++w) {
+      const int from = warp_of(qh >> 3, w) * 8 + (qh & 7);
+      const float weight = stat[from].x;
+      const float4 v = *reinterpret_cast<const float4*>(red + from * C::PITCH + d);
       y.x = fmaf(weight, v.x, y.x);
       y.y = fmaf(weight, v.y, y.y);
       y.z = fmaf(weight, v.z, y.z);
       y.w = fmaf(weight, v.w, y.w);
     }
-    if (nsplit > 1) {
-      *reinterpret_cast<float4*>(p.part_o + (long long)blockIdx.x * M::HQ * M::D + e) = y;
+    if (!whole) {
+      *reinterpret_cast<float4*>(p.part_o + slot * M::HQ * M::D + e) = y;
     } else {
       good &= isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w);
-      store_any(p.out, cell * M::HQ * M::D + e, OUT, y.x);
-      store_any(p.out, cell * M::HQ * M::D + e + 1, OUT, y.y);
-      store_any(p.out, cell * M::HQ * M::D + e + 2, OUT, y.z);
-      store_any(p.out, cell * M::HQ * M::D + e + 3, OUT, y.w);
+      const long long out = ((long long)p.seq_begin * p.layer_count + here) * M::HQ * M::D + e;
+      store_any(p.out, out, OUT, y.x);
+      store_any(p.out, out + 1, OUT, y.y);
+      store_any(p.out, out + 2, OUT, y.z);
+      store_any(p.out, out + 3, OUT, y.w);
     }
+  }
+  at += n_tiles;
+  tile = 0;
+  if (++layer == p.layer_count) {
+    layer = 0;
+    if (++seq < p.n_seq) tiles = tiles_of(seq);
+  }
   }
   if (!good && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
 }
 
-// The partials of a split (sequence, layer): a CTA joins 32 dims of one query
-// head, eight lanes of four dims for each of 32 shares of the splits.
-template <class M>
+// Cells shared by CTAs: a CTA joins 1024 / SHARES outputs of a cell, SHARES
+// threads (of neighbouring 256 / SHARES) taking every SHARES-th part of the same
+// four. One share where cells have few parts, 32 (then 32 dims of one head)
+// where they have many.
+template <class M, int SHARES>
 __global__ void __launch_bounds__(256) qx_q4_merge_kernel(const __grid_constant__ Q4DecodeParams p) {
-  constexpr int SLICES = M::D / 32;
-  __shared__ float red[32][33];
-  __shared__ float tops[8], dens[32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int slice = blockIdx.x % SLICES, qh = blockIdx.x / SLICES % M::HQ, rel = blockIdx.x / (SLICES * M::HQ);
-  const int i = rel / p.layer_count, layer = rel - i * p.layer_count;
-  const Q4Seq seq = p.seqs[i];
-  const int nsplit = (seq.begin + p.chunk - 1) / p.chunk;
-  if (nsplit == 1) return;
+  constexpr int E = 1024 / SHARES, SLICES = M::HQ * M::D / E, LANES = 256 / SHARES;
+  __shared__ float red[SHARES == 1 ? 1 : SHARES][E + 4];
+  __shared__ float2 stat[SHARES];
+  const int tid = threadIdx.x, slice = blockIdx.x % SLICES, cell = blockIdx.x / SLICES;
+  const int i = cell / p.layer_count, layer = cell - i * p.layer_count;
+  const int tiles = (p.seqs[i].begin + kQ4Tile - 1) / kQ4Tile;
+  const int place = p.padded ? (tiles + p.per_cta - 1) / p.per_cta * p.per_cta : tiles;
+  const int first = p.seqs[i].first + layer * place;
+  const int b0 = first / p.per_cta, parts = (first + tiles - 1) / p.per_cta - b0 + 1;
+  if (parts == 1) return;
   pdl_wait();
-  const long long item0 = seq.first + (long long)layer * nsplit;
-  const float2* ml = p.part_ml + item0 * M::HQ + qh;
-  float top = -INFINITY;
-  for (int s = tid; s < nsplit; s += 256) top = fmaxf(top, ml[(long long)s * M::HQ].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) tops[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, tops[w]);
-  const int share = tid >> 3, c = tid & 7;
-  const float* po = p.part_o + (item0 * M::HQ + qh) * M::D + 32 * slice + 4 * c;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float den = 0.0f;
+  const int share = tid / LANES, e = slice * E + 4 * (tid % LANES), qh = e / M::D;
+  // the first part lies in slot 1 of its CTA unless it is the CTA's first cell
+  auto slot = [&](int s) { return 2ll * (b0 + s) + (s == 0 && first != b0 * p.per_cta ? 1 : 0); };
+  float top = -INFINITY, den = 0.0f;
+  for (int s = share; s < parts; s += SHARES) top = fmaxf(top, p.part_ml[slot(s) * M::HQ + qh].x);
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int s = share; s < nsplit; s += 32) {
-    const float2 x = ml[(long long)s * M::HQ];
-    const float4 v = *reinterpret_cast<const float4*>(po + (long long)s * M::HQ * M::D);
-    const float w = fast_exp2(x.x - top);
-    den = fmaf(w, x.y, den);
-    acc.x = fmaf(w, v.x, acc.x);
-    acc.y = fmaf(w, v.y, acc.y);
-    acc.z = fmaf(w, v.z, acc.z);
-    acc.w = fmaf(w, v.w, acc.w);
+  for (int s = share; s < parts; s += SHARES) {
+    const float2 ml = p.part_ml[slot(s) * M::HQ + qh];
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(s) * M::HQ * M::D + e);
+    const float w = fast_exp2(ml.x - top);
+    den = fmaf(w, ml.y, den);
+    y.x = fmaf(w, v.x, y.x);
+    y.y = fmaf(w, v.y, y.y);
+    y.z = fmaf(w, v.z, y.z);
+    y.w = fmaf(w, v.w, y.w);
   }
-  red[share][4 * c] = acc.x;
-  red[share][4 * c + 1] = acc.y;
-  red[share][4 * c + 2] = acc.z;
-  red[share][4 * c + 3] = acc.w;
-  if (c == 0) dens[share] = den;
-  __syncthreads();
-  if (warp == 0) {
-    float num = 0.0f, all = 0.0f;
+  const long long out = ((long long)p.seq_begin * p.layer_count + cell) * M::HQ * M::D;
+  bool good = true;
+  if constexpr (SHARES == 1) {
+    const float o[4] = {y.x / den, y.y / den, y.z / den, y.w / den};
 #pragma unroll
-    for (int s = 0; s < 32; ++s) {
-      num += red[s][lane];
-      all += dens[s];
+    for (int c = 0; c < 4; ++c) {
+      good &= isfinite(o[c]);
+      store_any(p.out, out + e + c, p.out_dtype, o[c]);
     }
-    const float y = num / all;
-    if (!isfinite(y)) flag_error(p.err, QX_ERR_BIT_NONFINITE);
-    const long long unit = (long long)(p.seq_begin + i) * p.layer_count + layer;
-    store_any(p.out, (unit * M::HQ + qh) * M::D + 32 * slice + lane, p.out_dtype, y);
+  } else {
+    static_assert(SHARES == 1 || M::D % E == 0, "a CTA's outputs are one head's");
+    *reinterpret_cast<float4*>(&red[share][4 * (tid % LANES)]) = y;
+    if (tid % LANES == 0) stat[share] = make_float2(top, den);
+    __syncthreads();
+    if (tid < E) {
+      float all = -INFINITY, num = 0.0f, sum = 0.0f;
+#pragma unroll 8
+      for (int s = 0; s < SHARES; ++s) all = fmaxf(all, stat[s].x);
+#pragma unroll 8
+      for (int s = 0; s < SHARES; ++s) {
+        const float w = fast_exp2(stat[s].x - all);
+        sum = fmaf(w, stat[s].y, sum);
+        num = fmaf(w, red[s][tid], num);
+      }
+      const float o = num / sum;
+      good = isfinite(o);
+      store_any(p.out, out + slice * E + tid, p.out_dtype, o);
+    }
   }
+  if (!good) flag_error(p.err, QX_ERR_BIT_NONFINITE);
 }
 
 cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int threads, int smem, cudaStream_t stream,
@@ -685,14 +743,17 @@ cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int threads
 
 template <class M, int OUT>
 cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
-  cudaError_t e = cudaFuncSetAttribute(qx_q4_decode_kernel<M, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  constexpr int SMEM = Dec<M>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(qx_q4_decode_kernel<M, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) return e;
-  const int cells = p.n_seq * p.layer_count;
+  const int cells = p.n_seq * p.layer_count, ctas = (p.total + p.per_cta - 1) / p.per_cta;
   e = launch_dependent(qx_q4_prepare_kernel<M, Need<OUT>::PAIRS>, cells, 32 * (Dec<M>::UNITS + 4), 0, stream, p, launched);
-  if (e == cudaSuccess) e = launch_dependent(qx_q4_decode_kernel<M, OUT>, p.items, kThreads, kSmem, stream, p, launched);
-  if (e == cudaSuccess && p.split)
-    e = launch_dependent(qx_q4_merge_kernel<M>, cells * M::HQ * (M::D / 32), kThreads, 0, stream, p, launched);
-  return e;
+  if (e == cudaSuccess) e = launch_dependent(qx_q4_decode_kernel<M, OUT>, ctas, kThreads, SMEM, stream, p, launched);
+  if (e != cudaSuccess || p.max_parts == 1) return e;
+  constexpr int OUTPUTS = M::HQ * M::D;
+  if (p.max_parts <= 8)
+    return launch_dependent(qx_q4_merge_kernel<M, 1>, cells * (OUTPUTS / 1024), 256, 0, stream, p, launched);
+  return launch_dependent(qx_q4_merge_kernel<M, 32>, cells * (OUTPUTS / 32), 256, 0, stream, p, launched);
 }
 
 }  // namespace

@@ -1164,20 +1164,18 @@ qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a, int q_d
   });
 }
 
+// Tiles that a CTA of a 4-bit decode takes at least: two (a group of warps each)
+// on the shortest lines, up to eight once that leaves a CTA for every SM.
+int q4_least_tiles(int total, int sms) { return std::max(2, std::min(8, (total + sms - 1) / sms)); }
+
 // One decode step on a 4-bit arena, its arguments checked and its pages mapped.
 qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
   std::vector<int32_t> attend(a->seq_count), ones(a->seq_count, 1);
   for (int i = 0; i < a->seq_count; ++i) attend[i] = a->positions[i] + 1;
-  int chunk = a->split;
-  if (chunk == 0)
-    chunk = auto_chunk(ctx->sm_count * q4_decode_blocks_per_sm(), attend.data(), a->seq_count, a->layer_count,
-                       kQ4MaxSplits, kQ4Tile);
-  ctx->last_split = chunk;
   Q4DecodeParams p;
   p.arena = q4_arena(kv);
   p.layer_begin = a->layer_begin;
   p.layer_count = a->layer_count;
-  p.chunk = chunk;
   p.q = a->q;
   p.k = a->k;
   p.v = a->v;
@@ -1195,19 +1193,31 @@ qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
     memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
     p.n_seq = n;
     p.seq_begin = first;
-    p.split = 0;
-    long long items = 0;
+    p.padded = a->split > 0 ? 1 : 0;
+    p.per_cta = a->split / kQ4Tile;
+    auto tiles_of = [&](int i) { return (p.seqs[i].begin + kQ4Tile - 1) / kQ4Tile; };
+    long long total = 0;
     for (int i = 0; i < n; ++i) {
-      const int nsplit = (seqs[i].begin + chunk - 1) / chunk;
-      p.seqs[i].first = (int)items;
-      items += (long long)nsplit * a->layer_count;
-      if (nsplit > 1) p.split = 1;
+      const int place = p.padded ? (tiles_of(i) + p.per_cta - 1) / p.per_cta * p.per_cta : tiles_of(i);
+      p.seqs[i].first = (int)total;
+      total += (long long)place * a->layer_count;
+      if (total > 0x3fffffffLL) return fail(ctx, QXC_ERR_INVALID_ARG, "too much work in one call");
     }
-    if (items > 0x7fffffffLL) return fail(ctx, QXC_ERR_INVALID_ARG, "too much work in one call");
-    p.items = (int)items;
-    // workspace: the queries' operands and their units, then, where a sequence is
-    // split, the partials of every item: [HQ][D] sums, then [HQ] (m, l)
-    const size_t cells = (size_t)n * a->layer_count, heads = p.split ? (size_t)items * kv->hq : 0;
+    p.total = (int)total;
+    // every CTA the GPU holds at once takes the same stretch of the line
+    const int slots = q4_decode_blocks_per_sm() * ctx->sm_count;
+    if (!p.padded) p.per_cta = std::max(q4_least_tiles(p.total, ctx->sm_count), (p.total + slots - 1) / slots);
+    ctx->last_split = p.per_cta * kQ4Tile;
+    const int ctas = (p.total + p.per_cta - 1) / p.per_cta;
+    p.max_parts = 1;
+    for (int i = 0; i < n; ++i) {  // a cell between two borders of its own touches a CTA more than it fills
+      const int tiles = tiles_of(i);
+      const int parts = p.padded ? (tiles + p.per_cta - 1) / p.per_cta : tiles > 1 ? (tiles - 2) / p.per_cta + 2 : 1;
+      p.max_parts = std::max(p.max_parts, std::min(parts, ctas));
+    }
+    // workspace: the queries' operands and their units, then, where cells may be
+    // shared by CTAs, two partials a CTA: [HQ][D] sums, then [HQ] (m, l)
+    const size_t cells = (size_t)n * a->layer_count, heads = p.max_parts > 1 ? 2 * (size_t)ctas * kv->hq : 0;
     const size_t operands = cells * q4_operand_bytes(kv->hq, kv->d, a->out_dtype);
     const size_t units = (cells * kv->hq * sizeof(float) + 15) / 16 * 16, sums = heads * kv->d * sizeof(float);
     qxc_status st = reserve(ctx, &ctx->q4_work, operands + units + sums + heads * sizeof(float2));
