@@ -12,7 +12,7 @@
 // memory a side (288 bytes a row). Two groups of four warps take alternate tiles;
 // a warp takes a unit of eight query heads, one kv head of Qwen or four of
 // Granite (and then half of the tile's rows):
-//   copies   by bulk copies into a ring of four stages, two a group; the last
+//   copies   by bulk copies into a ring of six stages, three a group; the last
 //            warp of a group to finish a tile refills its stage. (A stage belongs
 //            to one group: a warp is then never two phases ahead of a barrier,
 //            which its parity could not tell from none.)
@@ -48,7 +48,7 @@ namespace qx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kStages = 4;
+constexpr int kStages = 6;
 constexpr int kSide = kQ4Tile * kQ4RowBytes;  // bytes of a tile's keys, or values
 constexpr int kStage = 2 * kSide;
 
@@ -148,9 +148,9 @@ struct Dec {
   static constexpr int PARTS = 4 / UNITS;         // of a tile's rows, a warp each
   static constexpr int ROWS = kQ4Tile / PARTS, BLOCKS = ROWS / 8;
   static constexpr int WARPS = 2 * PARTS;         // of a unit, both groups
-  static constexpr int PITCH = M::D + 8;          // floats per head in the closing exchange
-  static constexpr int OFF_RED = kStages * kStage;
-  static constexpr int OFF_STAT = OFF_RED + 8 * 8 * PITCH * 4;
+  static constexpr int OWN = 2 * NG / WARPS;      // blocks of 16 dims that a warp of a unit writes out
+  static constexpr int OFF_SWAP = kStages * kStage;   // [warp][lane] float4
+  static constexpr int OFF_STAT = OFF_SWAP + 8 * 32 * 16;  // [warp][8 heads] (m, l)
   static constexpr int OFF_BAR = OFF_STAT + 8 * 8 * 8;
   static constexpr int OFF_DONE = OFF_BAR + 8 * kStages;
   static constexpr int OFF_CURSOR = OFF_DONE + 4 * kStages;
@@ -586,66 +586,64 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     }
   }
 
-  // ---- the warps' sums meet in shared memory ------------------------------------
-  const bool whole = n_tiles == tiles;
-  const long long slot = 2ll * blockIdx.x + (at == start ? 0 : 1);
-  __syncthreads();  // the last cell's sums were read
-  float* red = reinterpret_cast<float*>(sm + C::OFF_RED);
-  float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);  // [warp][8]: (m, l), then the weight in .x
-  float all = sum.x + sum.y;
-  all += __shfl_xor_sync(0xffffffffu, all, 1);
-  all += __shfl_xor_sync(0xffffffffu, all, 2);
-  if (t == 0) stat[warp * 8 + g] = make_float2(m, all);
-#pragma unroll
-  for (int e = 0; e < 2 * NG; ++e)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      red[(warp * 8 + 2 * t + (c & 1)) * C::PITCH + 16 * e + 8 * (c >> 1) + g] = o[e][c];
-  __syncthreads();
-  // warp w of unit u
-  auto warp_of = [](int u, int w) { return w / C::PARTS * 4 + u * C::PARTS + w % C::PARTS; };
-  if (tid < M::HQ) {  // each head: what the warps of its unit count for
-    float2 ml[C::WARPS];
+  // ---- the sums of a unit's warps meet: each warp of the unit writes OWN blocks of
+  // 16 dims and gets the others' shares of them through shared memory, one block a
+  // round (a fragment is the same lanes' in every warp)
+  {
+    const bool whole = n_tiles == tiles;
+    const long long slot = 2ll * blockIdx.x + (at == start ? 0 : 1);
+    const int w = group * C::PARTS + part;  // this warp among its unit's
+    auto warp_of = [&](int i) { return i / C::PARTS * 4 + unit * C::PARTS + i % C::PARTS; };
+    float2* stat = reinterpret_cast<float2*>(sm + C::OFF_STAT);
+    float4* swap = reinterpret_cast<float4*>(sm + C::OFF_SWAP);
+    float all = sum.x + sum.y;
+    all += __shfl_xor_sync(0xffffffffu, all, 1);
+    all += __shfl_xor_sync(0xffffffffu, all, 2);
+    if (t == 0) stat[warp * 8 + g] = make_float2(m, all);
+    named_sync(1 + unit, 32 * C::WARPS);
     float top = -INFINITY, den = 0.0f;
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) {
-      ml[w] = stat[warp_of(tid >> 3, w) * 8 + (tid & 7)];
-      top = fmaxf(top, ml[w].x);
+    for (int i = 0; i < C::WARPS; ++i) top = fmaxf(top, stat[warp_of(i) * 8 + g].x);
+#pragma unroll
+    for (int i = 0; i < C::WARPS; ++i) {
+      const float2 ml = stat[warp_of(i) * 8 + g];
+      den = fmaf(fast_exp2(ml.x - top), ml.y, den);
     }
+    if (!whole && w == 0 && t == 0) p.part_ml[slot * M::HQ + 8 * unit + g] = make_float2(top, den);
+    const float scale = fast_exp2(m - top) * (whole ? 1.0f / den : 1.0f);
+    const float k0 = __shfl_sync(0xffffffffu, scale, 8 * t), k1 = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
+    auto block = [&](int e) {  // the fragment of dims 16 e .., scaled
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) {
-      ml[w].x = fast_exp2(ml[w].x - top);
-      den = fmaf(ml[w].x, ml[w].y, den);
-    }
-    if (!whole) p.part_ml[slot * M::HQ + tid] = make_float2(top, den);
-    const float scale = whole ? 1.0f / den : 1.0f;
+      for (int i = 0; i < 2 * NG; ++i)
+        if (i == e) v = make_float4(o[i][0] * k0, o[i][1] * k1, o[i][2] * k0, o[i][3] * k1);
+      return v;
+    };
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) stat[warp_of(tid >> 3, w) * 8 + (tid & 7)].x = ml[w].x * scale;
-  }
-  __syncthreads();
+    for (int b = 0; b < C::OWN; ++b) {
+      const int mine = w * C::OWN + b;
+      float4 v = block(mine);
 #pragma unroll
-  for (int e = 4 * tid; e < M::HQ * M::D; e += 4 * kThreads) {
-    const int qh = e / M::D, d = e - qh * M::D;
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) {
-      const int from = warp_of(qh >> 3, w) * 8 + (qh & 7);
-      const float weight = stat[from].x;
-      const float4 v = *reinterpret_cast<const float4*>(red + from * C::PITCH + d);
-      y.x = fmaf(weight, v.x, y.x);
-      y.y = fmaf(weight, v.y, y.y);
-      y.z = fmaf(weight, v.z, y.z);
-      y.w = fmaf(weight, v.w, y.w);
-    }
-    if (!whole) {
-      *reinterpret_cast<float4*>(p.part_o + slot * M::HQ * M::D + e) = y;
-    } else {
-      good &= isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w);
-      const long long out = ((long long)p.seq_begin * p.layer_count + here) * M::HQ * M::D + e;
-      store_any(p.out, out, OUT, y.x);
-      store_any(p.out, out + 1, OUT, y.y);
-      store_any(p.out, out + 2, OUT, y.z);
-      store_any(p.out, out + 3, OUT, y.w);
+      for (int r = 1; r < C::WARPS; ++r) {
+        swap[warp * 32 + lane] = block((w + r) % C::WARPS * C::OWN + b);
+        named_sync(1 + unit, 32 * C::WARPS);
+        const float4 x = swap[warp_of((w + C::WARPS - r) % C::WARPS) * 32 + lane];
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        named_sync(1 + unit, 32 * C::WARPS);
+      }
+      // heads 2 t and 2 t + 1, dims 16 mine + g and 8 further
+      const long long e = (8 * unit + 2 * t) * M::D + 16 * mine + g;
+      if (!whole) {
+        float* out = p.part_o + slot * M::HQ * M::D + e;
+        out[0] = v.x, out[M::D] = v.y, out[8] = v.z, out[M::D + 8] = v.w;
+      } else {
+        good &= isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
+        const long long out = ((long long)p.seq_begin * p.layer_count + here) * M::HQ * M::D + e;
+        store_any(p.out, out, OUT, v.x);
+        store_any(p.out, out + M::D, OUT, v.y);
+        store_any(p.out, out + 8, OUT, v.z);
+        store_any(p.out, out + M::D + 8, OUT, v.w);
+      }
     }
   }
   at += n_tiles;
