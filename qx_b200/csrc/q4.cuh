@@ -92,12 +92,12 @@ __device__ __forceinline__ void store8(void* base, long long i, int dtype, bool 
   }
 }
 
-// 1 / sqrt(mean + 1e-6) rounded once to f32. The sum of squares is a double
-// (products of two 16-bit inputs and their sum are exact in it), so its order
-// does not matter: quantised keys sit next to rounding borders, where an ulp
+// 1 / sqrt(mean + 1e-6) of a key head, rounded once to f32. The sum of squares is
+// a double (products of two 16-bit inputs and their sum are exact in it), so its
+// order does not matter: quantised keys sit next to rounding borders, where an ulp
 // of the norm would decide a code.
 template <class M>
-__device__ __forceinline__ float head_inv_rms(const float* x) {
+__device__ __forceinline__ float key_inv_rms(const float* x) {
   double sum = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum = fma((double)x[e], (double)x[e], sum);
@@ -106,20 +106,20 @@ __device__ __forceinline__ float head_inv_rms(const float* x) {
   return (float)rsqrt(sum * (1.0 / M::D) + 1.0e-6);
 }
 
-// Norm (Qwen) and rotation of this lane's eight dims of a head at `position`.
+// Of key heads: norm (Qwen) and rotation of this lane's eight dims of a head at `position`.
 // The operation order is each model's: granite_rope_pair's fused pair
 // (qx-consensus-math lib.rs:199-207), cpu_qk_norm_rope's separately rounded
-// one (qx-qwen-parity main.rs:1170-1210). False when a result is not finite.
+// one (qx-qwen-parity main.rs:1170-1210). tab: the table's entries of these dims
+// (rope_of_lane). False when a result is not finite.
 template <class M>
-__device__ __forceinline__ bool rotate_head(float* x, int c, int position, const float* norm, const float2* rope) {
+__device__ __forceinline__ bool rotate_key(float* x, int c, const float* norm, const float2* tab) {
   constexpr int LPH = Q4Row<M>::LPH;
   if constexpr (M::QWEN) {
-    const float inv = head_inv_rms<M>(x);
+    const float inv = key_inv_rms<M>(x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inv), norm ? norm[8 * c + e] : 1.0f);
   }
   const bool right = c >= LPH / 2;
-  const float2* tab = rope + (long long)position * (M::D / 2) + 8 * (c & (LPH / 2 - 1));
   bool good = true;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -135,6 +135,19 @@ __device__ __forceinline__ bool rotate_head(float* x, int c, int position, const
   return good;
 }
 
+// The rotation table's entries of lane c's dims at `position`.
+template <class M>
+__device__ __forceinline__ void rope_of_lane(const float2* rope, int position, int c, float2* tab) {
+  const float4* from = reinterpret_cast<const float4*>(rope + (long long)position * (M::D / 2) +
+                                                       8 * (c & (Q4Row<M>::LPH / 2 - 1)));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float4 v = from[e];
+    tab[2 * e] = make_float2(v.x, v.y);
+    tab[2 * e + 1] = make_float2(v.z, v.w);
+  }
+}
+
 // Codes -7..7 of this lane's eight dims and its group's scale. False when the scale is not finite: a value above 7 * 65504, an
 // infinity, or a NaN (which fmaxf alone would drop).
 __device__ __forceinline__ bool quantise8(const float* x, int* codes, __half* scale) {
@@ -147,11 +160,32 @@ __device__ __forceinline__ bool quantise8(const float* x, int* codes, __half* sc
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const __half h = __float2half_rn(__fdiv_rn(top, 7.0f));
+  // top / 7, correctly rounded: one multiplication and a correction by its
+  // residual (compared with the division for all 2^23 mantissas)
+  constexpr float SEVENTH = 1.0f / 7.0f;
+  const float guess = __fmul_rn(top, SEVENTH);
+  const __half h = __float2half_rn(__fmaf_rn(__fmaf_rn(-7.0f, guess, top), SEVENTH, guess));
   const float s = __half2float(h);
+  // x / s rounded to an integer: a product with the approximate reciprocal is off
+  // by less than 2^-19 of a step, so only quotients closer than that to a border
+  // between two codes need the division itself
+  float inv;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  float border = 1.0f;  // the smallest distance of a quotient from a border
 #pragma unroll
-  for (int e = 0; e < 8; ++e)  // a scale that rounds to zero: every value is zero
-    codes[e] = s > 0.0f ? __float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f)) : 0;
+  for (int e = 0; e < 8; ++e) {
+    const float q = x[e] * inv, n = rintf(q);
+    border = fminf(border, 0.5f - fabsf(q - n));
+    codes[e] = __float2int_rn(fminf(fmaxf(n, -7.0f), 7.0f));
+  }
+  if (border < 3.0e-6f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) codes[e] = __float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f));
+  }
+  if (!(s > 0.0f)) {  // a scale that rounds to zero: every value is zero
+#pragma unroll
+    for (int e = 0; e < 8; ++e) codes[e] = 0;
+  }
   *scale = h;
   return good && isfinite(s);
 }

@@ -44,7 +44,7 @@ struct Q4AppendParams {
   const float* q_norm;
   const float* k_norm;
   const float2* rope;  // Granite: (sin, cos); Qwen: (cos, sin); [position][D / 2]
-  int q_dtype, in_dtype, rot_dtype;
+  int in_dtype, rot_dtype;
   int vec;  // q, k, v and their strides allow 16-byte loads, q_rot and k_rot 16-byte stores
   unsigned* err;
   Q4Seq seqs[kQ4Seqs];

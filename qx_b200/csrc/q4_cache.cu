@@ -11,89 +11,236 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A warp takes 32 / LPH neighbouring heads of one (token, layer), in the
-// order query heads, key heads, value heads: D / 8 lanes a head, eight dims a
-// lane, 16-byte loads of 16-bit inputs.
-template <class M>
-__global__ void __launch_bounds__(kThreads) qx_q4_append_kernel(const __grid_constant__ Q4AppendParams p) {
+// N neighbouring elements as loaded, f32 (WIDE) or two 16-bit ones to a word;
+// VEC: 16-byte aligned rows. Types that the compiler knows, so that no load waits
+// for another's branch.
+template <int N, bool WIDE, bool VEC>
+struct Raw {
+  uint32_t w[WIDE ? N : N / 2];
+  __device__ __forceinline__ void load(const void* base, long long i) {
+    if constexpr (WIDE) {
+      const float* p = reinterpret_cast<const float*>(base) + i;
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        if constexpr (VEC) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p + e);
+          w[e] = u.x, w[e + 1] = u.y, w[e + 2] = u.z, w[e + 3] = u.w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[e + k] = __float_as_uint(p[e + k]);
+        }
+      }
+    } else {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + i;
+      if constexpr (VEC && N == 8) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+      } else if constexpr (VEC) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) w[e] = (uint32_t)p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
+      }
+    }
+  }
+  // elements 2 e and 2 e + 1
+  __device__ __forceinline__ float2 pair(int e, bool bf16) const {
+    if constexpr (WIDE) return make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+    if (bf16) return make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+  }
+};
+
+__device__ __forceinline__ void store4(void* base, long long i, int dtype, bool vec, const float* x) {
+  if (!vec) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_any(base, i + e, dtype, x[e]);
+  } else if (dtype == 0) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (dtype == 1) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b);
+      } else {
+        const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(base) + i) = make_uint2(w[0], w[1]);
+  }
+}
+
+// Four warps take one (token, layer): each a quarter of the query heads and half
+// of the key or value heads, D / 8 lanes a head. A key's or value's lane has eight
+// neighbouring dims; a query's has dims 4 c .. 4 c + 3 and the four that they are
+// rotated with, so that it needs no other lane but for the norm. A lane has the
+// same dims in all its heads: it loads its rotation and norm weights once, and all
+// its inputs before it uses the first.
+template <class M, bool WIDE, bool VEC>
+__global__ void __launch_bounds__(kThreads, WIDE ? 3 : 4) qx_q4_append_kernel(const __grid_constant__ Q4AppendParams p) {
   using R = Q4Row<M>;
-  constexpr int HPW = 32 / R::LPH;  // heads per warp
-  const int lane = threadIdx.x & 31, c = lane & (R::LPH - 1);
-  const int q_heads = p.q ? M::HQ : 0;
-  const int warps = (q_heads + 2 * M::HKV) / HPW;  // per (token, layer)
-  const long long w = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const long long unit = w / warps;
+  constexpr int HPW = 32 / R::LPH;         // heads per warp at once
+  constexpr int PASSES = M::HQ / HPW / 4;  // of query heads per warp
+  constexpr int HALF = M::D / 2;
+  static_assert(M::HKV == 2 * HPW, "a warp's half of the key or value heads is one pass");
+  const int lane = threadIdx.x & 31, c = lane & (R::LPH - 1), sub = lane / R::LPH;
+  const int quarter = (threadIdx.x >> 5) & 3;
+  const unsigned unit = blockIdx.x * (kThreads / 128) + (threadIdx.x >> 7);
   pdl_wait();
-  if (unit >= (long long)p.token_count * p.layer_count) return;
-  int head = (int)(w - unit * warps) * HPW + lane / R::LPH;
-  const int token = p.token_begin + (int)(unit / p.layer_count), l = (int)(unit % p.layer_count);
+  if (unit >= (unsigned)p.token_count * p.layer_count) return;
+  const unsigned step = p.layer_count == 1 ? unit : unit / p.layer_count;
+  const int token = p.token_begin + (int)step, l = (int)(unit - step * p.layer_count);
+  const bool value = quarter >= 2;
+  const int kv = (quarter & 1) * HPW + sub;       // key or value head
+  const int q0 = quarter * PASSES * HPW + sub;    // first query head
+  const bool bf16 = p.in_dtype == 1;
+  Raw<8, WIDE, VEC> y;
+  y.load(value ? p.v : p.k, token * (value ? p.v_stride : p.k_stride) + ((long long)l * M::HKV + kv) * M::D + 8 * c);
+  Raw<4, WIDE, VEC> x[PASSES][2];
+  if (p.q) {
+    const long long from = token * p.q_stride + ((long long)l * M::HQ + q0) * M::D + 4 * c;
+#pragma unroll
+    for (int a = 0; a < PASSES; ++a) {
+      x[a][0].load(p.q, from + a * HPW * M::D);
+      x[a][1].load(p.q, from + a * HPW * M::D + HALF);
+    }
+  }
   const Q4Seq s = p.seqs[find_seq(p.seqs, p.n_seq, token)];
   const int position = s.begin + token - s.first;
-  float x[8];
+  const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq, p.layer_begin + l, position);
+  const long long cell = (long long)token * p.layer_count + l;
   bool good = true;
-  if (head < q_heads) {
-    load8(p.q, token * p.q_stride + ((long long)l * M::HQ + head) * M::D + 8 * c, p.q_dtype, p.vec, x);
-    good = rotate_head<M>(x, c, position, p.q_norm, p.rope);
-    store8(p.q_rot, (((long long)token * p.layer_count + l) * M::HQ + head) * M::D + 8 * c, p.rot_dtype, p.vec, x);
-  } else {
-    head -= q_heads;
-    const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq, p.layer_begin + l, position);
+  {
+    float f[8];
     int codes[8];
     __half scale;
-    if (head < M::HKV) {
-      load8(p.k, token * p.k_stride + ((long long)l * M::HKV + head) * M::D + 8 * c, p.in_dtype, p.vec, x);
-      good = rotate_head<M>(x, c, position, p.k_norm, p.rope);
-      if (p.k_rot)
-        store8(p.k_rot, (((long long)token * p.layer_count + l) * M::HKV + head) * M::D + 8 * c, p.rot_dtype, p.vec, x);
-      good &= quantise8(x, codes, &scale);
-      put_key<M>(p.arena.k + row * kQ4RowBytes, head, c, key_codes(codes), scale);
-    } else {
-      head -= M::HKV;
-      load8(p.v, token * p.v_stride + ((long long)l * M::HKV + head) * M::D + 8 * c, p.in_dtype, p.vec, x);
-      good = quantise8(x, codes, &scale);
-      put_value<M>(p.arena.v + row * kQ4RowBytes, head, c, value_halves(codes), scale);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 z = y.pair(e, bf16);
+      f[2 * e] = z.x, f[2 * e + 1] = z.y;
     }
+    if (value) {
+      good = quantise8(f, codes, &scale);
+      put_value<M>(p.arena.v + row * kQ4RowBytes, kv, c, value_halves(codes), scale);
+    } else {
+      float2 tab[8];
+      rope_of_lane<M>(p.rope, position, c, tab);
+      good = rotate_key<M>(f, c, p.k_norm, tab);
+      if (p.k_rot) store8(p.k_rot, (cell * M::HKV + kv) * M::D + 8 * c, p.rot_dtype, VEC, f);
+      good &= quantise8(f, codes, &scale);
+      put_key<M>(p.arena.k + row * kQ4RowBytes, kv, c, key_codes(codes), scale);
+    }
+  }
+  if (p.q) {
+    // pairs of neighbouring dims: (cos, cos) and (sin, sin), norm weights
+    float2 cs[2], sn[2], w[4];
+    {
+      const float4* from = reinterpret_cast<const float4*>(p.rope + (long long)position * HALF + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 v = from[e];
+        cs[e] = M::QWEN ? make_float2(v.x, v.z) : make_float2(v.y, v.w);
+        sn[e] = M::QWEN ? make_float2(v.y, v.w) : make_float2(v.x, v.z);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 4 * c + 2 * (e & 1) + (e >> 1) * HALF;
+        w[e] = M::QWEN && p.q_norm ? make_float2(p.q_norm[d], p.q_norm[d + 1]) : make_float2(1.0f, 1.0f);
+      }
+    }
+    float2 bad = make_float2(0.0f, 0.0f);  // NaN once a result is not finite
+#pragma unroll
+    for (int a = 0; a < PASSES; ++a) {
+      float2 v[4];  // dims 4 c + 0, 1; + 2, 3; and their partners
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = x[a][e >> 1].pair(e & 1, bf16);
+      if constexpr (M::QWEN) {
+        const float2 s2 = __fadd2_rn(__ffma2_rn(v[0], v[0], __fmul2_rn(v[1], v[1])), __ffma2_rn(v[2], v[2], __fmul2_rn(v[3], v[3])));
+        float sum = s2.x + s2.y;
+#pragma unroll
+        for (int o = R::LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = rsqrtf(fmaf(sum, 1.0f / M::D, 1.0e-6f));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(__fmul2_rn(v[e], make_float2(inv, inv)), w[e]);
+      }
+      float out[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 minus = make_float2(-sn[e].x, -sn[e].y);
+        float2 left, right;
+        if constexpr (M::QWEN) {  // each product and sum rounded
+          left = __fadd2_rn(__fmul2_rn(v[e], cs[e]), __fmul2_rn(v[2 + e], minus));
+          right = __fadd2_rn(__fmul2_rn(v[2 + e], cs[e]), __fmul2_rn(v[e], sn[e]));
+        } else {
+          left = __ffma2_rn(v[2 + e], minus, __fmul2_rn(v[e], cs[e]));
+          right = __ffma2_rn(v[2 + e], cs[e], __fmul2_rn(v[e], sn[e]));
+        }
+        out[2 * e] = left.x, out[2 * e + 1] = left.y, out[4 + 2 * e] = right.x, out[5 + 2 * e] = right.y;
+        bad = __ffma2_rn(left, make_float2(0.0f, 0.0f), bad);
+        bad = __ffma2_rn(right, make_float2(0.0f, 0.0f), bad);
+      }
+      const long long to = (cell * M::HQ + q0 + a * HPW) * M::D + 4 * c;
+      store4(p.q_rot, to, p.rot_dtype, VEC, out);
+      store4(p.q_rot, to + HALF, p.rot_dtype, VEC, out + 4);
+    }
+    good &= bad.x + bad.y == 0.0f;
   }
   if (!good) flag_error(p.err, QX_ERR_BIT_NONFINITE);
 }
 
-// A lane takes eight dims of a head of one key or value row.
+// A lane takes eight dims of a head, of a row's key and value; a head's values are
+// spread over its lanes' words (half g of a group holds dim g of each of its four
+// lanes), which the lanes pass around.
 template <class M>
 __global__ void __launch_bounds__(kThreads) qx_q4_read_kernel(const __grid_constant__ Q4ReadParams p) {
   using R = Q4Row<M>;
-  constexpr int CHUNKS = M::HKV * R::LPH;  // lanes per row
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long unit = i / (2 * CHUNKS);
+  constexpr int LANES = M::HKV * R::LPH;  // per row
+  static_assert(kThreads % LANES == 0, "whole rows a CTA");
+  const int at = threadIdx.x % LANES, head = at / R::LPH, c = at & (R::LPH - 1);
+  const unsigned unit = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   pdl_wait();
-  if (unit >= (long long)p.token_count * p.layer_count) return;
-  const int at = (int)(i - unit * 2 * CHUNKS), side = at / CHUNKS, head = at % CHUNKS / R::LPH, c = at & (R::LPH - 1);
-  void* out = side ? p.value_out : p.key_out;
-  if (!out) return;
-  const int token = p.token_begin + (int)(unit / p.layer_count), l = (int)(unit % p.layer_count);
+  if (unit >= (unsigned)p.token_count * p.layer_count) return;
+  const unsigned step = p.layer_count == 1 ? unit : unit / p.layer_count;
+  const int token = p.token_begin + (int)step, l = (int)(unit - step * p.layer_count);
   const Q4Seq s = p.seqs[find_seq(p.seqs, p.n_seq, token)];
-  const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq, p.layer_begin + l,
-                               s.begin + token - s.first);
-  const char* src = (side ? p.arena.v : p.arena.k) + row * kQ4RowBytes;
-  int codes[8];
-  if (side == 0) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(src + R::key_word(head, c));
+  const long long row = kQ4RowBytes * kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, s.seq,
+                                             p.layer_begin + l, s.begin + token - s.first);
+  const long long out = (((long long)token * p.layer_count + l) * M::HKV + head) * M::D + 8 * c;
+  uint32_t key = 0u, value = 0u;
+  float key_scale = 0.0f, value_scale = 0.0f;
+  if (p.key_out) {
+    key = *reinterpret_cast<const uint32_t*>(p.arena.k + row + R::key_word(head, c));
+    key_scale = __half2float(*reinterpret_cast<const __half*>(p.arena.k + row + R::scale(head, c >> 2)));
+  }
+  if (p.value_out) {
+    value = *reinterpret_cast<const uint32_t*>(p.arena.v + row + head * R::HEAD + 4 * c);
+    value_scale = __half2float(*reinterpret_cast<const __half*>(p.arena.v + row + R::scale(head, c >> 2)));
+  }
+  // a nibble in the low bits of 2^23 is 2^23 plus it
+  float x[8];
+  if (p.key_out) {
+    const uint32_t turned = key ^ 0x88888888u;  // c + 8
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      codes[i] = (int)(w << (24 - 8 * i)) >> 28;
-      codes[4 + i] = (int)(w << (28 - 8 * i)) >> 28;
+      x[i] = (__uint_as_float((turned >> (8 * i + 4) & 15u) | 0x4b000000u) - 8388616.0f) * key_scale;
+      x[4 + i] = (__uint_as_float((turned >> (8 * i) & 15u) | 0x4b000000u) - 8388616.0f) * key_scale;
     }
-  } else {
+    store8(p.key_out, out, p.out_dtype, p.vec, x);
+  }
+  if (p.value_out) {
+    const int base = (threadIdx.x & 31) & ~(R::LPH - 1), j = c >> 2;
+    const int shift = 4 * (c & 3) + 16 * (j & 1);  // half g NG + j: NG is even
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
-      const uint32_t half = *reinterpret_cast<const uint16_t*>(src + R::value_half(head, c >> 2, g));
-      codes[g] = (int)((half >> (4 * (c & 3))) & 15u) - 7;
+      const uint32_t from = __shfl_sync(0xffffffffu, value, base + ((g * R::NG + j) >> 1));
+      x[g] = (__uint_as_float((from >> shift & 15u) | 0x4b000000u) - 8388615.0f) * value_scale;
     }
+    store8(p.value_out, out, p.out_dtype, p.vec, x);
   }
-  const float scale = __half2float(*reinterpret_cast<const __half*>(src + R::scale(head, c >> 2)));
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)codes[e], scale);
-  store8(out, (((long long)token * p.layer_count + l) * M::HKV + head) * M::D + 8 * c, p.out_dtype, p.vec, x);
 }
 
 // Launch as a programmatic dependent of the stream's previous kernel.
@@ -113,15 +260,17 @@ cudaError_t launch_dependent(void (*fn)(P), long long blocks, int threads, cudaS
 
 template <class M>
 cudaError_t append(const Q4AppendParams& p, cudaStream_t stream) {
-  const int warps = ((p.q ? M::HQ : 0) + 2 * M::HKV) / (32 / Q4Row<M>::LPH);
-  const long long total = (long long)p.token_count * p.layer_count * warps;
-  return launch_dependent(qx_q4_append_kernel<M>, (total + kThreads / 32 - 1) / (kThreads / 32), kThreads, stream, p);
+  const long long units = (long long)p.token_count * p.layer_count;
+  void (*fn)(Q4AppendParams) = p.in_dtype == 0 ? (p.vec ? qx_q4_append_kernel<M, true, true> : qx_q4_append_kernel<M, true, false>)
+                                               : (p.vec ? qx_q4_append_kernel<M, false, true> : qx_q4_append_kernel<M, false, false>);
+  return launch_dependent(fn, (units + kThreads / 128 - 1) / (kThreads / 128), kThreads, stream, p);
 }
 
 template <class M>
 cudaError_t read(const Q4ReadParams& p, cudaStream_t stream) {
-  const long long total = (long long)p.token_count * p.layer_count * 2 * M::HKV * Q4Row<M>::LPH;
-  return launch_dependent(qx_q4_read_kernel<M>, (total + kThreads - 1) / kThreads, kThreads, stream, p);
+  constexpr int ROWS = kThreads / (M::HKV * Q4Row<M>::LPH);  // a CTA
+  const long long total = (long long)p.token_count * p.layer_count;
+  return launch_dependent(qx_q4_read_kernel<M>, (total + ROWS - 1) / ROWS, kThreads, stream, p);
 }
 
 }  // namespace

@@ -186,12 +186,14 @@ __device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long fi
 #pragma unroll
   for (int j = 0; j < NG; ++j) load8(p.q, base + 32 * j, p.q_dtype, p.vec, x + 8 * j);
   if constexpr (M::QWEN) {
-    double sum = 0.0;
+    float s[8];
 #pragma unroll
-    for (int e = 0; e < NG * 8; ++e) sum = fma((double)x[e], (double)x[e], sum);
+    for (int e = 0; e < 8; ++e)
+      s[e] = fmaf(x[e], x[e], x[8 + e] * x[8 + e]) + fmaf(x[16 + e], x[16 + e], x[24 + e] * x[24 + e]);
+    float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    const float inv = (float)rsqrt(sum * (1.0 / M::D) + 1.0e-6);
+    const float inv = __frcp_rn(__fsqrt_rn(fmaf(sum, 1.0f / M::D, 1.0e-6f)));
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
@@ -290,7 +292,9 @@ __global__ void __launch_bounds__(256) qx_q4_prepare_kernel(const __grid_constan
       good = quantise8(x, codes, &scale);
       put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, value_halves(codes), scale);
     } else {
-      good = rotate_head<M>(x, c, position, p.k_norm, p.rope);
+      float2 tab[8];
+      rope_of_lane<M>(p.rope, position, c, tab);
+      good = rotate_key<M>(x, c, p.k_norm, tab);
       good &= quantise8(x, codes, &scale);
       put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, key_codes(codes), scale);
     }

@@ -1127,7 +1127,7 @@ qxc_status check_rows(qxc_ctx* ctx, const qxc_kv* kv, int layer_begin, int layer
   return QXC_OK;
 }
 
-qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a, int q_dtype, int rot_dtype) {
+qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
   Q4AppendParams p;
   p.arena = q4_arena(kv);
   p.layer_begin = a->layer_begin;
@@ -1144,11 +1144,9 @@ qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a, int q_d
   p.q_norm = a->q_norm;
   p.k_norm = a->k_norm;
   p.rope = rope_of(ctx, kv);
-  p.q_dtype = q_dtype;
   p.in_dtype = a->in_dtype;
-  p.rot_dtype = rot_dtype;
-  // elements of a 16-byte load
-  const long long lanes = 16 / (long long)std::min(dtype_size(a->in_dtype), dtype_size(q_dtype));
+  p.rot_dtype = a->rot_dtype;
+  const long long lanes = 16 / (long long)dtype_size(a->in_dtype);  // elements of a 16-byte load
   p.vec = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->q_rot, 16) &&
           aligned(a->k_rot, 16) && p.q_stride % lanes == 0 && p.k_stride % lanes == 0 && p.v_stride % lanes == 0;
   p.err = ctx->err_dev;
@@ -2735,7 +2733,7 @@ qxc_status qxc_kv_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
     DeviceGuard device(ctx->device);
     if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
     st = ensure_pages(ctx, kv, a->seq_count, ids.data(), ends.data());
-    if (st == QXC_OK) st = q4_append(ctx, kv, a, a->in_dtype, a->rot_dtype);
+    if (st == QXC_OK) st = q4_append(ctx, kv, a);
     if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
       for (int i = 0; i < a->seq_count; ++i) kv->len[ids[i]] = ends[i];
     return st;

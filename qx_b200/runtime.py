@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes as C
 import enum
 import weakref
+from array import array
 from dataclasses import dataclass
 
 import numpy as np
@@ -57,7 +58,7 @@ def _ptr(x) -> int | None:
 
 def _i32(values):
     """A host int32 array of `values`, or None."""
-    return None if values is None else (C.c_int32 * len(values))(*values)
+    return None if values is None else (C.c_int32 * len(values)).from_buffer(array("i", values))
 
 
 def _token_stride(x, features: int) -> int:
@@ -66,6 +67,8 @@ def _token_stride(x, features: int) -> int:
     pointer."""
     if x is None or isinstance(x, int) or not hasattr(x, "stride"):
         return 0
+    if x.is_contiguous() and x.numel() == x.shape[0] * features:
+        return features if x.shape[0] > 1 else 0
     shape, stride, dense = tuple(x.shape), tuple(x.stride()), 1
     for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
         if n != 1 and s != dense:
@@ -423,8 +426,11 @@ class KvArena:
     def _decode_args(self, q, k, v, out, positions, layer_begin, layer_count, seq_ids, q_dtype, in_dtype,
                      out_dtype, flags, split, q_rot_out, q_norm, k_norm):
         n = len(positions)
-        pos = (C.c_int32 * n)(*[int(x) for x in positions])
-        ids = (C.c_int32 * n)(*[int(x) for x in seq_ids]) if seq_ids is not None else None
+        try:
+            pos, ids = _i32(positions), _i32(seq_ids)
+        except TypeError:  # not whole numbers
+            pos = (C.c_int32 * n)(*[int(x) for x in positions])
+            ids = (C.c_int32 * n)(*[int(x) for x in seq_ids]) if seq_ids is not None else None
         a = _lib.DecodeArgs(layer_begin, layer_count, n, ids, pos, _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                             _ptr(q_rot_out), _ptr(q_norm), _ptr(k_norm), q_dtype, in_dtype, out_dtype, flags,
                             split)
