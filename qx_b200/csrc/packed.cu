@@ -34,7 +34,10 @@ namespace {
 
 template <class M, typename T>
 struct Packed {
-  static constexpr int NT = 320;
+  static constexpr int NT = 384;                    // warps 10 and 11 only give up registers
+  // registers a thread of the softmax warps (a row's scores and weights without a
+  // spill) and of the others, after the split
+  static constexpr int REGS = 224, REGS_OTHER = 48;
   static constexpr int HALVES = M::D / 64;          // 64-dim column blocks of a row
   static constexpr int TOKENS = 128 / M::G;         // tokens of a query tile
   static constexpr int BLK = 128 * 128;             // [128 rows][128 B]
@@ -50,8 +53,6 @@ struct Packed {
   static constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr float TAU = 8.0f;
   static constexpr float UNIT = M::SCALE * 1.4426950408889634f;  // base-2 logit of a score
-  // of every POLY pairs of exponentials the last runs on the FMA pipe
-  static constexpr int POLY = 4;
   static_assert(SMEM <= 227 * 1024, "fits one SM");
   static_assert(packed_block(M::QWEN) == 2 * TOKENS, "two tiles a block");
 };
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
   pdl_launch_dependents();
   bool ok = true;
 
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHER));
   if (warp == 9) {
     // ---- TMA producer: keys of tile i are load 2 i, its values load 2 i + 1 ------
     if (lane == 0) {
@@ -237,7 +239,8 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       for (int u = 0; u < 2; ++u)
         if (tiles[u]) ok &= mbar_wait_bounded(&odone[u], 0, p.err);
     }
-  } else {
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
     // ---- softmax of tile u: thread owns row r (token r / G of the tile, head r % G)
     const int u = warp >> 2, r = tid & 127;
     const int pos = q0 + u * C::TOKENS + r / M::G;  // within the prompt
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
         for (int j = 0; j < 16; ++j) {
           const int c = 32 * q + 2 * j;
           const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), make_float2(C::UNIT, C::UNIT), make_float2(-m, -m));
-          const float2 e = j % C::POLY == C::POLY - 1 ? exp2_poly2(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
           w[j] = pack_pair<T>(e);
           sum[j & 1] = __fadd2_rn(sum[j & 1], e);
         }
@@ -354,6 +357,11 @@ cudaError_t packed(const PackedParams& p, cudaStream_t stream) {
   using C = Packed<M, T>;
   cudaError_t e = cudaFuncSetAttribute(qx_packed_kernel<M, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;
+  // the kernel's split would wait for registers that a launch with fewer does not have
+  cudaFuncAttributes fa;
+  e = cudaFuncGetAttributes(&fa, qx_packed_kernel<M, T>);
+  if (e != cudaSuccess) return e;
+  if (fa.numRegs * C::NT < C::REGS * 256 + C::REGS_OTHER * 128) return cudaErrorLaunchOutOfResources;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.items);
   cfg.blockDim = dim3(C::NT);
