@@ -3,10 +3,14 @@
 //
 // A work item is a block of a prompt's tokens and one kv head: two query tiles
 // of 128 rows, each 128 / G tokens x the kv head's G query heads, so the heads
-// of a group share every key and value tile. One CTA per item, longest first:
-//   warp 9      TMA producer, one thread: both query tiles, then the key and
-//               value tiles of 128 tokens through one ring in the order of
-//               their use
+// of a group share every key and value tile. The grid has one CTA per item, longest
+// first; a CTA that is running takes further items by cancelling CTAs that are not
+// launched yet, so the next item's loads and first scores are under way while the
+// last one's outputs are written, and its set-up is paid once:
+//   warp 9      TMA producer, one thread: asks for the next item, then loads this
+//               one's query tiles, each as soon as the last scores of the tile
+//               before are done, and its key and value tiles of 128 tokens through
+//               one ring in the order of their use
 //   warp 8      MMA issuer, one thread: for each tile in turn O += P V, then the
 //               next scores S = Q K^T, so one tile's products run while the
 //               other's softmax does
@@ -17,7 +21,9 @@
 //               the thread rescales its row of O in TMEM, which no product
 //               uses while the tile's scores are being read.
 // S of a tile is issued after its P V, and tensor instructions of one thread
-// complete in order: once S is there, P may be overwritten and O is settled.
+// complete in order: once S is there, P may be overwritten and O is settled. An
+// item's first P V starts O afresh; its weights are written after the tile's
+// threads have read the last item's O.
 //
 // A key tile may hold tokens its rows do not attend: later ones of the prompt,
 // the next prompt's. Their scores are replaced by -inf, so their weights are
@@ -37,7 +43,7 @@ struct Packed {
   static constexpr int NT = 384;                    // warps 10 and 11 only give up registers
   // registers a thread of the softmax warps (a row's scores and weights without a
   // spill) and of the others, after the split
-  static constexpr int REGS = 224, REGS_OTHER = 48;
+  static constexpr int REGS = 216, REGS_OTHER = 72;
   static constexpr int HALVES = M::D / 64;          // 64-dim column blocks of a row
   static constexpr int TOKENS = 128 / M::G;         // tokens of a query tile
   static constexpr int BLK = 128 * 128;             // [128 rows][128 B]
@@ -46,9 +52,11 @@ struct Packed {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = 2 * TILE;
   static constexpr int OFF_BAR = OFF_RING + STAGES * TILE;
-  // qfull, ring full/empty, per tile: scores there, weights there, output done
-  static constexpr int NBAR = 1 + 2 * STAGES + 6;
-  static constexpr int SMEM = OFF_BAR + 8 * NBAR + 16 + 1024;  // + TMEM slot, + slack to align the base
+  // ring full/empty, per tile: queries there, queries done with, scores there,
+  // weights there, output done; answers there/read
+  static constexpr int NBAR = 2 * STAGES + 10 + 4;
+  static constexpr int OFF_ITEM = OFF_BAR + (8 * NBAR + 15) / 16 * 16;  // two answers of 16 bytes
+  static constexpr int SMEM = OFF_ITEM + 32 + 16 + 1024;       // + TMEM slot, + slack to align the base
   static constexpr uint32_t COL_S = 0, COL_O = 256;            // tile u: scores at 128 u, output at 256 + D u
   static constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr float TAU = 8.0f;
@@ -105,51 +113,106 @@ __device__ __noinline__ bool careful_row(const PackedParams& p, int first, int t
   return good;
 }
 
+// A work item of this CTA.
+struct Item {
+  int token, length;  // the prompt's first packed token, its tokens
+  int head;           // kv head
+  int q0;             // first token of the block, within the prompt
+  int tiles[2];       // key tiles that each query tile attends (0: past the prompt's end)
+};
+
+template <class M, int TOKENS>
+__device__ __forceinline__ void find_item(const PackedParams& p, int index, Item* out) {
+  int lo = 0, hi = p.n_seq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.seqs[mid].item <= index) lo = mid;
+    else hi = mid - 1;
+  }
+  const PackedSeq seq = p.seqs[lo];
+  const int rel = index - seq.item, blocks = (seq.length + 2 * TOKENS - 1) / (2 * TOKENS);
+  out->token = seq.token;
+  out->length = seq.length;
+  out->head = rel % M::HKV;
+  out->q0 = (blocks - 1 - rel / M::HKV) * 2 * TOKENS;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int begin = out->q0 + u * TOKENS, end = min(begin + TOKENS, seq.length);
+    out->tiles[u] = begin < seq.length ? (end + kPackedKeys - 1) / kPackedKeys : 0;
+  }
+}
+
+// A place in the ring of N tiles, and its barriers' parity there.
+template <int N>
+struct Place {
+  int at = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void advance() {
+    if (++at == N) {
+      at = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// Ask for a CTA of this grid that is not launched yet; the answer, 16 bytes, lands
+// in shared memory and completes them on the barrier. Not after an answer of none.
+__device__ __forceinline__ void ask_for_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_addr(answer)), "r"(smem_addr(bar))
+               : "memory");
+}
+// The block index of an answer, -1 for none.
+__device__ __forceinline__ int answered_cta(const void* answer) {
+  int got, x;
+  asm volatile(
+      "{\n"
+      ".reg .b128 r;\n"
+      ".reg .pred p;\n"
+      "ld.shared.b128 r, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      "selp.s32 %0, 1, 0, p;\n"
+      "mov.s32 %1, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n"
+      "}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_addr(answer))
+      : "memory");
+  return got ? x : -1;
+}
+
 template <class M, typename T>
 __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __grid_constant__ PackedParams p) {
   using C = Packed<M, T>;
   constexpr int NS = C::STAGES;
   extern __shared__ __align__(1024) unsigned char sm_raw[];
   unsigned char* sm = sm_raw + ((1024u - (smem_addr(sm_raw) & 1023u)) & 1023u);
-  uint64_t* qfull = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
-  uint64_t* full = qfull + 1;      // [NS] a key or value tile landed
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);  // [NS] a key or value tile landed
   uint64_t* empty = full + NS;     // [NS] its products completed
-  uint64_t* sfull = empty + NS;    // [tile] scores in TMEM (and everything issued before them done)
+  uint64_t* qfull = empty + NS;    // [tile] queries landed
+  uint64_t* qempty = qfull + 2;    // [tile] the item's last scores completed
+  uint64_t* sfull = qempty + 2;    // [tile] scores in TMEM (and everything issued before them done)
   uint64_t* pfull = sfull + 2;     // [tile] weights in TMEM
   uint64_t* odone = pfull + 2;     // [tile] output in TMEM
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(odone + 2);
+  uint64_t* ifull = odone + 2;     // [2] the answer to a request for an item landed
+  uint64_t* iempty = ifull + 2;    // [2] all warps have read it
+  unsigned char* answers = sm + C::OFF_ITEM;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(answers + 32);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // the item's prompt, kv head and block
-  int lo = 0, hi = p.n_seq - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.seqs[mid].item <= (int)blockIdx.x) lo = mid;
-    else hi = mid - 1;
-  }
-  const PackedSeq seq = p.seqs[lo];
-  const int rel = blockIdx.x - seq.item, h = rel % M::HKV;
-  const int blocks = (seq.length + 2 * C::TOKENS - 1) / (2 * C::TOKENS);
-  const int q0 = (blocks - 1 - rel / M::HKV) * 2 * C::TOKENS;  // first token of the block, within the prompt
-  // key tiles each query tile attends (0: past the prompt's end)
-  int tiles[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int begin = q0 + u * C::TOKENS, end = min(begin + C::TOKENS, seq.length);
-    tiles[u] = begin < seq.length ? (end + kPackedKeys - 1) / kPackedKeys : 0;
-  }
-  const int n = max(tiles[0], tiles[1]);
-
   if (tid == 0) {
-    mbar_init(qfull, 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int u = 0; u < 2; ++u) {
+      mbar_init(&qfull[u], 1);
+      mbar_init(&qempty[u], 1);
       mbar_init(&sfull[u], 1);
       mbar_init(&pfull[u], 4);
       mbar_init(&odone[u], 1);
+      mbar_init(&ifull[u], 1);
+      mbar_init(&iempty[u], 10);
     }
     fence_barrier_init();
   }
@@ -164,158 +227,217 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
   pdl_wait();
   pdl_launch_dependents();
   bool ok = true;
+  Item item;
+  // item k + 1 is the answer of slot k % 2: its block index, -1 past the last
+  auto next_item = [&](int k) {
+    const bool there = mbar_wait_bounded(&ifull[k & 1], (uint32_t)(k >> 1) & 1u, p.err);
+    ok &= there;
+    const int index = there ? answered_cta(answers + 16 * (k & 1)) : -1;
+    fence_proxy_async_shared();  // the read above comes before the next answer
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&iempty[k & 1]);
+    return index;
+  };
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHER));
   if (warp == 9) {
-    // ---- TMA producer: keys of tile i are load 2 i, its values load 2 i + 1 ------
+    // ---- TMA producer: of an item, keys of tile i are load 2 i, its values 2 i + 1
     if (lane == 0) {
       prefetch_tmap(&p.tmq);
       prefetch_tmap(&p.tmk);
       prefetch_tmap(&p.tmv);
-      const int used = tiles[1] ? 2 : 1;
-      mbar_arrive_expect_tx(qfull, used * C::TILE);
-      for (int u = 0; u < used; ++u)
-#pragma unroll
-        for (int b = 0; b < C::HALVES; ++b)
-          tma_load_3d(sm + C::OFF_Q + u * C::TILE + b * C::BLK, &p.tmq, 64 * b, h * M::G,
-                      seq.token + q0 + u * C::TOKENS, qfull);
-      for (int i = 0; i < 2 * n; ++i) {
-        const int s = i % NS;
-        if (i >= NS) ok &= mbar_wait_bounded(&empty[s], (uint32_t)(i / NS - 1) & 1u, p.err);
-        mbar_arrive_expect_tx(&full[s], C::TILE);
-#pragma unroll
-        for (int b = 0; b < C::HALVES; ++b)
-          tma_load_3d(sm + C::OFF_RING + s * C::TILE + b * C::BLK, i & 1 ? &p.tmv : &p.tmk, 64 * b, h,
-                      seq.token + (i >> 1) * kPackedKeys, &full[s]);
-      }
-      // no copy may still be landing when the CTA exits
-      for (int i = max(0, 2 * n - NS); i < 2 * n; ++i)
-        ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
     }
+    Place<NS> place;
+    int loads = 0, used[2] = {0, 0};
+    for (int k = 0, index = blockIdx.x; index >= 0; index = next_item(k++)) {
+      find_item<M, C::TOKENS>(p, index, &item);
+      if (lane == 0) {
+        const int n = 2 * max(item.tiles[0], item.tiles[1]);
+        auto queries = [&](int u) {
+          if (!item.tiles[u]) return;
+          if (used[u]) ok &= mbar_wait_bounded(&qempty[u], (uint32_t)(used[u] - 1) & 1u, p.err);
+          ++used[u];
+          mbar_arrive_expect_tx(&qfull[u], C::TILE);
+#pragma unroll
+          for (int b = 0; b < C::HALVES; ++b)
+            tma_load_3d(sm + C::OFF_Q + u * C::TILE + b * C::BLK, &p.tmq, 64 * b, item.head * M::G,
+                        item.token + item.q0 + u * C::TOKENS, &qfull[u]);
+        };
+        queries(0);
+        for (int i = 0; i < n; ++i, ++loads, place.advance()) {
+          const int s = place.at;
+          if (loads >= NS) ok &= mbar_wait_bounded(&empty[s], place.parity ^ 1u, p.err);
+          mbar_arrive_expect_tx(&full[s], C::TILE);
+#pragma unroll
+          for (int b = 0; b < C::HALVES; ++b)
+            tma_load_3d(sm + C::OFF_RING + s * C::TILE + b * C::BLK, i & 1 ? &p.tmv : &p.tmk, 64 * b, item.head,
+                        item.token + (i >> 1) * kPackedKeys, &full[s]);
+          if (i == 0) queries(1);
+        }
+        // asked for now, not before: who is done first takes the next item
+        if (k >= 2) ok &= mbar_wait_bounded(&iempty[k & 1], (uint32_t)((k >> 1) - 1) & 1u, p.err);
+        mbar_arrive_expect_tx(&ifull[k & 1], 16);
+        ask_for_cta(answers + 16 * (k & 1), &ifull[k & 1]);
+      }
+      __syncwarp();
+    }
+    // no copy may still be landing when the CTA exits
+    if (lane == 0)
+      for (int i = max(0, loads - NS); i < loads; ++i)
+        ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
   } else if (warp == 8) {
     // ---- MMA issuer ---------------------------------------------------------------
-    if (lane == 0) {
-      constexpr uint32_t IDESC_S = umma_idesc_16bit(128, kPackedKeys, C::FMT, false, false);
-      constexpr uint32_t IDESC_PV = umma_idesc_16bit(128, M::D, C::FMT, false, true);
-      const uint32_t sq = smem_addr(sm + C::OFF_Q), ring = smem_addr(sm + C::OFF_RING);
-      auto landed = [&](int i) {
-        ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
-        tc_fence_after();
-      };
-      auto scores = [&](int u, int i) {  // S of query tile u and key tile i
-        const uint32_t q = sq + u * C::TILE, k = ring + (2 * i % NS) * C::TILE;
+    constexpr uint32_t IDESC_S = umma_idesc_16bit(128, kPackedKeys, C::FMT, false, false);
+    constexpr uint32_t IDESC_PV = umma_idesc_16bit(128, M::D, C::FMT, false, true);
+    const uint32_t sq = smem_addr(sm + C::OFF_Q), ring = smem_addr(sm + C::OFF_RING);
+    Place<NS> keys, values;
+    int items[2] = {0, 0}, weights[2] = {0, 0};            // per tile: items, weight tiles taken
+    for (int k = 0, index = blockIdx.x; index >= 0; index = next_item(k++)) {
+      find_item<M, C::TOKENS>(p, index, &item);
+      if (lane == 0) {
+        const int n = max(item.tiles[0], item.tiles[1]);
+        auto landed = [&](const Place<NS>& s) {
+          ok &= mbar_wait_bounded(&full[s.at], s.parity, p.err);
+          tc_fence_after();
+        };
+        auto scores = [&](int u, int i) {  // S of query tile u and key tile i
+          const uint32_t q = sq + u * C::TILE, ks = ring + keys.at * C::TILE;
 #pragma unroll
-        for (int kk = 0; kk < M::D / 16; ++kk)
-          tc_mma_bf16(tbase + C::COL_S + 128 * u, umma_desc_sw128(q + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024),
-                      umma_desc_sw128(k + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024), IDESC_S, kk > 0);
-        tc_commit(&sfull[u]);
-      };
-      auto output = [&](int u, int i) {  // O += P V of query tile u and key tile i
-        ok &= mbar_wait_bounded(&pfull[u], (uint32_t)i & 1u, p.err);
-        tc_fence_after();
-        const uint32_t v = ring + ((2 * i + 1) % NS) * C::TILE;
+          for (int kk = 0; kk < M::D / 16; ++kk)
+            tc_mma_bf16(tbase + C::COL_S + 128 * u, umma_desc_sw128(q + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024),
+                        umma_desc_sw128(ks + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024), IDESC_S, kk > 0);
+          tc_commit(&sfull[u]);
+          if (i + 1 == item.tiles[u]) tc_commit(&qempty[u]);
+        };
+        auto output = [&](int u, int i) {  // O += P V of query tile u and key tile i
+          ok &= mbar_wait_bounded(&pfull[u], (uint32_t)weights[u] & 1u, p.err);
+          ++weights[u];
+          tc_fence_after();
+          const uint32_t v = ring + values.at * C::TILE;
 #pragma unroll
-        for (int kk = 0; kk < kPackedKeys / 16; ++kk)
-          tc_mma_ts_bf16(tbase + C::COL_O + M::D * u, tbase + C::COL_S + 128 * u + 8 * kk,
-                         umma_desc_sw128(v + kk * 2048, C::BLK, 1024), IDESC_PV, (i > 0 ? 1u : 0u) | (kk > 0 ? 1u : 0u));
-      };
-      ok &= mbar_wait_bounded(qfull, 0, p.err);
-      landed(0);
-      for (int u = 0; u < 2; ++u)
-        if (tiles[u]) scores(u, 0);
-      tc_commit(&empty[0]);
-      for (int i = 0; i < n; ++i) {
-        landed(2 * i + 1);
-        if (i + 1 < n) landed(2 * i + 2);
-        for (int u = 0; u < 2; ++u) {
-          if (i < tiles[u]) output(u, i);
-          if (i + 1 < tiles[u]) scores(u, i + 1);
-          else if (i + 1 == tiles[u]) tc_commit(&odone[u]);
+          for (int kk = 0; kk < kPackedKeys / 16; ++kk)
+            tc_mma_ts_bf16(tbase + C::COL_O + M::D * u, tbase + C::COL_S + 128 * u + 8 * kk,
+                           umma_desc_sw128(v + kk * 2048, C::BLK, 1024), IDESC_PV, (i > 0 ? 1u : 0u) | (kk > 0 ? 1u : 0u));
+        };
+        landed(keys);
+        for (int u = 0; u < 2; ++u)
+          if (item.tiles[u]) {
+            ok &= mbar_wait_bounded(&qfull[u], (uint32_t)items[u] & 1u, p.err);
+            ++items[u];
+            tc_fence_after();
+            scores(u, 0);
+          }
+        tc_commit(&empty[keys.at]);
+        keys.advance();
+        for (int i = 0; i < n; ++i) {
+          values = keys;  // this step's values, then the next step's keys
+          landed(values);
+          keys.advance();
+          if (i + 1 < n) landed(keys);
+          for (int u = 0; u < 2; ++u) {
+            if (i < item.tiles[u]) output(u, i);
+            if (i + 1 < item.tiles[u]) scores(u, i + 1);
+            else if (i + 1 == item.tiles[u]) tc_commit(&odone[u]);
+          }
+          tc_commit(&empty[values.at]);
+          if (i + 1 < n) {
+            tc_commit(&empty[keys.at]);
+            keys.advance();
+          }
         }
-        tc_commit(&empty[(2 * i + 1) % NS]);
-        if (i + 1 < n) tc_commit(&empty[(2 * i + 2) % NS]);
       }
-      // TMEM and the ring are released only after every product completed
-      for (int u = 0; u < 2; ++u)
-        if (tiles[u]) ok &= mbar_wait_bounded(&odone[u], 0, p.err);
+      __syncwarp();
     }
+    // TMEM is released only after every product completed
+    if (lane == 0)
+      for (int u = 0; u < 2; ++u)
+        if (items[u]) ok &= mbar_wait_bounded(&odone[u], (uint32_t)(items[u] - 1) & 1u, p.err);
   } else if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
     // ---- softmax of tile u: thread owns row r (token r / G of the tile, head r % G)
     const int u = warp >> 2, r = tid & 127;
-    const int pos = q0 + u * C::TOKENS + r / M::G;  // within the prompt
     const uint32_t trow = tbase + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ts = trow + C::COL_S + 128 * u, to = trow + C::COL_O + M::D * u;
-    float m = -INFINITY;
-    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-    for (int i = 0; i < tiles[u]; ++i) {
-      ok &= mbar_wait_bounded(&sfull[u], (uint32_t)i & 1u, p.err);
-      __syncwarp();
-      tc_fence_after();
-      float s[128];
+    int seen = 0, written = 0;  // score tiles, items of this query tile
+    for (int k = 0, index = blockIdx.x; index >= 0; index = next_item(k++)) {
+      find_item<M, C::TOKENS>(p, index, &item);
+      const int tiles = u ? item.tiles[1] : item.tiles[0];
+      if (!tiles) continue;
+      const int pos = item.q0 + u * C::TOKENS + r / M::G;  // within the prompt
+      float m = -INFINITY;
+      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      for (int i = 0; i < tiles; ++i, ++seen) {
+        ok &= mbar_wait_bounded(&sfull[u], (uint32_t)seen & 1u, p.err);
+        __syncwarp();
+        tc_fence_after();
+        float s[128];
 #pragma unroll
-      for (int c = 0; c < 128; c += 32) tmem_ld32_sync(ts + c, s + c);
-      if (i == tiles[u] - 1 || (i + 1) * kPackedKeys > q0 + u * C::TOKENS) {  // some key is later than some row
-        const int limit = pos - i * kPackedKeys;
+        for (int c = 0; c < 128; c += 32) tmem_ld32_sync(ts + c, s + c);
+        if (i == tiles - 1 || (i + 1) * kPackedKeys > item.q0 + u * C::TOKENS) {  // some key is later than some row
+          const int limit = pos - i * kPackedKeys;
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c > limit) s[c] = -INFINITY;
-      }
-      float m4[4] = {s[0], s[1], s[2], s[3]};
+          for (int c = 0; c < 128; ++c)
+            if (c > limit) s[c] = -INFINITY;
+        }
+        float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < 124; c += 8) {
+        for (int c = 4; c < 124; c += 8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m4[e] = fmax3f(m4[e], s[c + 2 * e], s[c + 2 * e + 1]);
-      }
-      m4[0] = fmax3f(m4[0], s[124], s[125]);
-      m4[1] = fmax3f(m4[1], s[126], s[127]);
-      const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * C::UNIT;
-      const bool raise = top > m + C::TAU;  // true on the first tile (m = -inf)
-      if (__any_sync(0xffffffffu, raise)) {
-        const float keep = raise ? fast_exp2(m - top) : 1.0f;
-        if (i > 0) {
+          for (int e = 0; e < 4; ++e) m4[e] = fmax3f(m4[e], s[c + 2 * e], s[c + 2 * e + 1]);
+        }
+        m4[0] = fmax3f(m4[0], s[124], s[125]);
+        m4[1] = fmax3f(m4[1], s[126], s[127]);
+        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * C::UNIT;
+        const bool raise = top > m + C::TAU;  // true on the first tile (m = -inf)
+        if (__any_sync(0xffffffffu, raise)) {
+          const float keep = raise ? fast_exp2(m - top) : 1.0f;
+          if (i > 0) {
 #pragma unroll
-          for (int c = 0; c < M::D; c += 16) {
-            float o[16];
-            uint32_t b[16];
-            tmem_ld16_sync(to + c, o);
+            for (int c = 0; c < M::D; c += 16) {
+              float o[16];
+              uint32_t b[16];
+              tmem_ld16_sync(to + c, o);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) b[e] = __float_as_uint(o[e] * keep);
-            tmem_st16u(to + c, b);
+              for (int e = 0; e < 16; ++e) b[e] = __float_as_uint(o[e] * keep);
+              tmem_st16u(to + c, b);
+            }
           }
+          sum[0] = __fmul2_rn(sum[0], make_float2(keep, keep));
+          sum[1] = __fmul2_rn(sum[1], make_float2(keep, keep));
+          if (raise) m = top;
         }
-        sum[0] = __fmul2_rn(sum[0], make_float2(keep, keep));
-        sum[1] = __fmul2_rn(sum[1], make_float2(keep, keep));
-        if (raise) m = top;
-      }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t w[16];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int c = 32 * q + 2 * j;
-          const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), make_float2(C::UNIT, C::UNIT), make_float2(-m, -m));
-          const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-          w[j] = pack_pair<T>(e);
-          sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+          for (int j = 0; j < 16; ++j) {
+            const int c = 32 * q + 2 * j;
+            const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), make_float2(C::UNIT, C::UNIT), make_float2(-m, -m));
+            const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            w[j] = pack_pair<T>(e);
+            sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+          }
+          tmem_st16u(ts + 16 * q, w);
         }
-        tmem_st16u(ts + 16 * q, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[u]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[u]);
-    }
-    // ---- output ---------------------------------------------------------------------
-    if (tiles[u]) {
-      ok &= mbar_wait_bounded(&odone[u], 0, p.err);
+      // ---- output -------------------------------------------------------------------
+      ok &= mbar_wait_bounded(&odone[u], (uint32_t)written & 1u, p.err);
+      ++written;
       __syncwarp();
       tc_fence_after();
       const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), inv = 1.0f / all;
-      const bool real = pos < seq.length;
-      const int token = seq.token + pos, qh = h * M::G + r % M::G;
+      const bool real = pos < item.length;
+      const int token = item.token + pos, qh = item.head * M::G + r % M::G;
       bool good = true;
-      T* out = static_cast<T*>(p.out) + ((long long)token * M::HQ + qh) * M::D;
+      // four lanes exchange their rows' 16-byte pieces, so that a store writes 64
+      // bytes of 8 rows and not 16 of 32: lane t of the four ends with piece t of each
+      const int r0 = r & ~3, pos0 = item.q0 + u * C::TOKENS + r0 / M::G;
+      T* out = static_cast<T*>(p.out) + ((long long)(item.token + pos0) * M::HQ + item.head * M::G + r0 % M::G) * M::D +
+               8 * (lane & 3);
 #pragma unroll
       for (int c = 0; c < M::D; c += 32) {
         float o[32];
@@ -327,18 +449,32 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
           good &= isfinite(y.x) && isfinite(y.y);
           w[e] = pack_pair<T>(y);
         }
-        if (real) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            reinterpret_cast<uint4*>(out + c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        for (int bit = 1; bit < 4; bit <<= 1) {
+          const bool upper = lane & bit;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if ((e >> 2) & bit) continue;
+            const int f = e + 4 * bit;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[e] : w[f], bit);
+            if (upper) w[e] = got;
+            else w[f] = got;
+          }
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (pos0 + j / M::G < item.length)
+            *reinterpret_cast<uint4*>(out + (j / M::G * M::HQ + j % M::G) * M::D + c) =
+                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       }
+      __syncwarp();  // a row that is recomputed is written after this
+      tc_fence_before();  // O was read: the next item's first product may write it once its weights are there
       unsigned redo = __ballot_sync(0xffffffffu, real && ok && !good && isfinite(m) && isfinite(all));
       bool bad = real && !good && !(isfinite(m) && isfinite(all));
       while (redo) {
         const int src = __ffs(redo) - 1;
         redo &= redo - 1;
-        bad |= !careful_row<M, T>(p, seq.token, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, qh, src),
+        bad |= !careful_row<M, T>(p, item.token, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, qh, src),
                                   __shfl_sync(0xffffffffu, m, src), __shfl_sync(0xffffffffu, all, src));
       }
       if (bad && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);

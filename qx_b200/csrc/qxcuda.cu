@@ -1025,12 +1025,13 @@ namespace {
 // The caller's current device, put back when a call leaves.
 struct DeviceGuard {
   int before = -1;
-  bool ok;
+  bool moved = false, ok;
   explicit DeviceGuard(int device) {
-    ok = cudaGetDevice(&before) == cudaSuccess && (before == device || cudaSetDevice(device) == cudaSuccess);
+    ok = cudaGetDevice(&before) == cudaSuccess;
+    if (ok && before != device) ok = moved = cudaSetDevice(device) == cudaSuccess;
   }
   ~DeviceGuard() {
-    if (before >= 0) cudaSetDevice(before);
+    if (moved) cudaSetDevice(before);
   }
 };
 
