@@ -72,7 +72,10 @@ const char* qxc_status_string(qxc_status status);
 /* One context per host thread; `device` is the CUDA ordinal. */
 qxc_status qxc_init(int device, qxc_ctx** out);
 void qxc_destroy(qxc_ctx* ctx);
-/* Use the caller's cudaStream_t (NULL restores the context's own stream). */
+/* Use the caller's cudaStream_t (NULL restores the context's own stream). The
+ * calls of a context share its workspaces: order work that is still running on
+ * the old stream before what follows on the new one, and do not replay two
+ * captured graphs of one context at the same time. */
 qxc_status qxc_set_stream(qxc_ctx* ctx, void* cuda_stream);
 void* qxc_get_stream(qxc_ctx* ctx);
 /* Wait for all work on the context stream, then report any device-side
@@ -83,7 +86,8 @@ qxc_status qxc_sync(qxc_ctx* ctx);
 const char* qxc_last_error(const qxc_ctx* ctx);
 /* Number of kernels this context has launched so far. */
 uint64_t qxc_launch_count(const qxc_ctx* ctx);
-/* Cache positions per split chosen by the last decode call on this context. */
+/* Cache positions per split chosen by the last decode call on this context
+ * (4-bit arenas: rows of a CTA's stretch of all the call's rows). */
 int32_t qxc_last_split(const qxc_ctx* ctx);
 /* (new; host only, no device) The automatic split the decode calls choose:
  * cache rows per split for `n` sequences of attend[i] rows, `units` work
@@ -147,7 +151,9 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
  *   values  c + 7 in nibble r / 8 (low first) of its 16-bit half (r % 8) * NG + j
  * Contiguous or paged, any input type of either model; first_position must be
  * 0. Cursors, paging, views (bytes), qxc_kv_read / write (raw rows) work as on
- * any arena, qxc_decode reads and writes it, qxc_attention_layer and
+ * any arena, qxc_decode reads and writes it (with the hardware exponential;
+ * its workspace grows with sequences and layers, and a call that grows it
+ * cannot be captured: QXC_ERR_UNSUPPORTED), qxc_attention_layer and
  * qxc_attention_stack run on it through qxc_decode. The verify, partials,
  * exchange, prefill and hash calls return QXC_ERR_UNSUPPORTED. A value beyond
  * 7 * 65504, an infinity or a NaN in a new row is reported by qxc_sync
@@ -163,7 +169,7 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
  * advance by counts unless QXC_DECODE_NO_ADVANCE. Device pointers of any
  * element alignment (16-byte aligned ones are read and written faster);
  * asynchronous. q and q_rot may both be NULL (keys and values only), k_rot may
- * be NULL. */
+ * be NULL. q_rot may be q itself, and k_rot k, where type and layout are the same. */
 typedef struct qxc_append_args {
   int32_t layer_begin;
   int32_t layer_count;
@@ -212,7 +218,7 @@ qxc_status qxc_kv_read_rows(qxc_ctx* ctx, qxc_kv* kv, const qxc_read_rows_args* 
  * pool of `pool_pages` pages of `page_size` rows ([page][kv_heads][head_dim]);
  * each sequence has one block table, shared by its layers, mapping its logical
  * pages to physical pages. Pages are mapped on demand, in order, by the calls
- * that write rows (decode, verify, partials, qxc_kv_write) and by
+ * that write rows (decode, verify, partials, append, qxc_kv_write) and by
  * qxc_kv_set_len; a call the pool cannot serve fails with
  * QXC_ERR_OUT_OF_MEMORY and maps nothing. qxc_kv_reset returns a sequence's
  * pages to the pool; rollback / commit keep them for the sequence's regrowth;
@@ -242,7 +248,7 @@ qxc_status qxc_kv_pool_buffer(qxc_kv* kv, int32_t key, void** device_ptr, size_t
 /* ---- decode ------------------------------------------------------------ */
 /* Stream ordering. Every kernel here is launched as a programmatic
  * dependent of the stream's previous kernel. A single-sequence decode on a
- * contiguous Qwen arena may start reading cached rows before the previous
+ * contiguous 16-bit Qwen arena may start reading cached rows before the previous
  * kernel has finished: it reads only rows that no earlier launch of this
  * context can still be writing. A caller that writes the arena with its own
  * kernel on the same stream must not launch that kernel with programmatic
@@ -493,9 +499,12 @@ qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* args);
  * lengths may be 0; at most 2^24 tokens. Each tensor is [tokens][heads *
  * head_dim], 16-byte aligned, with token strides in elements that are
  * multiples of 8 (0 = dense): q, k and v may be parts of one joint projection.
- * Rows of `out` past the last prompt are not written. A row that attends a
- * NaN or an infinity is not finite (QXC_ERR_NONFINITE at qxc_sync); rows that
- * do not attend it are unaffected. Device pointers, asynchronous. */
+ * Rows of `out` past the last prompt are not written; `out` must not overlap
+ * an input. What a row that attends a NaN or an infinity holds is unspecified
+ * in every dim that it can reach (all of them from a query or a key, its own
+ * from a value); a row that is not finite is reported by qxc_sync
+ * (QXC_ERR_NONFINITE). Rows that do not attend it are unaffected. Device
+ * pointers, asynchronous. */
 typedef struct qxc_packed_args {
   int32_t model;
   int32_t seq_count;
@@ -516,7 +525,9 @@ qxc_status qxc_attend_packed(qxc_ctx* ctx, const qxc_packed_args* args);
  * queries, the rotated keys before quantisation (rounded to dtype) and the
  * values as given. Arguments, position and alignment rules as theirs (q and k
  * any alignment). Lengths advance unless QXC_DECODE_NO_ADVANCE (more layers to
- * come). Device pointers, asynchronous. */
+ * come). The rotated rows lie in a workspace of the context that grows with
+ * the tokens of a call: the first call of a size cannot be captured
+ * (QXC_ERR_UNSUPPORTED). Device pointers, asynchronous. */
 typedef struct qxc_prefill_packed_args {
   int32_t layer;
   int32_t seq_count;

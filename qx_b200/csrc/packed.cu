@@ -27,9 +27,9 @@
 //
 // A key tile may hold tokens its rows do not attend: later ones of the prompt,
 // the next prompt's. Their scores are replaced by -inf, so their weights are
-// zero, but a zero weight times an infinite or NaN value is NaN: a row whose
-// sums are finite and whose output is not is recomputed token by token
-// (careful_row), over what it attends only.
+// zero, but a zero weight times an infinite or NaN value is NaN: of a row whose
+// sums are finite and whose output is not, the dims that this can have touched are
+// computed again over what it attends only (careful_row).
 #include <type_traits>
 
 #include "q4.cuh"
@@ -76,41 +76,63 @@ __device__ __forceinline__ uint32_t pack_pair(float2 x) {
   }
 }
 
-// One output row by a whole warp, over tokens first .. token only, against the
-// row's own reference m and sum.
+// One output row of a non-finite tile again, by a whole warp: the dims in which a
+// token of [token + 1, end), which the row does not attend but its key tiles hold,
+// is not finite, over tokens first .. token only, against the row's own reference
+// m and sum. A dim ends as soon as it is not finite by what the row does attend,
+// so that only the rows of one query tile before a dim's first such value walk all
+// their tokens. False when the row is not finite.
 template <class M, typename T>
-__device__ __noinline__ bool careful_row(const PackedParams& p, int first, int token, int qh, float m, float sum) {
+__device__ __noinline__ bool careful_row(const PackedParams& p, int first, int token, int end, int qh, float m, float sum) {
   constexpr int N = M::D / 32;
   using P = Packed<M, T>;
   const int lane = threadIdx.x & 31, h = qh / M::G;
   const T* q = static_cast<const T*>(p.q) + token * p.q_stride + qh * M::D;
+  auto value = [&](int t, int e) {
+    return Elem<T>::to_f32(static_cast<const T*>(p.v)[t * p.v_stride + h * M::D + 32 * e + lane]);
+  };
   float o[N];
+  bool dirty[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) o[e] = 0.0f;
+  for (int e = 0; e < N; ++e) {
+    o[e] = 0.0f;
+    dirty[e] = false;
+  }
+  for (int t = token + 1; t < end; ++t)
+#pragma unroll
+    for (int e = 0; e < N; ++e) dirty[e] |= !isfinite(value(t, e));
   for (int t0 = first; t0 <= token; t0 += 32) {
+    bool open = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) open |= dirty[e] && isfinite(o[e]);
+    if (!__any_sync(0xffffffffu, open)) break;
     float weight = 0.0f;
     if (t0 + lane <= token) {
       const T* k = static_cast<const T*>(p.k) + (t0 + lane) * p.k_stride + h * M::D;
       float dot = 0.0f;
-      for (int d = 0; d < M::D; ++d) dot = fmaf(Elem<T>::to_f32(q[d]), Elem<T>::to_f32(k[d]), dot);
+      for (int d = 0; d < M::D; d += 8) {
+        float x[8], y[8];
+        Vec16<T>::load(q + d, x);
+        Vec16<T>::load(k + d, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
+      }
       weight = fast_exp2(fmaf(dot, P::UNIT, -m));
     }
     for (int u = 0; u < 32 && t0 + u <= token; ++u) {
       const float w = __shfl_sync(0xffffffffu, weight, u);
-      const T* v = static_cast<const T*>(p.v) + (t0 + u) * p.v_stride + h * M::D;
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = fmaf(w, Elem<T>::to_f32(v[32 * e + lane]), o[e]);
+      for (int e = 0; e < N; ++e) o[e] = fmaf(w, value(t0 + u, e), o[e]);
     }
   }
   bool good = true;
   T* out = static_cast<T*>(p.out) + ((long long)token * M::HQ + qh) * M::D;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float y = o[e] / sum;
-    good &= isfinite(y);
-    out[32 * e + lane] = Elem<T>::from_f32(y);
+    if (dirty[e]) out[32 * e + lane] = Elem<T>::from_f32(o[e] / sum);
+    good &= isfinite(Elem<T>::to_f32(out[32 * e + lane]));
   }
-  return good;
+  return __all_sync(0xffffffffu, good);
 }
 
 // A work item of this CTA.
@@ -474,7 +496,8 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       while (redo) {
         const int src = __ffs(redo) - 1;
         redo &= redo - 1;
-        bad |= !careful_row<M, T>(p, item.token, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, qh, src),
+        bad |= !careful_row<M, T>(p, item.token, __shfl_sync(0xffffffffu, token, src),
+                                  min(item.token + tiles * kPackedKeys, p.tokens), __shfl_sync(0xffffffffu, qh, src),
                                   __shfl_sync(0xffffffffu, m, src), __shfl_sync(0xffffffffu, all, src));
       }
       if (bad && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);

@@ -109,6 +109,7 @@ struct PackedParams {
   void* out;  // [token][HQ][D]
   long long q_stride, k_stride, v_stride;  // elements between tokens
   int dtype;
+  int tokens;  // of all the call's prompts
   int n_seq;
   int items;
   unsigned* err;

@@ -1097,7 +1097,7 @@ qxc_status each_part(int seq_count, const int32_t* seq_ids, const int32_t* begin
 }
 
 // Layers, sequences and rows of a call that writes or reads many rows of a
-// 4-bit arena; `rows[i]` becomes the end of sequence i's range.
+// 4-bit arena; ids[i] and ends[i] become sequence i and the end of its range.
 qxc_status check_rows(qxc_ctx* ctx, const qxc_kv* kv, int layer_begin, int layer_count, int seq_count,
                       const int32_t* seq_ids, const int32_t* begins, const int32_t* counts, std::vector<int>* ids,
                       std::vector<int>* ends, long long* total) {
@@ -1287,6 +1287,7 @@ qxc_status attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
     if (a->lengths[i]) prompts.push_back({token, a->lengths[i], 0});
     token += a->lengths[i];
   }
+  p.tokens = token;
   // the longest work items first: what is left at the end of a launch is short
   std::stable_sort(prompts.begin(), prompts.end(),
                    [](const PackedSeq& x, const PackedSeq& y) { return x.length > y.length; });
@@ -1794,7 +1795,7 @@ qxc_status qxc_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
     if (st != QXC_OK) return st;
   }
   if (is_q4(kv)) {
-    qxc_status st = q4_decode(ctx, kv, a);
+    qxc_status st = guarded(ctx, [&] { return q4_decode(ctx, kv, a); });
     if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
       for (int i = 0; i < a->seq_count; ++i) kv->len[a->seq_ids ? a->seq_ids[i] : i] += 1;
     return st;
@@ -2800,6 +2801,8 @@ qxc_status qxc_attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
 qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed_args* a) {
   if (!ctx || !kv || !a) return fail(ctx, QXC_ERR_INVALID_ARG, "null argument");
   return guarded(ctx, [&]() -> qxc_status {
+    if (kv->ctx != ctx) return fail(ctx, QXC_ERR_INVALID_ARG, "KV arena belongs to another context");
+    if (!is_q4(kv)) return fail(ctx, QXC_ERR_UNSUPPORTED, "the call needs a 4-bit arena");
     long long total;
     qxc_status st = check_lengths(ctx, a->seq_count, a->lengths, &total);
     if (st != QXC_OK) return st;

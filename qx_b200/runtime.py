@@ -61,12 +61,22 @@ def _i32(values):
     return None if values is None else (C.c_int32 * len(values)).from_buffer(array("i", values))
 
 
-def _token_stride(x, features: int) -> int:
-    """Elements between the tokens of a tensor [tokens, ...] whose remaining
-    dimensions are dense and hold `features` elements; 0 (dense) for a raw
-    pointer."""
+def _room(x, elements: int):
+    """The pointer of a dense tensor of at least `elements` elements; a raw
+    pointer as it is."""
+    if hasattr(x, "numel") and x.numel() < elements:
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {x.numel()} elements, {elements} needed")
+    return _ptr(x)
+
+
+def _token_stride(x, features: int, tokens: int = 0) -> int:
+    """Elements between the tokens of a tensor [tokens, ...], `tokens` of them
+    at least, whose remaining dimensions are dense and hold `features`
+    elements; 0 (dense) for a raw pointer."""
     if x is None or isinstance(x, int) or not hasattr(x, "stride"):
         return 0
+    if x.shape[0] < tokens:
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {x.shape[0]} tokens, {tokens} needed")
     if x.is_contiguous() and x.numel() == x.shape[0] * features:
         return features if x.shape[0] > 1 else 0
     shape, stride, dense = tuple(x.shape), tuple(x.stride()), 1
@@ -164,9 +174,10 @@ class Context:
         tensors [tokens, ...] of `dtype`, their token strides taken from the
         tensors; out is dense."""
         hq, hkv, d = model_shape(model)
-        n = _i32(lengths)
-        a = _lib.PackedArgs(model, len(lengths), n, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _token_stride(q, hq * d),
-                            _token_stride(k, hkv * d), _token_stride(v, hkv * d), dtype)
+        n, tokens = _i32(lengths), sum(lengths)
+        a = _lib.PackedArgs(model, len(lengths), n, _ptr(q), _ptr(k), _ptr(v), _room(out, tokens * hq * d),
+                            _token_stride(q, hq * d, tokens), _token_stride(k, hkv * d, tokens),
+                            _token_stride(v, hkv * d, tokens), dtype)
         self.check(self.lib.qxc_attend_packed(self.handle, C.byref(a)))
 
     def lse_merge(self, model: int, n_parts: int, partials, out, out_dtype: int = F32) -> None:
@@ -380,6 +391,11 @@ class KvArena:
             return BF16 if self.model == MODEL_QWEN3 else F32
         return self.key_dtype if self.model == MODEL_QWEN3 else F32
 
+    def _tokens(self, counts) -> int:
+        """Tokens that the tensors of a call hold at least; 0 for counts that
+        no sequence has room for, which the call refuses."""
+        return sum(counts) if max(counts, default=0) <= self.capacity else 0
+
     def append(self, q, k, v, positions, counts, seq_ids=None, layer_begin: int = 0, layer_count: int | None = None,
                in_dtype: int | None = None, q_rot=None, k_rot=None, rot_dtype: int = BF16, q_norm=None, k_norm=None,
                flags: int = 0) -> None:
@@ -392,9 +408,11 @@ class KvArena:
         if len(counts) != len(positions) or (seq_ids is not None and len(seq_ids) != len(positions)):
             raise QxError(_lib.ERR_INVALID_ARG, "positions, counts and seq_ids differ in length")
         qn, kn = layer_count * self.hq * self.d, layer_count * self.hkv * self.d
+        tokens = self._tokens(counts)
         a = _lib.AppendArgs(layer_begin, layer_count, len(positions), _i32(seq_ids), _i32(positions), _i32(counts),
-                            _ptr(q), _ptr(k), _ptr(v), _ptr(q_rot), _ptr(k_rot), _token_stride(q, qn),
-                            _token_stride(k, kn), _token_stride(v, kn), _ptr(q_norm), _ptr(k_norm),
+                            _ptr(q), _ptr(k), _ptr(v), _room(q_rot, tokens * qn), _room(k_rot, tokens * kn),
+                            _token_stride(q, qn, tokens), _token_stride(k, kn, tokens),
+                            _token_stride(v, kn, tokens), _ptr(q_norm), _ptr(k_norm),
                             self._default_dtype() if in_dtype is None else in_dtype, rot_dtype, flags)
         self.ctx.check(self.lib.qxc_kv_append(self.ctx.handle, self.handle, C.byref(a)))
 
@@ -406,8 +424,9 @@ class KvArena:
         layer_count = self.layers - layer_begin if layer_count is None else layer_count
         if len(counts) != len(begins) or (seq_ids is not None and len(seq_ids) != len(begins)):
             raise QxError(_lib.ERR_INVALID_ARG, "begins, counts and seq_ids differ in length")
+        elements = self._tokens(counts) * layer_count * self.hkv * self.d
         a = _lib.ReadRowsArgs(layer_begin, layer_count, len(begins), _i32(seq_ids), _i32(begins), _i32(counts),
-                              _ptr(key_out), _ptr(value_out), out_dtype)
+                              _room(key_out, elements), _room(value_out, elements), out_dtype)
         self.ctx.check(self.lib.qxc_kv_read_rows(self.ctx.handle, self.handle, C.byref(a)))
 
     def prefill_packed(self, q, k, v, out, lengths, seq_ids=None, layer: int = 0, dtype: int = BF16, q_norm=None,
@@ -417,10 +436,10 @@ class KvArena:
         [tokens, ...] of `dtype`, token strides taken from the tensors."""
         if seq_ids is not None and len(seq_ids) != len(lengths):
             raise QxError(_lib.ERR_INVALID_ARG, "lengths and seq_ids differ in length")
-        qn, kn = self.hq * self.d, self.hkv * self.d
+        qn, kn, tokens = self.hq * self.d, self.hkv * self.d, self._tokens(lengths)
         a = _lib.PrefillPackedArgs(layer, len(lengths), _i32(seq_ids), _i32(lengths), _ptr(q), _ptr(k), _ptr(v),
-                                   _ptr(out), _token_stride(q, qn), _token_stride(k, kn), _token_stride(v, kn),
-                                   _ptr(q_norm), _ptr(k_norm), dtype, flags)
+                                   _room(out, tokens * qn), _token_stride(q, qn, tokens),
+                                   _token_stride(k, kn, tokens), _token_stride(v, kn, tokens), _ptr(q_norm), _ptr(k_norm), dtype, flags)
         self.ctx.check(self.lib.qxc_prefill_packed(self.ctx.handle, self.handle, C.byref(a)))
 
     def _decode_args(self, q, k, v, out, positions, layer_begin, layer_count, seq_ids, q_dtype, in_dtype,

@@ -127,6 +127,59 @@ def test_what_a_row_does_not_attend_does_not_reach_it(gpu_ctx, model, bad):
 
 
 @pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_bad_value_reaches_its_own_dim_only(gpu_ctx, model, dtype):
+    """Values of two dims are bad from one token on: the rows from it on have
+    these dims not finite and the others right, the rows before it all right."""
+    rng = np.random.default_rng([model, dtype, 20])
+    n = 300
+    q, k, v = inputs(rng, model, n, dtype)
+    bad = {130: (5, float("nan")), 201: (40, float("-inf"))}
+    clean = v.clone()
+    for at, (dim, x) in bad.items():
+        v[at:, :, dim] = x
+    out = torch.zeros_like(q)
+    gpu_ctx.attend_packed(model, q, k, v, out, [n], dtype=dtype)
+    with pytest.raises(QxError) as e:
+        gpu_ctx.sync()
+    assert e.value.status == _lib.ERR_NONFINITE
+    for at, (dim, _) in bad.items():
+        assert not torch.isfinite(out[at:, :, dim]).any()
+        out[at:, :, dim] = 0.0
+        clean[at:, :, dim] = 0.0
+    # a zeroed value from a row on is a zeroed output from it on, the rows before are as they were
+    for at, (dim, _) in bad.items():
+        check_dim(model, q, k, v, out, at, dim, dtype)
+    assert torch.isfinite(out).all()
+    keep = [d for d in range(q.shape[2]) if d not in (5, 40)]
+    check_columns(model, q, k, clean, out, n, dtype, keep)
+
+
+def check_columns(model, q, k, v, out, n, dtype, columns):
+    """As check() for one prompt, some of its output dims."""
+    only = torch.zeros(v.shape[2], device="cuda", dtype=v.dtype)
+    only[columns] = 1.0
+    check(model, q, k, v * only, out * only, [n], dtype)
+
+
+def check_dim(model, q, k, v, out, end, dim, dtype):
+    """As check() for the rows before `end` and one dim."""
+    check_columns(model, q[:end], k[:end], torch.nan_to_num(v[:end], 0, 0, 0), out[:end], end, dtype, [dim])
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_values_that_are_all_bad(gpu_ctx, model):
+    rng = np.random.default_rng(21)
+    q, k, v = inputs(rng, model, 3000, BF16)
+    v[:] = float("nan")
+    out = torch.zeros_like(q)
+    gpu_ctx.attend_packed(model, q, k, v, out, [3000])
+    with pytest.raises(QxError) as e:
+        gpu_ctx.sync()
+    assert e.value.status == _lib.ERR_NONFINITE and torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("model", MODELS)
 @pytest.mark.parametrize("scale", [0.0, 30.0])
 def test_flat_and_peaked_scores(gpu_ctx, model, scale):
     rng = np.random.default_rng(5)
@@ -172,6 +225,62 @@ def test_captured_and_replayed(gpu_ctx):
             stream.synchronize()
             check(MODEL_QWEN3, q, k, v, out, lengths, BF16, heads=[0, 17])
     gpu_ctx.set_stream(old)
+
+
+def test_captured_prefill_outlives_a_larger_one(gpu_ctx):
+    """A captured prefill keeps its workspace when a later call needs a larger one."""
+    rng = np.random.default_rng(22)
+    old, stream = gpu_ctx.stream, torch.cuda.Stream()
+    small = KvArena(gpu_ctx, MODEL_GRANITE, 1, 2, 40, Q4)
+    q, k, v = inputs(rng, MODEL_GRANITE, 60, BF16)
+    out = torch.zeros_like(q)
+    go = lambda: small.prefill_packed(q, k, v, out, [40, 20], flags=_lib.DECODE_NO_ADVANCE)  # noqa: E731
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        gpu_ctx.set_stream(stream)
+        go()
+        stream.synchronize()
+        want, rows = out.clone(), [small.read(i, 0, 0, n) for i, n in enumerate((40, 20))]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            go()
+        lengths = [3000] * 40  # past any call of these tests
+        large = KvArena(gpu_ctx, MODEL_GRANITE, 1, 40, 3000, Q4)
+        lq, lk, lv = (torch.zeros(sum(lengths), h, 64, device="cuda", dtype=torch.bfloat16) for h in (16, 8, 8))
+        large.prefill_packed(lq, lk, lv, lq.clone(), lengths)
+        out.zero_()
+        graph.replay()
+        stream.synchronize()
+    gpu_ctx.set_stream(old)
+    gpu_ctx.sync()
+    assert torch.equal(out, want)
+    for i, n in enumerate((40, 20)):
+        assert all(np.array_equal(a, b) for a, b in zip(small.read(i, 0, 0, n), rows[i]))
+    small.close()
+    large.close()
+
+
+def test_prefill_of_more_sequences_than_a_launch_holds(gpu_ctx):
+    rng = np.random.default_rng(23)
+    lengths = [int(x) for x in rng.integers(0, 5, 230)]
+    ids = [int(x) for x in rng.permutation(230)]
+    arena = KvArena(gpu_ctx, MODEL_QWEN3, 1, 230, 5, Q4)
+    q, k, v = inputs(rng, MODEL_QWEN3, sum(lengths), BF16)
+    out = torch.zeros_like(q)
+    arena.prefill_packed(q, k, v, out, lengths, seq_ids=ids)
+    gpu_ctx.sync()
+    begin = 0
+    for i, n in zip(ids, lengths):
+        rows = slice(begin, begin + n)
+        begin += n
+        assert arena.len(i) == n
+        if n:
+            qr, kr = (torch.from_numpy(ref.rotate64(MODEL_QWEN3, host(x[rows]), range(n), None)) for x in (q, k))
+            check_rounded(MODEL_QWEN3, qr, kr, v[rows], out[rows])
+            (_, _), (vc, vs) = stored(arena, i, 0, 0, n)
+            want = ref.quantise(v[rows].float().cpu().numpy())
+            assert np.array_equal(vc, want[0]) and np.array_equal(vs, want[1])
+    arena.close()
 
 
 @pytest.mark.parametrize("model", MODELS)
@@ -256,6 +365,8 @@ def test_refusals(gpu_ctx):
     refused(bad, lambda: go(q, k, k, flat[1:1 + 64 * 1024].view(64, 16, 64), [3]))
     odd = torch.as_strided(flat, (50, 16, 64), (1028, 64, 1))
     refused(bad, lambda: go(odd, k, k, q, [3]))
+    refused(bad, lambda: go(q, k[:2], k, q, [3]))
+    refused(bad, lambda: go(q, k, k, q[:2], [3]))
     arena = KvArena(gpu_ctx, MODEL_GRANITE, 1, 2, 16, Q4)
     pre = lambda lengths, a=arena, **kw: a.prefill_packed(q, k, k, q.clone(), lengths, **kw)  # noqa: E731
     refused(_lib.ERR_POSITION, lambda: pre([17]))
@@ -263,6 +374,8 @@ def test_refusals(gpu_ctx):
     refused(bad, lambda: pre([1, 1, 1]))
     refused(bad, lambda: pre([1], layer=1))
     refused(unsupported, lambda: pre([1], dtype=F32))
+    refused(bad, lambda: arena.prefill_packed(q, k, k[:3], q.clone(), [2, 2]))
+    refused(bad, lambda: arena.prefill_packed(q, k, k, q[:3].clone(), [2, 2]))
     plain = KvArena(gpu_ctx, MODEL_GRANITE, 1, 2, 16, BF16)
     refused(unsupported, lambda: pre([1], plain))
     pre([3, 2])

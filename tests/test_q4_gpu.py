@@ -21,7 +21,7 @@ import pytest
 import torch
 
 import q4_reference as ref
-from qx_b200 import (BF16, DECODE_NO_ADVANCE, F16, F32, MODEL_GRANITE, MODEL_QWEN3, Q4, KvArena, QxError, _lib)
+from qx_b200 import (BF16, DECODE_NO_ADVANCE, F16, F32, MODEL_GRANITE, MODEL_QWEN3, Q4, Context, KvArena, QxError, _lib)
 from qx_b200.runtime import model_shape
 
 pytestmark = pytest.mark.gpu
@@ -452,6 +452,104 @@ def test_decode_captured_and_replayed(gpu_ctx):
             stream.synchronize()
             check_decode(gpu_ctx, arena, q, k, v, out, [3000, 40], F32)
     gpu_ctx.set_stream(old)
+    arena.close()
+
+
+def test_a_captured_step_outlives_a_larger_one():
+    """A captured decode keeps its workspace when a later call needs a larger
+    one; a call that needs a larger one cannot be captured."""
+    rng = np.random.default_rng(19)
+    ctx = Context(0)
+    stream = torch.cuda.Stream()
+    arena = make_arena(ctx, MODEL_GRANITE, [701] * 30, layers=3)
+    fill(ctx, arena, rng, [700] * 30)
+    q, k, v = (tensor(rng, (1, 3, h, 64), BF16) for h in (16, 8, 8))
+    out = torch.zeros(1, 3, 16, 64, device="cuda")
+    small = lambda: arena.decode(q, k, v, out, [700], q_dtype=BF16, in_dtype=BF16, flags=DECODE_NO_ADVANCE)  # noqa: E731
+    lq, lk, lv = (tensor(rng, (30, 3, h, 64), BF16) for h in (16, 8, 8))
+    lout = torch.zeros(30, 3, 16, 64, device="cuda")
+    large = lambda: arena.decode(lq, lk, lv, lout, [700] * 30, q_dtype=BF16, in_dtype=BF16, flags=DECODE_NO_ADVANCE)  # noqa: E731
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        ctx.set_stream(stream)
+        small()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            small()
+        with pytest.raises(QxError) as e:
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                small()  # a graph with no node cannot be made
+                large()
+        assert e.value.status == _lib.ERR_UNSUPPORTED
+        for _ in range(2):
+            large()
+            stream.synchronize()
+            check_decode(ctx, arena, lq, lk, lv, lout, [700] * 30, F32)
+            out.zero_()
+            graph.replay()
+            stream.synchronize()
+            check_decode(ctx, arena, q, k, v, out, [700], F32)
+    ctx.sync()
+    arena.close()
+    ctx.close()
+
+
+def test_two_contexts_at_once(gpu_ctx):
+    """Contexts of their own stream and workspaces do not wait for each other."""
+    rng = np.random.default_rng(24)
+    both = [(Context(0), m) for m in MODELS]
+    work = []
+    for ctx, model in both:
+        arena = make_arena(ctx, model, [2001, 301])
+        fill(ctx, arena, rng, [2000, 300])
+        q, k, v = (tensor(rng, (2, 1, h, arena.d), BF16) for h in (arena.hq, arena.hkv, arena.hkv))
+        work.append((ctx, arena, q, k, v, torch.zeros(2, 1, arena.hq, arena.d, device="cuda")))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for ctx, arena, q, k, v, out in work:
+            arena.decode(q, k, v, out, [2000, 300], q_dtype=BF16, in_dtype=BF16, flags=DECODE_NO_ADVANCE)
+    for ctx, arena, q, k, v, out in work:
+        ctx.sync()
+        check_decode(ctx, arena, q, k, v, out, [2000, 300], F32)
+        arena.close()
+        ctx.close()
+
+
+def test_offsets_past_32_bits(gpu_ctx):
+    """The last rows of an arena whose keys alone pass 2^32 bytes: written, read
+    back and attended, its other cells left as they were."""
+    rng = np.random.default_rng(25)
+    cap, layers, seqs = 40960, 40, 10
+    arena = KvArena(gpu_ctx, MODEL_QWEN3, layers, seqs, cap, Q4)
+    assert cap * layers * seqs * 288 > 2 ** 32
+    k, v = (tensor(rng, (cap - 1, 4, 128), BF16) for _ in range(2))
+    arena.append(None, k, v, [0], [cap - 1], seq_ids=[seqs - 1], layer_begin=layers - 1, layer_count=1, in_dtype=BF16)
+    gpu_ctx.sync()
+    keys, values = (torch.zeros(3, 1, 4, 128, device="cuda") for _ in range(2))
+    arena.read_rows(keys, values, [cap - 4], [3], seq_ids=[seqs - 1], layer_begin=layers - 1, layer_count=1)
+    gpu_ctx.sync()
+    codes, scales = ref.quantise(v[-3:].float().cpu().numpy())
+    assert np.array_equal(host(values)[:, 0], ref.values(codes, scales))
+    run_decode(gpu_ctx, arena, rng, [cap - 1], BF16, F32, ids=[seqs - 1], layer_begin=layers - 1, layer_count=1)
+    arena.close()
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rotation_in_place(gpu_ctx, model, dtype):
+    rng = np.random.default_rng([model, dtype, 26])
+    arena = make_arena(gpu_ctx, model, [130, 130])
+    qw, kw = norms(rng, model)
+    q, k, v = (tensor(rng, (130, h, arena.d), dtype) for h in (arena.hq, arena.hkv, arena.hkv))
+    got = []
+    for seq, (a, b) in enumerate(((torch.zeros_like(q), torch.zeros_like(k)), (q, k))):
+        arena.append(q, k, v, [0], [130], seq_ids=[seq], q_rot=a, k_rot=b, in_dtype=dtype, rot_dtype=dtype, q_norm=qw,
+                     k_norm=kw)
+        gpu_ctx.sync()
+        got.append((a, b, *arena.read(seq, 0, 0, 130)))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert all(np.array_equal(x, y) for x, y in zip(got[0][2:], got[1][2:]))
     arena.close()
 
 
