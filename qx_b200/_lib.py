@@ -107,8 +107,8 @@ class StaticDecodeArgs(C.Structure):
 class AppendArgs(C.Structure):
     """qxc_append_args (rows of new tokens into a 4-bit arena)."""
     _fields_ = [("layer_begin", C.c_int32), ("layer_count", C.c_int32), ("seq_count", C.c_int32),
-                ("seq_ids", C.POINTER(C.c_int32)), ("positions", C.POINTER(C.c_int32)),
-                ("counts", C.POINTER(C.c_int32)), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("seq_ids", C.c_void_p), ("positions", C.c_void_p),
+                ("counts", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
                 ("q_rot", C.c_void_p), ("k_rot", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
                 ("v_stride", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("in_dtype", C.c_int32),
                 ("rot_dtype", C.c_int32), ("flags", C.c_int32)]
@@ -117,22 +117,22 @@ class AppendArgs(C.Structure):
 class ReadRowsArgs(C.Structure):
     """qxc_read_rows_args (rows of a 4-bit arena as values)."""
     _fields_ = [("layer_begin", C.c_int32), ("layer_count", C.c_int32), ("seq_count", C.c_int32),
-                ("seq_ids", C.POINTER(C.c_int32)), ("begins", C.POINTER(C.c_int32)),
-                ("counts", C.POINTER(C.c_int32)), ("key_out", C.c_void_p), ("value_out", C.c_void_p),
+                ("seq_ids", C.c_void_p), ("begins", C.c_void_p),
+                ("counts", C.c_void_p), ("key_out", C.c_void_p), ("value_out", C.c_void_p),
                 ("out_dtype", C.c_int32)]
 
 
 class PackedArgs(C.Structure):
     """qxc_packed_args (causal attention of packed prompts)."""
-    _fields_ = [("model", C.c_int32), ("seq_count", C.c_int32), ("lengths", C.POINTER(C.c_int32)),
+    _fields_ = [("model", C.c_int32), ("seq_count", C.c_int32), ("lengths", C.c_void_p),
                 ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
                 ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("dtype", C.c_int32)]
 
 
 class PrefillPackedArgs(C.Structure):
     """qxc_prefill_packed_args (packed prompts into a 4-bit arena)."""
-    _fields_ = [("layer", C.c_int32), ("seq_count", C.c_int32), ("seq_ids", C.POINTER(C.c_int32)),
-                ("lengths", C.POINTER(C.c_int32)), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+    _fields_ = [("layer", C.c_int32), ("seq_count", C.c_int32), ("seq_ids", C.c_void_p),
+                ("lengths", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
                 ("out", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
                 ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("dtype", C.c_int32), ("flags", C.c_int32)]
 

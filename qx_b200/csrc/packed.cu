@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
 }
 
 template <class M, typename T>
-cudaError_t packed(const PackedParams& p, cudaStream_t stream) {
+cudaError_t setup() {
   using C = Packed<M, T>;
   cudaError_t e = cudaFuncSetAttribute(qx_packed_kernel<M, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;
@@ -520,7 +520,12 @@ cudaError_t packed(const PackedParams& p, cudaStream_t stream) {
   cudaFuncAttributes fa;
   e = cudaFuncGetAttributes(&fa, qx_packed_kernel<M, T>);
   if (e != cudaSuccess) return e;
-  if (fa.numRegs * C::NT < C::REGS * 256 + C::REGS_OTHER * 128) return cudaErrorLaunchOutOfResources;
+  return fa.numRegs * C::NT < C::REGS * 256 + C::REGS_OTHER * 128 ? cudaErrorLaunchOutOfResources : cudaSuccess;
+}
+
+template <class M, typename T>
+cudaError_t packed(const PackedParams& p, cudaStream_t stream) {
+  using C = Packed<M, T>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.items);
   cfg.blockDim = dim3(C::NT);
@@ -535,6 +540,13 @@ cudaError_t packed(const PackedParams& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t setup_packed() {
+  for (cudaError_t e : {setup<Qwen3Heads, __nv_bfloat16>(), setup<Qwen3Heads, __half>(),
+                        setup<GraniteHeads, __nv_bfloat16>(), setup<GraniteHeads, __half>()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
+}
 
 cudaError_t launch_packed(bool qwen, const PackedParams& p, cudaStream_t stream) {
   if (p.dtype == 1)

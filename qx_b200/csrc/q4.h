@@ -122,7 +122,11 @@ constexpr int kPackedKeys = 128;  // keys of a tile
 
 cudaError_t launch_q4_append(bool qwen, const Q4AppendParams& p, cudaStream_t stream);
 cudaError_t launch_q4_read(bool qwen, const Q4ReadParams& p, cudaStream_t stream);
-// The decode and, where p.split says so, the merge; the kernels launched.
+// The kernels' attributes on the current device, before the first launch there.
+cudaError_t setup_q4_decode();
+cudaError_t setup_packed();
+// The preparation, the attention and, where CTAs share cells, the merge; the
+// kernels launched.
 cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream, int* launched);
 // Decode CTAs resident on one SM.
 int q4_decode_blocks_per_sm();

@@ -744,13 +744,15 @@ cudaError_t launch_dependent(void (*fn)(Q4DecodeParams), int blocks, int threads
 }
 
 template <class M, int OUT>
+cudaError_t setup() {
+  return cudaFuncSetAttribute(qx_q4_decode_kernel<M, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Dec<M>::SMEM);
+}
+
+template <class M, int OUT>
 cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
-  constexpr int SMEM = Dec<M>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(qx_q4_decode_kernel<M, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e != cudaSuccess) return e;
   const int cells = p.n_seq * p.layer_count, ctas = (p.total + p.per_cta - 1) / p.per_cta;
-  e = launch_dependent(qx_q4_prepare_kernel<M, Need<OUT>::PAIRS>, cells, 32 * (Dec<M>::UNITS + 4), 0, stream, p, launched);
-  if (e == cudaSuccess) e = launch_dependent(qx_q4_decode_kernel<M, OUT>, ctas, kThreads, SMEM, stream, p, launched);
+  cudaError_t e = launch_dependent(qx_q4_prepare_kernel<M, Need<OUT>::PAIRS>, cells, 32 * (Dec<M>::UNITS + 4), 0, stream, p, launched);
+  if (e == cudaSuccess) e = launch_dependent(qx_q4_decode_kernel<M, OUT>, ctas, kThreads, Dec<M>::SMEM, stream, p, launched);
   if (e != cudaSuccess || p.max_parts == 1) return e;
   constexpr int OUTPUTS = M::HQ * M::D;
   if (p.max_parts <= 8)
@@ -759,6 +761,13 @@ cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) 
 }
 
 }  // namespace
+
+cudaError_t setup_q4_decode() {
+  for (cudaError_t e : {setup<Qwen3Heads, 0>(), setup<Qwen3Heads, 1>(), setup<Qwen3Heads, 2>(), setup<GraniteHeads, 0>(),
+                        setup<GraniteHeads, 1>(), setup<GraniteHeads, 2>()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
+}
 
 cudaError_t launch_q4_decode(bool qwen, const Q4DecodeParams& p, cudaStream_t stream, int* launched) {
   *launched = 0;

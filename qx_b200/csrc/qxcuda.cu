@@ -99,6 +99,7 @@ struct qxc_ctx {
   // outgrown are kept until the context goes, since a captured graph may
   // still name them
   Workspace q4_work, packed_rot;
+  bool q4_decode_set = false, packed_set = false;  // their kernels' attributes
   std::vector<void*> outgrown;
   // prefill's rotated-query scratch (bf16 elements)
   unsigned short* prefill_q = nullptr;
@@ -1169,6 +1170,10 @@ int q4_least_tiles(int total, int sms) { return std::max(2, std::min(8, (total +
 
 // One decode step on a 4-bit arena, its arguments checked and its pages mapped.
 qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
+  if (!ctx->q4_decode_set) {
+    QXC_CUDA(ctx, setup_q4_decode());
+    ctx->q4_decode_set = true;
+  }
   std::vector<int32_t> attend(a->seq_count), ones(a->seq_count, 1);
   for (int i = 0; i < a->seq_count; ++i) attend[i] = a->positions[i] + 1;
   Q4DecodeParams p;
@@ -1281,6 +1286,10 @@ qxc_status attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
     return fail(ctx, QXC_ERR_INVALID_ARG, "packed tensors must be 16-byte aligned, their token strides multiples of 8");
   if (p.q_stride < (long long)hq * d || p.k_stride < (long long)hkv * d || p.v_stride < (long long)hkv * d)
     return fail(ctx, QXC_ERR_INVALID_ARG, "a token stride is shorter than a token's heads");
+  if (!ctx->packed_set) {
+    QXC_CUDA(ctx, setup_packed());
+    ctx->packed_set = true;
+  }
   std::vector<PackedSeq> prompts;
   int token = 0;
   for (int i = 0; i < a->seq_count; ++i) {

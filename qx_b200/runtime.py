@@ -61,6 +61,18 @@ def _i32(values):
     return None if values is None else (C.c_int32 * len(values)).from_buffer(array("i", values))
 
 
+_no_ints = array("i")
+
+
+def _ints(values):
+    """A host int32 array of `values`, to be kept while a call reads it, and
+    its address; None gives address None."""
+    if values is None:
+        return _no_ints, None
+    a = array("i", values)
+    return a, a.buffer_info()[0]
+
+
 def _room(x, elements: int):
     """The pointer of a dense tensor of at least `elements` elements; a raw
     pointer as it is."""
@@ -174,7 +186,7 @@ class Context:
         tensors [tokens, ...] of `dtype`, their token strides taken from the
         tensors; out is dense."""
         hq, hkv, d = model_shape(model)
-        n, tokens = _i32(lengths), sum(lengths)
+        (keep, n), tokens = _ints(lengths), sum(lengths)
         a = _lib.PackedArgs(model, len(lengths), n, _ptr(q), _ptr(k), _ptr(v), _room(out, tokens * hq * d),
                             _token_stride(q, hq * d, tokens), _token_stride(k, hkv * d, tokens),
                             _token_stride(v, hkv * d, tokens), dtype)
@@ -409,7 +421,8 @@ class KvArena:
             raise QxError(_lib.ERR_INVALID_ARG, "positions, counts and seq_ids differ in length")
         qn, kn = layer_count * self.hq * self.d, layer_count * self.hkv * self.d
         tokens = self._tokens(counts)
-        a = _lib.AppendArgs(layer_begin, layer_count, len(positions), _i32(seq_ids), _i32(positions), _i32(counts),
+        (keep_s, ids), (keep_p, at), (keep_c, n) = _ints(seq_ids), _ints(positions), _ints(counts)
+        a = _lib.AppendArgs(layer_begin, layer_count, len(positions), ids, at, n,
                             _ptr(q), _ptr(k), _ptr(v), _room(q_rot, tokens * qn), _room(k_rot, tokens * kn),
                             _token_stride(q, qn, tokens), _token_stride(k, kn, tokens),
                             _token_stride(v, kn, tokens), _ptr(q_norm), _ptr(k_norm),
@@ -425,7 +438,8 @@ class KvArena:
         if len(counts) != len(begins) or (seq_ids is not None and len(seq_ids) != len(begins)):
             raise QxError(_lib.ERR_INVALID_ARG, "begins, counts and seq_ids differ in length")
         elements = self._tokens(counts) * layer_count * self.hkv * self.d
-        a = _lib.ReadRowsArgs(layer_begin, layer_count, len(begins), _i32(seq_ids), _i32(begins), _i32(counts),
+        (keep_s, ids), (keep_b, at), (keep_c, n) = _ints(seq_ids), _ints(begins), _ints(counts)
+        a = _lib.ReadRowsArgs(layer_begin, layer_count, len(begins), ids, at, n,
                               _room(key_out, elements), _room(value_out, elements), out_dtype)
         self.ctx.check(self.lib.qxc_kv_read_rows(self.ctx.handle, self.handle, C.byref(a)))
 
@@ -437,7 +451,8 @@ class KvArena:
         if seq_ids is not None and len(seq_ids) != len(lengths):
             raise QxError(_lib.ERR_INVALID_ARG, "lengths and seq_ids differ in length")
         qn, kn, tokens = self.hq * self.d, self.hkv * self.d, self._tokens(lengths)
-        a = _lib.PrefillPackedArgs(layer, len(lengths), _i32(seq_ids), _i32(lengths), _ptr(q), _ptr(k), _ptr(v),
+        (keep_s, ids), (keep_l, n) = _ints(seq_ids), _ints(lengths)
+        a = _lib.PrefillPackedArgs(layer, len(lengths), ids, n, _ptr(q), _ptr(k), _ptr(v),
                                    _room(out, tokens * qn), _token_stride(q, qn, tokens),
                                    _token_stride(k, kn, tokens), _token_stride(v, kn, tokens), _ptr(q_norm), _ptr(k_norm), dtype, flags)
         self.ctx.check(self.lib.qxc_prefill_packed(self.ctx.handle, self.handle, C.byref(a)))

@@ -577,6 +577,36 @@ def test_q4_layer_runs_on_a_4bit_arena(gpu_ctx):
     assert ((got[0] - got[1]).view(-1, 32).abs() <= step).all()
 
 
+@pytest.mark.parametrize("page", [0, 64])
+def test_a_stack_of_layers_on_a_4bit_arena(gpu_ctx, page):
+    """qxc_attention_stack is its layers one after another, bit for bit."""
+    rng = np.random.default_rng([27, page])
+    from qx_b200 import Q4Weights
+
+    def weights(rows):
+        codes = torch.from_numpy(rng.integers(0, 256, (rows, 32, 16), dtype=np.uint8)).cuda()
+        return Q4Weights(codes, torch.full((rows, 32), 0.01, dtype=torch.float16).cuda(), rows, 1024)
+    layers = [{"norm": torch.ones(1024, device="cuda"), **{n: weights(r) for n, r in zip("qkvo", (1024, 512, 512, 1024))}}
+              for _ in range(3)]
+    stack, chain = (KvArena(gpu_ctx, MODEL_GRANITE, 3, 1, 70, Q4, page_size=page, pool_pages=2 if page else 0) for _ in range(2))
+    for position in range(66):
+        x = tensor(rng, (1024,), F32)
+        out, y = torch.zeros(1024, device="cuda"), x.clone()
+        stack.attention_stack(x, out, layers, position)
+        for i, w in enumerate(layers):
+            z = torch.zeros(1024, device="cuda")
+            chain.attention_layer(y, z, w["norm"], w["q"], w["k"], w["v"], w["o"], position=position, layer=i,
+                                  flags=DECODE_NO_ADVANCE if i < 2 else 0)
+            y = z
+        gpu_ctx.sync()
+        assert torch.equal(out, y) and torch.isfinite(y).all()
+    assert stack.len(0) == chain.len(0) == 66
+    for i in range(3):
+        assert all(np.array_equal(a, b) for a, b in zip(stack.read(0, i, 0, 66), chain.read(0, i, 0, 66)))
+    stack.close()
+    chain.close()
+
+
 def test_refusals(gpu_ctx):
     arena = KvArena(gpu_ctx, MODEL_GRANITE, 2, 2, 64, Q4)
     plain = KvArena(gpu_ctx, MODEL_GRANITE, 1, 1, 64, F32)
