@@ -110,9 +110,9 @@ __device__ __forceinline__ float key_inv_rms(const float* x) {
 // The operation order is each model's: granite_rope_pair's fused pair
 // (qx-consensus-math lib.rs:199-207), cpu_qk_norm_rope's separately rounded
 // one (qx-qwen-parity main.rs:1170-1210). tab: the table's entries of these dims
-// (rope_of_lane). False when a result is not finite.
+// (rope_of_lane).
 template <class M>
-__device__ __forceinline__ bool rotate_key(float* x, int c, const float* norm, const float2* tab) {
+__device__ __forceinline__ void rotate_key(float* x, int c, const float* norm, const float2* tab) {
   constexpr int LPH = Q4Row<M>::LPH;
   if constexpr (M::QWEN) {
     const float inv = key_inv_rms<M>(x);
@@ -120,7 +120,6 @@ __device__ __forceinline__ bool rotate_key(float* x, int c, const float* norm, c
     for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inv), norm ? norm[8 * c + e] : 1.0f);
   }
   const bool right = c >= LPH / 2;
-  bool good = true;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float y = __shfl_xor_sync(0xffffffffu, x[e], LPH / 2);
@@ -130,9 +129,7 @@ __device__ __forceinline__ bool rotate_key(float* x, int c, const float* norm, c
                    : __fsub_rn(__fmul_rn(x[e], t.x), __fmul_rn(y, t.y));
     else
       x[e] = right ? __fmaf_rn(x[e], t.y, __fmul_rn(y, t.x)) : __fmaf_rn(-y, t.x, __fmul_rn(x[e], t.y));
-    good &= isfinite(x[e]);
   }
-  return good;
 }
 
 // The rotation table's entries of lane c's dims at `position`.
@@ -148,15 +145,16 @@ __device__ __forceinline__ void rope_of_lane(const float2* rope, int position, i
   }
 }
 
-// Codes -7..7 of this lane's eight dims and its group's scale. False when the scale is not finite: a value above 7 * 65504, an
-// infinity, or a NaN (which fmaxf alone would drop).
-__device__ __forceinline__ bool quantise8(const float* x, int* codes, __half* scale) {
+// The codes of this lane's eight dims, each plus `offset` (0 or 7) in the low byte
+// of an integer, and its group's scale. False when the scale is not finite: a value
+// above 7 * 65504, an infinity, or a NaN (which fmaxf alone would drop).
+__device__ __forceinline__ bool quantise8(const float* x, int offset, uint32_t* codes, __half* scale) {
   float top = 0.0f;
-  bool good = true;
+  float2 bad = make_float2(0.0f, 0.0f);  // NaN once a value is not finite
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    top = fmaxf(top, fabsf(x[e]));
-    good &= isfinite(x[e]);
+  for (int e = 0; e < 8; e += 2) {
+    top = fmax3f(top, fabsf(x[e]), fabsf(x[e + 1]));
+    bad = __ffma2_rn(make_float2(x[e], x[e + 1]), make_float2(0.0f, 0.0f), bad);
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -166,38 +164,46 @@ __device__ __forceinline__ bool quantise8(const float* x, int* codes, __half* sc
   const float guess = __fmul_rn(top, SEVENTH);
   const __half h = __float2half_rn(__fmaf_rn(__fmaf_rn(-7.0f, guess, top), SEVENTH, guess));
   const float s = __half2float(h);
-  // x / s rounded to an integer: a product with the approximate reciprocal is off
-  // by less than 2^-19 of a step, so only quotients closer than that to a border
-  // between two codes need the division itself
+  // x / s rounded to an integer, by adding 1.5 * 2^23: a product with the
+  // approximate reciprocal is off by less than 2^-19 of a step, so only quotients
+  // closer than that to a border between two codes need the division itself, and
+  // only the scales that fp16 rounds coarsely, its subnormals, need the limits
   float inv;
   asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  float border = 1.0f;  // the smallest distance of a quotient from a border
+  const float base = 12582912.0f + (float)offset;
+  float away = 0.0f;  // the largest distance of a quotient from its integer
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float q = x[e] * inv, n = rintf(q);
-    border = fminf(border, 0.5f - fabsf(q - n));
-    codes[e] = __float2int_rn(fminf(fmaxf(n, -7.0f), 7.0f));
+  for (int e = 0; e < 8; e += 2) {
+    const float2 q = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(inv, inv));
+    const float2 n = __fadd2_rn(q, make_float2(base, base));
+    const float2 back = __fadd2_rn(n, make_float2(-base, -base));
+    const float2 d = __ffma2_rn(back, make_float2(-1.0f, -1.0f), q);
+    away = fmax3f(away, fabsf(d.x), fabsf(d.y));
+    codes[e] = __float_as_uint(n.x);
+    codes[e + 1] = __float_as_uint(n.y);
   }
-  if (border < 3.0e-6f) {
+  if (away > 0.5f - 3.0e-6f || top * inv > 7.4f) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) codes[e] = __float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f));
+    for (int e = 0; e < 8; ++e)
+      codes[e] = (uint32_t)(__float2int_rn(fminf(fmaxf(__fdiv_rn(x[e], s), -7.0f), 7.0f)) + offset);
   }
   if (!(s > 0.0f)) {  // a scale that rounds to zero: every value is zero
 #pragma unroll
-    for (int e = 0; e < 8; ++e) codes[e] = 0;
+    for (int e = 0; e < 8; ++e) codes[e] = (uint32_t)offset;
   }
   *scale = h;
-  return good && isfinite(s);
+  return bad.x + bad.y == 0.0f && isfinite(s);
 }
 
-// This lane's eight codes as a word of a key row.
-__device__ __forceinline__ uint32_t key_codes(const int* c) {
-  uint32_t w = 0u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w |= ((uint32_t)c[i] & 15u) << (8 * i + 4) | ((uint32_t)c[4 + i] & 15u) << (8 * i);
-  }
-  return w;
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// This lane's eight codes (offset 0) as a word of a key row.
+__device__ __forceinline__ uint32_t key_codes(const uint32_t* c) {
+  const uint32_t high = low_bytes(c[0], c[1], c[2], c[3]), low = low_bytes(c[4], c[5], c[6], c[7]);
+  return ((high << 4) & 0xf0f0f0f0u) | (low & 0x0f0f0f0fu);
 }
 
 // Store this lane's word and scale as part of a key row.
@@ -208,13 +214,12 @@ __device__ __forceinline__ void put_key(char* row, int head, int c, uint32_t cod
 }
 
 // The halves g = 2 t (low 16 bits) and 2 t + 1 of a value row's group that
-// lane t of a quad stores: nibble i of half g comes from lane i, which holds
+// lane t of a quad stores, from its codes (offset 7): nibble i of half g comes from lane i, which holds
 // dims 8 i + g. Every lane of the warp takes part.
-__device__ __forceinline__ uint32_t value_halves(const int* c) {
+__device__ __forceinline__ uint32_t value_halves(const uint32_t* c) {
   const int lane = threadIdx.x & 31, t = lane & 3;
-  uint32_t codes = 0u, out = 0u;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) codes |= (uint32_t)(c[e] + 7) << (4 * e);
+  const uint32_t codes = low_bytes(c[0], c[2], c[4], c[6]) + 16u * low_bytes(c[1], c[3], c[5], c[7]);
+  uint32_t out = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = __shfl_sync(0xffffffffu, codes, (lane & ~3) + i) >> (8 * t);

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 4) qx_q4_append_kernel(co
   bool good = true;
   {
     float f[8];
-    int codes[8];
+    uint32_t codes[8];
     __half scale;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -124,14 +124,14 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 4) qx_q4_append_kernel(co
       f[2 * e] = z.x, f[2 * e + 1] = z.y;
     }
     if (value) {
-      good = quantise8(f, codes, &scale);
+      good = quantise8(f, 7, codes, &scale);
       put_value<M>(p.arena.v + row * kQ4RowBytes, kv, c, value_halves(codes), scale);
     } else {
       float2 tab[8];
       rope_of_lane<M>(p.rope, position, c, tab);
-      good = rotate_key<M>(f, c, p.k_norm, tab);
+      rotate_key<M>(f, c, p.k_norm, tab);
       if (p.k_rot) store8(p.k_rot, (cell * M::HKV + kv) * M::D + 8 * c, p.rot_dtype, VEC, f);
-      good &= quantise8(f, codes, &scale);
+      good = quantise8(f, 0, codes, &scale);
       put_key<M>(p.arena.k + row * kQ4RowBytes, kv, c, key_codes(codes), scale);
     }
   }

@@ -286,16 +286,16 @@ __global__ void __launch_bounds__(256) qx_q4_prepare_kernel(const __grid_constan
     const long long row = kv_row(p.arena.paging, p.arena.capacity, p.arena.layers, seq.seq, p.layer_begin + layer, position);
     float x[8];
     load8(value ? p.v : p.k, (cell * M::HKV + h) * M::D + 8 * c, p.in_dtype, p.vec, x);
-    int codes[8];
+    uint32_t codes[8];
     __half scale;
     if (value) {
-      good = quantise8(x, codes, &scale);
+      good = quantise8(x, 7, codes, &scale);
       put_value<M>(p.arena.v + row * kQ4RowBytes, h, c, value_halves(codes), scale);
     } else {
       float2 tab[8];
       rope_of_lane<M>(p.rope, position, c, tab);
-      good = rotate_key<M>(x, c, p.k_norm, tab);
-      good &= quantise8(x, codes, &scale);
+      rotate_key<M>(x, c, p.k_norm, tab);
+      good = quantise8(x, 0, codes, &scale);
       put_key<M>(p.arena.k + row * kQ4RowBytes, h, c, key_codes(codes), scale);
     }
   }
