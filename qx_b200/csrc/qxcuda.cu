@@ -1165,7 +1165,11 @@ qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
 }
 
 // Tiles that a CTA of a 4-bit decode takes at least: two (a group of warps each)
-// on the shortest lines, up to eight once that leaves a CTA for every SM.
+// on the shortest lines, up to eight once that leaves a CTA for every SM. Longer
+// stretches mean fewer parts to join, shorter ones more CTAs: this rule, always two,
+// always eight take 8.1, 8.1, 12.0 us for one Granite layer of 512 rows, 9.3, 9.3,
+// 13.0 for a Qwen3 layer of 2000, 14.1, 16.9, 14.3 for one of 32768, 11.9, 11.8,
+// 13.6 for 8 sequences of 1000.
 int q4_least_tiles(int total, int sms) { return std::max(2, std::min(8, (total + sms - 1) / sms)); }
 
 // One decode step on a 4-bit arena, its arguments checked and its pages mapped.
