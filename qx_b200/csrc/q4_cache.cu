@@ -89,7 +89,8 @@ __device__ __forceinline__ void store4(void* base, long long i, int dtype, bool 
 // neighbouring dims; a query's has dims 4 c .. 4 c + 3 and the four that they are
 // rotated with, so that it needs no other lane but for the norm. A lane has the
 // same dims in all its heads: it loads its rotation and norm weights once, and all
-// its inputs before it uses the first.
+// its inputs before it uses the first. (With those of 32-bit inputs in flight it
+// has 80 registers, of 16-bit ones 64: three CTAs an SM, four.)
 template <class M, bool WIDE, bool VEC>
 __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 4) qx_q4_append_kernel(const __grid_constant__ Q4AppendParams p) {
   using R = Q4Row<M>;

@@ -76,28 +76,39 @@ def _ints(values):
 def _room(x, elements: int):
     """The pointer of a dense tensor of at least `elements` elements; a raw
     pointer as it is."""
-    if hasattr(x, "numel") and x.numel() < elements:
-        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {x.numel()} elements, {elements} needed")
-    return _ptr(x)
+    if x is None:
+        return None
+    try:
+        held = x.numel()
+    except AttributeError:
+        return _ptr(x)
+    if held < elements:
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {held} elements, {elements} needed")
+    return x.data_ptr()
 
 
 def _token_stride(x, features: int, tokens: int = 0) -> int:
     """Elements between the tokens of a tensor [tokens, ...], `tokens` of them
     at least, whose remaining dimensions are dense and hold `features`
     elements; 0 (dense) for a raw pointer."""
-    if x is None or isinstance(x, int) or not hasattr(x, "stride"):
+    if x is None or isinstance(x, int):
         return 0
-    if x.shape[0] < tokens:
-        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {x.shape[0]} tokens, {tokens} needed")
-    if x.is_contiguous() and x.numel() == x.shape[0] * features:
-        return features if x.shape[0] > 1 else 0
-    shape, stride, dense = tuple(x.shape), tuple(x.stride()), 1
-    for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
-        if n != 1 and s != dense:
+    try:
+        held = x.shape[0]
+        plain = x.is_contiguous() and x.numel() == held * features
+    except AttributeError:  # no tensor
+        return 0
+    if held < tokens:
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {held} tokens, {tokens} needed")
+    if plain:
+        return features if held > 1 else 0
+    shape, stride, dense = x.shape, x.stride(), 1
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] != 1 and stride[i] != dense:
             raise QxError(_lib.ERR_INVALID_ARG, f"the heads of a token must be dense: strides {stride}")
-        dense *= n
+        dense *= shape[i]
     if dense != features:
-        raise QxError(_lib.ERR_INVALID_ARG, f"a token of shape {shape[1:]} must hold {features} elements")
+        raise QxError(_lib.ERR_INVALID_ARG, f"a token of shape {tuple(shape[1:])} must hold {features} elements")
     if shape[0] > 1 and stride[0] < features:
         raise QxError(_lib.ERR_INVALID_ARG, f"the tokens of a tensor must not overlap: strides {stride}")
     return stride[0] if shape[0] > 1 else 0
@@ -404,9 +415,10 @@ class KvArena:
         return self.key_dtype if self.model == MODEL_QWEN3 else F32
 
     def _tokens(self, counts) -> int:
-        """Tokens that the tensors of a call hold at least; 0 for counts that
-        no sequence has room for, which the call refuses."""
-        return sum(counts) if max(counts, default=0) <= self.capacity else 0
+        """Tokens that the tensors of a call hold at least; 0 for more than its
+        sequences have room for, which the call refuses."""
+        tokens = sum(counts)
+        return tokens if tokens <= self.capacity * len(counts) else 0
 
     def append(self, q, k, v, positions, counts, seq_ids=None, layer_begin: int = 0, layer_count: int | None = None,
                in_dtype: int | None = None, q_rot=None, k_rot=None, rot_dtype: int = BF16, q_norm=None, k_norm=None,
@@ -454,7 +466,8 @@ class KvArena:
         (keep_s, ids), (keep_l, n) = _ints(seq_ids), _ints(lengths)
         a = _lib.PrefillPackedArgs(layer, len(lengths), ids, n, _ptr(q), _ptr(k), _ptr(v),
                                    _room(out, tokens * qn), _token_stride(q, qn, tokens),
-                                   _token_stride(k, kn, tokens), _token_stride(v, kn, tokens), _ptr(q_norm), _ptr(k_norm), dtype, flags)
+                                   _token_stride(k, kn, tokens), _token_stride(v, kn, tokens), _ptr(q_norm),
+                                   _ptr(k_norm), dtype, flags)
         self.ctx.check(self.lib.qxc_prefill_packed(self.ctx.handle, self.handle, C.byref(a)))
 
     def _decode_args(self, q, k, v, out, positions, layer_begin, layer_count, seq_ids, q_dtype, in_dtype,
