@@ -323,72 +323,82 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       for (int i = max(0, loads - NS); i < loads; ++i)
         ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
   } else if (warp == 8) {
-    // ---- MMA issuer ---------------------------------------------------------------
+    // ---- MMA issuer: the whole warp walks, one lane issues -------------------------
     constexpr uint32_t IDESC_S = umma_idesc_16bit(128, kPackedKeys, C::FMT, false, false);
     constexpr uint32_t IDESC_PV = umma_idesc_16bit(128, M::D, C::FMT, false, true);
-    const uint32_t sq = smem_addr(sm + C::OFF_Q), ring = smem_addr(sm + C::OFF_RING);
-    Place<NS> keys, values;
+    const uint32_t one = one_lane(), tm = __reduce_max_sync(0xffffffffu, tbase);
+    // a descriptor counts addresses in units of 16 bytes in its lowest bits
+    const uint64_t dq = umma_desc_sw128(smem_addr(sm + C::OFF_Q), 16, 1024);
+    const uint64_t dk = umma_desc_sw128(smem_addr(sm + C::OFF_RING), 16, 1024);
+    const uint64_t dv = umma_desc_sw128(smem_addr(sm + C::OFF_RING), C::BLK, 1024);
+    Place<NS> keys, values;                                // of the step's tiles, of the next step's keys
     int items[2] = {0, 0}, weights[2] = {0, 0};            // per tile: items, weight tiles taken
-    for (int k = 0, index = blockIdx.x; index >= 0; index = next_item(k++)) {
+    for (int k = 0, index = blockIdx.x; index >= 0; index = __reduce_max_sync(0xffffffffu, next_item(k++))) {
       find_item<M, C::TOKENS>(p, index, &item);
-      if (lane == 0) {
-        const int n = max(item.tiles[0], item.tiles[1]);
-        auto landed = [&](const Place<NS>& s) {
-          ok &= mbar_wait_bounded(&full[s.at], s.parity, p.err);
-          tc_fence_after();
-        };
-        auto scores = [&](int u, int i) {  // S of query tile u and key tile i
-          const uint32_t q = sq + u * C::TILE, ks = ring + keys.at * C::TILE;
+      const int n = max(item.tiles[0], item.tiles[1]);
+      auto landed = [&](const Place<NS>& s) {
+        ok &= mbar_wait_bounded(&full[s.at], s.parity, p.err);
+        __syncwarp();
+        tc_fence_after();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (one) tc_commit(bar);
+        __syncwarp();
+      };
+      auto scores = [&](int u, int i) {  // S of query tile u and key tile i
 #pragma unroll
-          for (int kk = 0; kk < M::D / 16; ++kk)
-            tc_mma_bf16(tbase + C::COL_S + 128 * u, umma_desc_sw128(q + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024),
-                        umma_desc_sw128(ks + (kk >> 2) * C::BLK + (kk & 3) * 32, 16, 1024), IDESC_S, kk > 0);
-          tc_commit(&sfull[u]);
-          if (i + 1 == item.tiles[u]) tc_commit(&qempty[u]);
-        };
-        auto output = [&](int u, int i) {  // O += P V of query tile u and key tile i
-          ok &= mbar_wait_bounded(&pfull[u], (uint32_t)weights[u] & 1u, p.err);
-          ++weights[u];
-          tc_fence_after();
-          const uint32_t v = ring + values.at * C::TILE;
+        for (int kk = 0; kk < M::D / 16; ++kk) {
+          const uint32_t at = ((kk >> 2) * C::BLK + (kk & 3) * 32) >> 4;
+          tc_mma_one(one, tm + C::COL_S + 128 * u, dq + (uint32_t)(u * (C::TILE >> 4)) + at,
+                     dk + (uint32_t)(keys.at * (C::TILE >> 4)) + at, IDESC_S, kk > 0);
+        }
+        commit(&sfull[u]);
+        if (i + 1 == item.tiles[u]) commit(&qempty[u]);
+      };
+      auto output = [&](int u, int i) {  // O += P V of query tile u and key tile i
+        ok &= mbar_wait_bounded(&pfull[u], (uint32_t)weights[u] & 1u, p.err);
+        ++weights[u];
+        __syncwarp();
+        tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < kPackedKeys / 16; ++kk)
-            tc_mma_ts_bf16(tbase + C::COL_O + M::D * u, tbase + C::COL_S + 128 * u + 8 * kk,
-                           umma_desc_sw128(v + kk * 2048, C::BLK, 1024), IDESC_PV, (i > 0 ? 1u : 0u) | (kk > 0 ? 1u : 0u));
-        };
-        landed(keys);
-        for (int u = 0; u < 2; ++u)
-          if (item.tiles[u]) {
-            ok &= mbar_wait_bounded(&qfull[u], (uint32_t)items[u] & 1u, p.err);
-            ++items[u];
-            tc_fence_after();
-            scores(u, 0);
-          }
-        tc_commit(&empty[keys.at]);
+        for (int kk = 0; kk < kPackedKeys / 16; ++kk)
+          tc_mma_ts_one(one, tm + C::COL_O + M::D * u, tm + C::COL_S + 128 * u + 8 * kk,
+                        dv + (uint32_t)(values.at * (C::TILE >> 4)) + (uint32_t)(kk * (2048 >> 4)), IDESC_PV,
+                        (i > 0 ? 1u : 0u) | (kk > 0 ? 1u : 0u));
+      };
+      landed(keys);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (item.tiles[u]) {
+          ok &= mbar_wait_bounded(&qfull[u], (uint32_t)items[u] & 1u, p.err);
+          ++items[u];
+          __syncwarp();
+          tc_fence_after();
+          scores(u, 0);
+        }
+      commit(&empty[keys.at]);
+      keys.advance();
+      for (int i = 0; i < n; ++i) {
+        values = keys;  // this step's values, then the next step's keys
+        landed(values);
         keys.advance();
-        for (int i = 0; i < n; ++i) {
-          values = keys;  // this step's values, then the next step's keys
-          landed(values);
+        if (i + 1 < n) landed(keys);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (i < item.tiles[u]) output(u, i);
+          if (i + 1 < item.tiles[u]) scores(u, i + 1);
+          else if (i + 1 == item.tiles[u]) commit(&odone[u]);
+        }
+        commit(&empty[values.at]);
+        if (i + 1 < n) {
+          commit(&empty[keys.at]);
           keys.advance();
-          if (i + 1 < n) landed(keys);
-          for (int u = 0; u < 2; ++u) {
-            if (i < item.tiles[u]) output(u, i);
-            if (i + 1 < item.tiles[u]) scores(u, i + 1);
-            else if (i + 1 == item.tiles[u]) tc_commit(&odone[u]);
-          }
-          tc_commit(&empty[values.at]);
-          if (i + 1 < n) {
-            tc_commit(&empty[keys.at]);
-            keys.advance();
-          }
         }
       }
-      __syncwarp();
     }
     // TMEM is released only after every product completed
-    if (lane == 0)
-      for (int u = 0; u < 2; ++u)
-        if (items[u]) ok &= mbar_wait_bounded(&odone[u], (uint32_t)(items[u] - 1) & 1u, p.err);
+    for (int u = 0; u < 2; ++u)
+      if (items[u]) ok &= mbar_wait_bounded(&odone[u], (uint32_t)(items[u] - 1) & 1u, p.err);
   } else if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
     // ---- softmax of tile u: thread owns row r (token r / G of the tile, head r % G)
