@@ -68,8 +68,8 @@ struct Packed {
   static constexpr int OFF_RING = 2 * TILE;
   static constexpr int OFF_BAR = OFF_RING + STAGES * TILE;
   // ring full/empty, per tile: queries there, queries done with, scores there,
-  // weights there, output done; answers there/read
-  static constexpr int NBAR = 2 * STAGES + 10 + 4;
+  // weights there (by halves), output done; answers there/read
+  static constexpr int NBAR = 2 * STAGES + 12 + 4;
   static constexpr int OFF_ITEM = OFF_BAR + (8 * NBAR + 15) / 16 * 16;  // two answers of 16 bytes
   static constexpr int SMEM = OFF_ITEM + 32 + 16 + 1024;       // + TMEM slot, + slack to align the base
   static constexpr uint32_t COL_S = 0, COL_O = 256;            // tile u: scores at 128 u, output at 256 + D u
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
   uint64_t* qfull = empty + NS;    // [tile] queries landed
   uint64_t* qempty = qfull + 2;    // [tile] the item's last scores completed
   uint64_t* sfull = qempty + 2;    // [tile] scores in TMEM (and everything issued before them done)
-  uint64_t* pfull = sfull + 2;     // [tile] weights in TMEM
-  uint64_t* odone = pfull + 2;     // [tile] output in TMEM
+  uint64_t* pfull = sfull + 2;     // [tile][half] weights of 64 keys in TMEM
+  uint64_t* odone = pfull + 4;     // [tile] output in TMEM
   uint64_t* ifull = odone + 2;     // [2] the answer to a request for an item landed
   uint64_t* iempty = ifull + 2;    // [2] all warps have read it
   unsigned char* answers = sm + C::OFF_ITEM;
@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       mbar_init(&qfull[u], 1);
       mbar_init(&qempty[u], 1);
       mbar_init(&sfull[u], 1);
-      mbar_init(&pfull[u], 4);
+      mbar_init(&pfull[2 * u], 4);
+      mbar_init(&pfull[2 * u + 1], 4);
       mbar_init(&odone[u], 1);
       mbar_init(&ifull[u], 1);
       mbar_init(&iempty[u], 10);
@@ -356,15 +357,18 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
         if (i + 1 == item.tiles[u]) commit(&qempty[u]);
       };
       auto output = [&](int u, int i) {  // O += P V of query tile u and key tile i
-        ok &= mbar_wait_bounded(&pfull[u], (uint32_t)weights[u] & 1u, p.err);
-        ++weights[u];
-        __syncwarp();
-        tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < kPackedKeys / 16; ++kk)
+        for (int kk = 0; kk < kPackedKeys / 16; ++kk) {
+          if (kk % 4 == 0) {
+            ok &= mbar_wait_bounded(&pfull[2 * u + kk / 4], (uint32_t)weights[u] & 1u, p.err);
+            __syncwarp();
+            tc_fence_after();
+          }
           tc_mma_ts_one(one, tm + C::COL_O + M::D * u, tm + C::COL_S + 128 * u + 8 * kk,
                         dv + (uint32_t)(values.at * (C::TILE >> 4)) + (uint32_t)(kk * (2048 >> 4)), IDESC_PV,
                         (i > 0 ? 1u : 0u) | (kk > 0 ? 1u : 0u));
+        }
+        ++weights[u];
       };
       landed(keys);
 #pragma unroll
@@ -419,7 +423,8 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
         tc_fence_after();
         float s[128];
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld32_sync(ts + c, s + c);
+        for (int c = 0; c < 128; c += 32) tmem_ld32(ts + c, s + c);
+        tmem_wait_ld<128>(s);
         if (i == tiles - 1 || (i + 1) * kPackedKeys > item.q0 + u * C::TOKENS) {  // some key is later than some row
           const int limit = pos - i * kPackedKeys;
 #pragma unroll
@@ -465,11 +470,13 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
             sum[j & 1] = __fadd2_rn(sum[j & 1], e);
           }
           tmem_st16u(ts + 16 * q, w);
+          if (q & 1) {  // the products of the first 64 keys start while the others' weights are made
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[2 * u + q / 2]);
+          }
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[u]);
       }
       // ---- output -------------------------------------------------------------------
       ok &= mbar_wait_bounded(&odone[u], (uint32_t)written & 1u, p.err);
@@ -479,21 +486,23 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), inv = 1.0f / all;
       const bool real = pos < item.length;
       const int token = item.token + pos, qh = item.head * M::G + r % M::G;
-      bool good = true;
+      float2 off = make_float2(0.0f, 0.0f);  // NaN once an output is not finite
       // four lanes exchange their rows' 16-byte pieces, so that a store writes 64
       // bytes of 8 rows and not 16 of 32: lane t of the four ends with piece t of each
       const int r0 = r & ~3, pos0 = item.q0 + u * C::TOKENS + r0 / M::G;
       T* out = static_cast<T*>(p.out) + ((long long)(item.token + pos0) * M::HQ + item.head * M::G + r0 % M::G) * M::D +
                8 * (lane & 3);
+      float o[M::D];
+#pragma unroll
+      for (int c = 0; c < M::D; c += 32) tmem_ld32(to + c, o + c);
+      tmem_wait_ld<M::D>(o);
 #pragma unroll
       for (int c = 0; c < M::D; c += 32) {
-        float o[32];
-        tmem_ld32_sync(to + c, o);
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 y = make_float2(o[2 * e] * inv, o[2 * e + 1] * inv);
-          good &= isfinite(y.x) && isfinite(y.y);
+          const float2 y = __fmul2_rn(make_float2(o[c + 2 * e], o[c + 2 * e + 1]), make_float2(inv, inv));
+          off = __ffma2_rn(y, make_float2(0.0f, 0.0f), off);
           w[e] = pack_pair<T>(y);
         }
 #pragma unroll
@@ -514,6 +523,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
             *reinterpret_cast<uint4*>(out + (j / M::G * M::HQ + j % M::G) * M::D + c) =
                 make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       }
+      const bool good = off.x + off.y == 0.0f;
       __syncwarp();  // a row that is recomputed is written after this
       tc_fence_before();  // O was read: the next item's first product may write it once its weights are there
       unsigned redo = __ballot_sync(0xffffffffu, real && ok && !good && isfinite(m) && isfinite(all));
