@@ -503,7 +503,9 @@ qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* args);
  * an input. What a row that attends a NaN or an infinity holds is unspecified
  * in every dim that it can reach (all of them from a query or a key, its own
  * from a value); a row that is not finite is reported by qxc_sync
- * (QXC_ERR_NONFINITE). Rows that do not attend it are unaffected. Device
+ * (QXC_ERR_NONFINITE). Rows that do not attend it are unaffected. The weights
+ * are summed before they are divided by their own sum, the largest up to 2^8:
+ * bf16 values beyond 2^120 / tokens can pass f32, and are then reported. Device
  * pointers, asynchronous. */
 typedef struct qxc_packed_args {
   int32_t model;

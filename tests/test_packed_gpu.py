@@ -168,6 +168,23 @@ def check_dim(model, q, k, v, out, end, dim, dtype):
 
 
 @pytest.mark.parametrize("model", MODELS)
+def test_the_largest_values_of_later_tokens_do_not_leak(gpu_ctx, model):
+    """bf16 holds 3e38: a weight of a later token has to be zero, not merely small.
+    (The rows that do attend them pass f32 in their sums of weights, which are up
+    to 2^8 before they are divided by their own sum, and are reported.)"""
+    rng = np.random.default_rng(28)
+    q, k, v = inputs(rng, model, 250, BF16)
+    clean = attend(gpu_ctx, model, q, k, v, [250], BF16)
+    v[170:] = 3.0e38
+    out = torch.zeros_like(q)
+    gpu_ctx.attend_packed(model, q, k, v, out, [250])
+    with pytest.raises(QxError) as e:
+        gpu_ctx.sync()
+    assert e.value.status == _lib.ERR_NONFINITE
+    assert torch.equal(out[:170], clean[:170])
+
+
+@pytest.mark.parametrize("model", MODELS)
 def test_values_that_are_all_bad(gpu_ctx, model):
     rng = np.random.default_rng(21)
     q, k, v = inputs(rng, model, 3000, BF16)
