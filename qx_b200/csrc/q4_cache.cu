@@ -232,13 +232,20 @@ __global__ void __launch_bounds__(kThreads) qx_q4_read_kernel(const __grid_const
     value_scale = __half2float(*reinterpret_cast<const __half*>(p.arena.v + row + R::scale(head, c >> 2)));
   }
   // a nibble in the low bits of 2^23 is 2^23 plus it
+  auto put2 = [](float* to, uint32_t a, uint32_t b, float base, float scale) {
+    const float2 c = __fadd2_rn(make_float2(__uint_as_float((a & 15u) | 0x4b000000u), __uint_as_float((b & 15u) | 0x4b000000u)),
+                                make_float2(-base, -base));
+    const float2 y = __fmul2_rn(c, make_float2(scale, scale));
+    to[0] = y.x;
+    to[1] = y.y;
+  };
   float x[8];
   if (p.key_out) {
     const uint32_t turned = key ^ 0x88888888u;  // c + 8
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = (__uint_as_float((turned >> (8 * i + 4) & 15u) | 0x4b000000u) - 8388616.0f) * key_scale;
-      x[4 + i] = (__uint_as_float((turned >> (8 * i) & 15u) | 0x4b000000u) - 8388616.0f) * key_scale;
+    for (int i = 0; i < 4; i += 2) {
+      put2(x + i, turned >> (8 * i + 4), turned >> (8 * i + 12), 8388616.0f, key_scale);
+      put2(x + 4 + i, turned >> (8 * i), turned >> (8 * i + 8), 8388616.0f, key_scale);
     }
     store8(p.key_out, out, p.out_dtype, p.vec, x);
   }
@@ -246,9 +253,10 @@ __global__ void __launch_bounds__(kThreads) qx_q4_read_kernel(const __grid_const
     const int base = (threadIdx.x & 31) & ~(R::LPH - 1), j = c >> 2;
     const int shift = 4 * (c & 3) + 16 * (j & 1);  // half g NG + j: NG is even
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const uint32_t from = __shfl_sync(0xffffffffu, value, base + ((g * R::NG + j) >> 1));
-      x[g] = (__uint_as_float((from >> shift & 15u) | 0x4b000000u) - 8388615.0f) * value_scale;
+    for (int g = 0; g < 8; g += 2) {
+      const uint32_t a = __shfl_sync(0xffffffffu, value, base + ((g * R::NG + j) >> 1));
+      const uint32_t b = __shfl_sync(0xffffffffu, value, base + (((g + 1) * R::NG + j) >> 1));
+      put2(x + g, a >> shift, b >> shift, 8388615.0f, value_scale);
     }
     store8(p.value_out, out, p.out_dtype, p.vec, x);
   }
