@@ -11,7 +11,7 @@
 //               as the last scores of the tile before are done, and its key and
 //               value tiles of 128 tokens through one ring in the order of their
 //               use, then asks for the next item
-//   warp 8      MMA issuer, one thread: for each tile in turn O += P V, then the
+//   warp 8      MMA issuer, one lane: for each tile in turn O += P V, then the
 //               next scores S = Q K^T, so one tile's products run while the
 //               other's softmax does
 //   warps 0-3, 4-7  the softmax of the first, the second tile: a thread owns a
@@ -25,20 +25,26 @@
 // item's first P V starts O afresh; its weights are written after the tile's
 // threads have read the last item's O.
 //
-// Measured: a Qwen3 prompt of 16384 tokens 1.67 to 1.79 ms (1230 to 1320 TFLOP/s
-// of the causal half; a library product of bf16 matrices reaches 1646 for a moment,
-// 1373 for seconds), 11 ragged Qwen3 prompts of together 12345 tokens 186 to 193 us
-// (860 to 890), one of 2048 43 us (795), 10 ragged Granite prompts of 30000 tokens
-// 525 us (640), 7 of 777 10.5 us. A step, both tiles against a key tile, takes about
-// 3400 cycles where the tensor pipe needs 2048 and the special-function unit's 32768
-// exponentials 2048: each is busy 60% of the time, since a tile's scores, softmax
-// and products follow one another and two tiles overlap only in part. Of what was
-// tried: registers split 216 to 72 between the softmax and the issuing warps (one
-// size for all spills) 1720 -> 1670 us and 223 -> 208; every fourth exponential as a
-// polynomial on the FMA pipe 1666 -> 1710; further items by cancelling 212 -> 204,
-// asked for at an item's start and not at its end 43 -> 53 us (2048 tokens: who is
-// last takes two); outputs in 64-byte pieces 204 -> 193; weights handed over by
-// halves no change. Granite's 64 dims halve the products, not the softmax.
+// Measured: a Qwen3 prompt of 16384 tokens 1.56 to 1.60 ms (1375 to 1410 TFLOP/s of
+// the causal half; a library product of bf16 matrices reaches 1646 for a moment, 1373
+// for seconds), 11 ragged Qwen3 prompts of together 12345 tokens 160 to 165 us (1000 to
+// 1030), one of 2048 33 to 38 us, 3 Granite prompts of 8200 tokens 171 us (800), 7 of
+// 777 10 us. A step, both tiles against a key tile, takes 3100 cycles of which the
+// tensor pipe needs 2048: a tile's scores (512, and about 270 to hand them over), its
+// row maxima (400), its exponentials (1400) and the products of their last half (256)
+// follow one another, and the other tile's do not fill all of the gaps. An item adds
+// about 3000 cycles for its outputs. Steps:
+//   products issued by a converged warp, operands in uniform registers: a single
+//   diverged lane took 105 cycles an instruction of 64     190 -> 172 us (11 prompts)
+//   weights handed over by halves, loads in flight together     172 -> 165
+//   outputs in 64-byte pieces by an exchange among four lanes   204 -> 193
+//   further items by cancelling CTAs                            212 -> 204
+//   (asked for at an item's start, not its end: 2048 tokens 43 -> 53, who is last
+//   takes two)
+//   registers split 216 to 72 between the softmax and the issuing warps, where one
+//   size for all spills                                         223 -> 208
+//   exponentials against the reference so far, made again where it moves: spills,
+//   twice the time; a persistent grid with dealt items: 224 -> 244
 //
 // A key tile may hold tokens its rows do not attend: later ones of the prompt,
 // the next prompt's. Their scores are replaced by -inf, so their weights are

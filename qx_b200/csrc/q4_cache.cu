@@ -6,8 +6,8 @@
 // once. qx_q4_read_kernel expands rows into plain tensors.
 //
 // Measured: 32768 bf16 Qwen3 tokens (norm, rotation, 4-bit rows; 640 MB) written in
-// 132 us, 4.85 TB/s, 74% of a copy's rate; read back as bf16 in 19 us, 4.5 TB/s.
-// 9001 bf16 Granite tokens: 17.1 and 6.3 us; one token: 1.8 and 1.5 us. The writes
+// 131 us, 4.9 TB/s, 75% of a copy's rate; read back as bf16 in 18 us, 4.8 TB/s.
+// 9001 bf16 Granite tokens: 17.3 and 6.1 us; one token: 1.6 and 1.5 us. The writes
 // are bound by instructions and latency together: issue slots are busy 68% of the
 // time, DRAM 54%, with 32 warps an SM of which most wait for their loads. What
 // brought them there from 312 us: inputs of known types, all loaded before the
