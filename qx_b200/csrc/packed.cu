@@ -28,7 +28,7 @@
 // Measured: a Qwen3 prompt of 16384 tokens 1.56 to 1.60 ms (1375 to 1410 TFLOP/s of
 // the causal half; a library product of bf16 matrices reaches 1646 for a moment, 1373
 // for seconds), 11 ragged Qwen3 prompts of together 12345 tokens 160 to 165 us (1000 to
-// 1030), one of 2048 33 to 38 us, 3 Granite prompts of 8200 tokens 171 us (800), 7 of
+// 1030), one of 2048 33 to 39 us, 3 Granite prompts of 8200 tokens 175 us (785), 7 of
 // 777 10 us. A step, both tiles against a key tile, takes 3100 cycles of which the
 // tensor pipe needs 2048: a tile's scores (512, and about 270 to hand them over), its
 // row maxima (400), its exponentials (1400) and the products of their last half (256)
@@ -51,6 +51,10 @@
 // zero, but a zero weight times an infinite or NaN value is NaN: of a row whose
 // sums are finite and whose output is not, the dims that this can have touched are
 // computed again over what it attends only (careful_row).
+//
+// A wait that runs out (1 s) ends its warp's walk, and the others' with it: they
+// wait once more at most for what no longer comes, then for their own copies and
+// products, and leave.
 #include <type_traits>
 
 #include "q4.cuh"
@@ -299,11 +303,11 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
   pdl_launch_dependents();
   bool ok = true;
   Item item;
-  // item k + 1 is the answer of slot k % 2: its block index, -1 past the last
+  // item k + 1 is the answer of slot k % 2: its block index, -1 past the last, or
+  // once a wait of this warp has run out
   auto next_item = [&](int k) {
-    const bool there = mbar_wait_bounded(&ifull[k & 1], (uint32_t)(k >> 1) & 1u, p.err);
-    ok &= there;
-    const int index = there ? answered_cta(answers + 16 * (k & 1)) : -1;
+    if (__all_sync(0xffffffffu, ok)) ok &= mbar_wait_bounded(&ifull[k & 1], (uint32_t)(k >> 1) & 1u, p.err);
+    const int index = __all_sync(0xffffffffu, ok) ? answered_cta(answers + 16 * (k & 1)) : -1;
     fence_proxy_async_shared();  // the read above comes before the next answer
     __syncwarp();
     if (lane == 0) mbar_arrive(&iempty[k & 1]);
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
                         item.token + item.q0 + u * C::TOKENS, &qfull[u]);
         };
         queries(0);
-        for (int i = 0; i < n; ++i, ++loads, place.advance()) {
+        for (int i = 0; i < n && ok; ++i, ++loads, place.advance()) {
           const int s = place.at;
           if (loads >= NS) ok &= mbar_wait_bounded(&empty[s], place.parity ^ 1u, p.err);
           mbar_arrive_expect_tx(&full[s], C::TILE);
@@ -347,15 +351,20 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
         }
         // asked for now, not before: who is done first takes the next item
         if (k >= 2) ok &= mbar_wait_bounded(&iempty[k & 1], (uint32_t)((k >> 1) - 1) & 1u, p.err);
-        mbar_arrive_expect_tx(&ifull[k & 1], 16);
-        ask_for_cta(answers + 16 * (k & 1), &ifull[k & 1]);
+        if (ok) {
+          mbar_arrive_expect_tx(&ifull[k & 1], 16);
+          ask_for_cta(answers + 16 * (k & 1), &ifull[k & 1]);
+        }
       }
       __syncwarp();
     }
     // no copy may still be landing when the CTA exits
-    if (lane == 0)
+    if (lane == 0) {
       for (int i = max(0, loads - NS); i < loads; ++i)
         ok &= mbar_wait_bounded(&full[i % NS], (uint32_t)(i / NS) & 1u, p.err);
+      for (int u = 0; u < 2; ++u)
+        if (used[u]) ok &= mbar_wait_bounded(&qfull[u], (uint32_t)(used[u] - 1) & 1u, p.err);
+    }
   } else if (warp == 8) {
     // ---- MMA issuer: the whole warp walks, one lane issues -------------------------
     constexpr uint32_t IDESC_S = umma_idesc_16bit(128, kPackedKeys, C::FMT, false, false);
@@ -431,6 +440,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
           commit(&empty[keys.at]);
           keys.advance();
         }
+        if (!__all_sync(0xffffffffu, ok)) break;
       }
     }
     // TMEM is released only after every product completed
@@ -512,6 +522,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
             if (lane == 0) mbar_arrive(&pfull[2 * u + q / 2]);
           }
         }
+        if (!__all_sync(0xffffffffu, ok)) break;  // here, while the products run
       }
       // ---- output -------------------------------------------------------------------
       ok &= mbar_wait_bounded(&odone[u], (uint32_t)written & 1u, p.err);
