@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     const int kk = at - start + k, s = kk % kStages;
     unsigned char* data = sm + s * kStage;
     const int valid = min(kQ4Tile, attend - (tile + k) * kQ4Tile);
-    ok &= mbar_wait_bounded(&full[s], (uint32_t)(kk / kStages) & 1u, p.err);
+    if (ok) ok = mbar_wait_bounded(&full[s], (uint32_t)(kk / kStages) & 1u, p.err);
     __syncwarp();
     const int r0 = C::ROWS * part;
     if (r0 < valid) {
@@ -587,9 +587,11 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
         }
       }
     }
-    // the last warp of the group to finish a tile refills its stage
+    // the last warp of the group to finish a tile refills its stage; a warp whose
+    // wait ran out neither waits nor counts again, so no stage of its group is
+    // refilled from then on
     __syncwarp();
-    if (lane == 0 && count_up(&done[s]) == 3u) {
+    if (lane == 0 && ok && count_up(&done[s]) == 3u) {
       done[s] = 0u;
       Cursor c = cursor[group];
       if (c.at < end) {
@@ -667,6 +669,11 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
     layer = 0;
     if (++seq < p.n_seq) tiles = tiles_of(seq);
   }
+  }
+  if (!ok && lane == 0) {  // what is still on its way to the group's stages lands before the CTA exits
+    const int issued = cursor[group].at;
+    for (int at = max(start + group, issued - kStages); at < min(issued, end); at += 2)
+      mbar_wait_bounded(&full[(at - start) % kStages], (uint32_t)((at - start) / kStages) & 1u, p.err);
   }
   if (!good && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
 }
