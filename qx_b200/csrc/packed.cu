@@ -109,9 +109,9 @@ __device__ __forceinline__ uint32_t pack_pair(float2 x) {
 
 // 2^x, x <= TAU, of a pair on the FMA pipe: x = n + f, n rounded by adding and
 // taking off 1.5 * 2^23, 2^f by a polynomial of degree 3 (fitted for the smallest
-// relative error on [-0.5, 0.5], 7.5e-5: a third of half a step of fp16), 2^n
-// through the exponent field. x below -126, -inf among them, gives 0: the value at
-// -126 is taken off, which no larger result notices.
+// relative error on [-0.5, 0.5], 7.5e-5; a weight's rounding to fp16 is up to
+// 4.9e-4), 2^n through the exponent field. x below -126, -inf among them, gives 0:
+// the value at -126 is taken off, which no larger result notices.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   constexpr float C0 = 0.9999281167984009f, C1 = 0.6932609677314758f, C2 = 0.24261054396629333f, C3 = 0.05517132207751274f;
   constexpr float ROUND = 12582912.0f;
