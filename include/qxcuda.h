@@ -496,7 +496,7 @@ qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* args);
  * scale and head layout of `model`. q and k are already rotated. bf16 or f16
  * in and out, f32 scores, softmax and accumulation (the weights of one key
  * tile are rounded to the input type for their product with the values).
- * lengths may be 0; at most 2^24 tokens. Each tensor is [tokens][heads *
+ * lengths may be 0; at most 2^18 tokens a prompt and 2^24 together. Each tensor is [tokens][heads *
  * head_dim], 16-byte aligned, with token strides in elements that are
  * multiples of 8 (0 = dense): q, k and v may be parts of one joint projection.
  * Rows of `out` past the last prompt are not written; `out` must not overlap

@@ -50,7 +50,7 @@
 // the next prompt's. Their scores are replaced by -inf, so their weights are
 // zero, but a zero weight times an infinite or NaN value is NaN: of a row whose
 // sums are finite and whose output is not, the dims that this can have touched are
-// computed again over what it attends only (careful_row).
+// computed again over what it attends only (careful_rows).
 //
 // A wait that runs out (1 s) ends its warp's walk, and the others' with it: they
 // wait once more at most for what no longer comes, then for their own copies and
@@ -128,61 +128,99 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
   return __fadd2_rn(y, make_float2(-least, -least));
 }
 
-// One output row of a non-finite tile again, by a whole warp: the dims in which a
-// token of [token + 1, end), which the row does not attend but its key tiles hold,
-// is not finite, over tokens first .. token only, against the row's own reference
-// m and sum. A dim ends as soon as it is not finite by what the row does attend,
-// so that only the rows of one query tile before a dim's first such value walk all
-// their tokens. False when the row is not finite.
+// Up to eight neighbouring output rows of a tile (those of `rows`, a bit each) again,
+// by a whole warp: the dims in which a token that a row does not attend, but its key
+// tiles hold (up to `end`), is not finite, over the tokens it does attend only,
+// against the row's own reference m and sum, which lane `from` + a holds for row a.
+// A dim ends as soon as it is not finite by what a row does attend, so that only the
+// rows of one query tile before a dim's first such value walk all their tokens. The
+// warps that wait for this one do so for 1 s at most: hence eight rows together, which
+// share their loads, and a limit on a prompt's length (140001 tokens: 0.3 s). False
+// when a row is not finite.
 template <class M, typename T>
-__device__ __noinline__ bool careful_row(const PackedParams& p, int first, int token, int end, int qh, float m, float sum) {
-  constexpr int N = M::D / 32;
+__device__ __noinline__ bool careful_rows(const PackedParams& p, int first, int token, int end, int h, unsigned rows,
+                                          int from, float m, float sum) {
+  constexpr int N = M::D / 32, TG = 8 / M::G, U = 32 / N;
   using P = Packed<M, T>;
-  const int lane = threadIdx.x & 31, h = qh / M::G;
-  const T* q = static_cast<const T*>(p.q) + token * p.q_stride + qh * M::D;
+  const int lane = threadIdx.x & 31, last = token + (31 - __clz(rows)) / M::G;
   auto value = [&](int t, int e) {
     return Elem<T>::to_f32(static_cast<const T*>(p.v)[t * p.v_stride + h * M::D + 32 * e + lane]);
   };
-  float o[N];
-  bool dirty[N];
+  float o[8][N];
+  bool dirty[TG][N];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    o[e] = 0.0f;
-    dirty[e] = false;
+#pragma unroll
+    for (int j = 0; j < TG; ++j) dirty[j][e] = false;
+#pragma unroll
+    for (int a = 0; a < 8; ++a) o[a][e] = 0.0f;
   }
   for (int t = token + 1; t < end; ++t)
 #pragma unroll
-    for (int e = 0; e < N; ++e) dirty[e] |= !isfinite(value(t, e));
-  for (int t0 = first; t0 <= token; t0 += 32) {
+    for (int e = 0; e < N; ++e) {
+      const bool bad = !isfinite(value(t, e));
+#pragma unroll
+      for (int j = 0; j < TG; ++j) dirty[j][e] |= bad && t > token + j;
+    }
+  for (int t0 = first; t0 <= last; t0 += 32) {
     bool open = false;
 #pragma unroll
-    for (int e = 0; e < N; ++e) open |= dirty[e] && isfinite(o[e]);
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+      for (int a = 0; a < 8; ++a) open |= dirty[a / M::G][e] && (rows >> a & 1u) && isfinite(o[a][e]);
     if (!__any_sync(0xffffffffu, open)) break;
-    float weight = 0.0f;
-    if (t0 + lane <= token) {
+    float weight[8];
+#pragma unroll
+    for (int a = 0; a < 8; ++a) weight[a] = 0.0f;
+    if (t0 + lane <= last) {
       const T* k = static_cast<const T*>(p.k) + (t0 + lane) * p.k_stride + h * M::D;
-      float dot = 0.0f;
+#pragma unroll 4
       for (int d = 0; d < M::D; d += 8) {
-        float x[8], y[8];
-        Vec16<T>::load(q + d, x);
+        float y[8];
         Vec16<T>::load(k + d, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
-      }
-      weight = fast_exp2(fmaf(dot, P::UNIT, -m));
-    }
-    for (int u = 0; u < 32 && t0 + u <= token; ++u) {
-      const float w = __shfl_sync(0xffffffffu, weight, u);
+        for (int a = 0; a < 8; ++a) {
+          if (TG > 1 && !(rows >> a & 1u)) continue;  // a token past the last
+          float x[8];
+          Vec16<T>::load(static_cast<const T*>(p.q) + (token + a / M::G) * p.q_stride + (h * M::G + a % M::G) * M::D + d, x);
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = fmaf(w, value(t0 + u, e), o[e]);
+          for (int e = 0; e < 8; ++e) weight[a] = fmaf(x[e], y[e], weight[a]);
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+      const float ref = __shfl_sync(0xffffffffu, m, from + a);
+      weight[a] = t0 + lane <= token + a / M::G ? fast_exp2(fmaf(weight[a], P::UNIT, -ref)) : 0.0f;
+    }
+    for (int u0 = 0; u0 < 32; u0 += U) {  // 32 loads in flight
+      float x[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[u][e] = t0 + u0 + u <= last ? value(t0 + u0 + u, e) : 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+          const float w = __shfl_sync(0xffffffffu, weight[a], u0 + u);
+          if (TG > 1 && t0 + u0 + u > token + a / M::G) continue;  // a zero weight would not do
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[a][e] = fmaf(w, x[u][e], o[a][e]);
+        }
     }
   }
   bool good = true;
-  T* out = static_cast<T*>(p.out) + ((long long)token * M::HQ + qh) * M::D;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    if (dirty[e]) out[32 * e + lane] = Elem<T>::from_f32(o[e] / sum);
-    good &= isfinite(Elem<T>::to_f32(out[32 * e + lane]));
+  for (int a = 0; a < 8; ++a) {
+    const float all = __shfl_sync(0xffffffffu, sum, from + a);
+    if (!(rows >> a & 1u)) continue;
+    T* out = static_cast<T*>(p.out) + ((long long)(token + a / M::G) * M::HQ + h * M::G + a % M::G) * M::D;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (dirty[a / M::G][e]) out[32 * e + lane] = Elem<T>::from_f32(o[a][e] / all);
+      good &= isfinite(Elem<T>::to_f32(out[32 * e + lane]));
+    }
   }
   return __all_sync(0xffffffffu, good);
 }
@@ -531,7 +569,7 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       tc_fence_after();
       const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), inv = 1.0f / all;
       const bool real = pos < item.length;
-      const int token = item.token + pos, qh = item.head * M::G + r % M::G;
+      const int token = item.token + pos;
       float2 off = make_float2(0.0f, 0.0f);  // NaN once an output is not finite
       // four lanes exchange their rows' 16-byte pieces, so that a store writes 64
       // bytes of 8 rows and not 16 of 32: lane t of the four ends with piece t of each
@@ -574,12 +612,12 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
       tc_fence_before();  // O was read: the next item's first product may write it once its weights are there
       unsigned redo = __ballot_sync(0xffffffffu, real && ok && !good && isfinite(m) && isfinite(all));
       bool bad = real && !good && !(isfinite(m) && isfinite(all));
-      while (redo) {
-        const int src = __ffs(redo) - 1;
-        redo &= redo - 1;
-        bad |= !careful_row<M, T>(p, item.token, __shfl_sync(0xffffffffu, token, src),
-                                  min(item.token + tiles * kPackedKeys, p.tokens), __shfl_sync(0xffffffffu, qh, src),
-                                  __shfl_sync(0xffffffffu, m, src), __shfl_sync(0xffffffffu, all, src));
+      while (redo) {  // eight neighbouring lanes' rows together
+        const int from = (__ffs(redo) - 1) & ~7;
+        const unsigned rows = redo >> from & 255u;
+        redo &= ~(255u << from);
+        bad |= !careful_rows<M, T>(p, item.token, __shfl_sync(0xffffffffu, token, from),
+                                   min(item.token + tiles * kPackedKeys, p.tokens), item.head, rows, from, m, all);
       }
       if (bad && ok) flag_error(p.err, QX_ERR_BIT_NONFINITE);
     }

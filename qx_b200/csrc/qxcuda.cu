@@ -1242,12 +1242,14 @@ qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
   });
 }
 
-// Lengths of packed prompts: every one >= 0, together within 32-bit indices.
+// Lengths of packed prompts: every one in 0..2^18 (see careful_rows in packed.cu),
+// together within 32-bit indices.
 qxc_status check_lengths(qxc_ctx* ctx, int seq_count, const int32_t* lengths, long long* total) {
   if (seq_count < 1 || !lengths) return fail(ctx, QXC_ERR_INVALID_ARG, "seq_count >= 1 and lengths required");
   *total = 0;
   for (int i = 0; i < seq_count; ++i) {
-    if (lengths[i] < 0) return fail(ctx, QXC_ERR_INVALID_ARG, "prompt %d has length %d", i, lengths[i]);
+    if (lengths[i] < 0 || lengths[i] > (1 << 18))
+      return fail(ctx, QXC_ERR_INVALID_ARG, "prompt %d has length %d, outside 0..2^18", i, lengths[i]);
     *total += lengths[i];
   }
   if (*total > (1 << 24)) return fail(ctx, QXC_ERR_INVALID_ARG, "%lld packed tokens; at most 2^24", *total);

@@ -185,6 +185,28 @@ def test_the_largest_values_of_later_tokens_do_not_leak(gpu_ctx, model):
 
 
 @pytest.mark.parametrize("model", MODELS)
+def test_a_bad_value_at_the_end_of_a_very_long_prompt(gpu_ctx, model):
+    """The rows of its tile are computed again over all their tokens, within the
+    time that the rest of the kernel waits for them."""
+    n = 140001
+    hq, hkv, d = model_shape(model)
+    gen = torch.Generator(device="cuda").manual_seed(29)
+    q, k, v = (torch.randn(n, h, d, device="cuda", generator=gen).bfloat16() for h in (hq, hkv, hkv))
+    clean = attend(gpu_ctx, model, q, k, v, [n], BF16)
+    v[n - 1] = float("nan")
+    out = torch.zeros_like(q)
+    gpu_ctx.attend_packed(model, q, k, v, out, [n])
+    with pytest.raises(QxError) as e:
+        gpu_ctx.sync()
+    assert e.value.status == _lib.ERR_NONFINITE
+    assert torch.isnan(out[n - 1]).all() and torch.isfinite(out[:n - 1]).all()
+    # of a mean of n values of size 1: half a step, weights rounded or not
+    tol = 2.0 ** -8 * clean[n - 200:n - 1].double().abs() + (2.0 ** -8 + n * 2.0 ** -23) * 1.0
+    assert ((out[n - 200:n - 1].double() - clean[n - 200:n - 1].double()).abs() <= tol).all()
+    assert torch.equal(out[:n - 200], clean[:n - 200])
+
+
+@pytest.mark.parametrize("model", MODELS)
 def test_values_that_are_all_bad(gpu_ctx, model):
     rng = np.random.default_rng(21)
     q, k, v = inputs(rng, model, 3000, BF16)
@@ -372,6 +394,8 @@ def test_refusals(gpu_ctx):
     refused(bad, lambda: go(q, k, k, q, []))
     refused(bad, lambda: go(q, k, k, q, [3, -1]))
     refused(bad, lambda: go(q, k, k, q, [2 ** 24, 1]))
+    refused(bad, lambda: go(q.data_ptr(), k.data_ptr(), k.data_ptr(), q.data_ptr(), [2 ** 18 + 1]))
+    refused(bad, lambda: go(q.data_ptr(), k.data_ptr(), k.data_ptr(), q.data_ptr(), [2 ** 18] * 64 + [1]))
     refused(bad, lambda: go(q, k, None, q, [3]))
     refused(bad, lambda: go(q, q, k, q, [3]))
     refused(bad, lambda: go(q.transpose(0, 1), k, k, q, [3]))
