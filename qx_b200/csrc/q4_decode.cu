@@ -696,8 +696,11 @@ __global__ void __launch_bounds__(256) qx_q4_merge_kernel(const __grid_constant_
   const int place = p.padded ? (tiles + p.per_cta - 1) / p.per_cta * p.per_cta : tiles;
   const int first = p.seqs[i].first + layer * place;
   const int b0 = first / p.per_cta, parts = (first + tiles - 1) / p.per_cta - b0 + 1;
-  if (parts == 1) return;
+  // Before any CTA leaves: cells whose borders are CTA borders are all whole, and a grid
+  // that did not wait would be complete while the attention still runs, with nothing to
+  // keep the stream's next kernel from its workspace and rows.
   pdl_wait();
+  if (parts == 1) return;
   const int share = tid / LANES, e = slice * E + 4 * (tid % LANES), qh = e / M::D;
   // the first part lies in slot 1 of its CTA unless it is the CTA's first cell
   auto slot = [&](int s) { return 2ll * (b0 + s) + (s == 0 && first != b0 * p.per_cta ? 1 : 0); };

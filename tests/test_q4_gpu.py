@@ -661,3 +661,57 @@ def test_refusals(gpu_ctx):
     refused(bad, lambda: paged.read_rows(k, k, [0], [1]))
     for a in (arena, plain, paged):
         a.close()
+
+
+# ---- steps that follow one another ---------------------------------------------------
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("seqs,layers,rows", [(1, 24, 64), (112, 2, 64), (128, 3, 128), (148, 6, 64), (213, 2, 100), (5, 4, 700)])
+def test_steps_without_a_synchronisation_between_them(gpu_ctx, model, seqs, layers, rows):
+    """Steps with different inputs, one behind another on the stream, give what each
+    gives alone. In most of these shapes the borders of the cells are borders of CTAs,
+    so the grid that joins parts finds none."""
+    rng = np.random.default_rng([model, seqs, layers, rows])
+    steps, at = 6, [rows - 1] * seqs
+    arena = make_arena(gpu_ctx, model, [rows] * seqs, layers)
+    fill(gpu_ctx, arena, rng, at)
+    ins = [[tensor(rng, (seqs, layers, h, arena.d), BF16) for h in (arena.hq, arena.hkv, arena.hkv)] for _ in range(steps)]
+    outs = [[torch.zeros(seqs, layers, arena.hq, arena.d, device="cuda", dtype=torch.bfloat16) for _ in range(steps)]
+            for _ in range(2)]
+    gpu_ctx.sync()
+    for i, alone in enumerate((False, True)):
+        for _ in range(1 if alone else 4):
+            for (q, k, v), out in zip(ins, outs[i]):
+                arena.decode(q, k, v, out, at, q_dtype=BF16, in_dtype=BF16, out_dtype=BF16, flags=DECODE_NO_ADVANCE)
+                if alone:
+                    gpu_ctx.sync()
+        gpu_ctx.sync()
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    some = sorted({0, seqs // 2, seqs - 1})
+    q, k, v = ([x[some] for x in ins[-1]])
+    check_decode(gpu_ctx, arena, q, k, v, outs[0][-1][some], [rows - 1] * len(some), BF16, ids=some)
+    arena.close()
+
+
+def test_an_append_right_behind_a_step(gpu_ctx):
+    """An append into sequences that were reset right after a decode was enqueued does
+    not reach the rows which that decode still reads."""
+    rng = np.random.default_rng(31)
+    seqs, layers, rows = 112, 2, 64
+    arena = make_arena(gpu_ctx, MODEL_GRANITE, [rows] * seqs, layers)
+    q, k, v = (tensor(rng, (seqs, layers, h, 64), BF16) for h in (16, 8, 8))
+    ak, av = (tensor(rng, (seqs * (rows - 1), layers, 8, 64), BF16) for _ in range(2))
+    other = tensor(rng, (seqs * (rows - 1), layers, 8, 64), BF16, 3.0)
+    outs = []
+    for behind in (True, False):
+        out = torch.zeros(seqs, layers, 16, 64, device="cuda", dtype=torch.bfloat16)
+        for _ in range(8):
+            arena.reset(-1)
+            arena.append(None, ak, av, [0] * seqs, [rows - 1] * seqs, in_dtype=BF16)
+            arena.decode(q, k, v, out, [rows - 1] * seqs, q_dtype=BF16, in_dtype=BF16, out_dtype=BF16)
+            if behind:
+                arena.reset(-1)
+                arena.append(None, other, other, [0] * seqs, [rows - 1] * seqs, in_dtype=BF16)
+            gpu_ctx.sync()
+            outs.append(out.clone())
+    assert all(torch.equal(outs[-1], o) for o in outs)
+    arena.close()
