@@ -82,6 +82,8 @@ def _room(x, elements: int):
         held = x.numel()
     except AttributeError:
         return _ptr(x)
+    if not x.is_contiguous():
+        raise QxError(_lib.ERR_INVALID_ARG, f"an output must be dense: shape {tuple(x.shape)}, strides {x.stride()}")
     if held < elements:
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {held} elements, {elements} needed")
     return x.data_ptr()

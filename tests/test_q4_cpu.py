@@ -7,8 +7,8 @@ import pytest
 import torch
 
 import q4_reference as ref
-from qx_b200 import MODEL_GRANITE, MODEL_QWEN3, KvPrecision, ExecutionPlan, QxError, _lib
-from qx_b200.runtime import _token_stride
+from qx_b200 import MODEL_GRANITE, MODEL_QWEN3, Context, ExecutionPlan, KvArena, KvPrecision, QxError, _lib
+from qx_b200.runtime import _token_stride, model_shape
 
 
 def kv_bytes(desc):
@@ -90,3 +90,56 @@ def test_reference_quantiser_rounds_ties_to_even_and_keeps_the_largest():
     assert scales[0, 0].tolist() == [1.0, 0.0]
     assert codes[0, 0, :5].tolist() == [14, 7, 9, 9, 5]
     assert (codes[0, 0, 32:] == 7).all()
+
+
+class Calls:
+    """A library that notes the calls it gets instead of making them."""
+
+    def __init__(self):
+        self.made = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.made.append(name) or _lib.OK
+
+
+def bare(model=MODEL_GRANITE, device=-1):
+    """A context and a 4-bit arena without a GPU, whose device is the CPU."""
+    ctx, arena = object.__new__(Context), object.__new__(KvArena)
+    ctx.lib = arena.lib = Calls()
+    ctx.handle = arena.handle = None
+    ctx.device, arena.ctx, arena.model = device, ctx, model
+    arena.layers, arena.sequences, arena.capacity = 1, 4, 64
+    arena.key_dtype = arena.value_dtype = _lib.Q4
+    arena.hq, arena.hkv, arena.d = model_shape(model)
+    arena.row_shape = (288,)
+    return ctx, arena
+
+
+def refused(lib, call, status=_lib.ERR_INVALID_ARG, match=None):
+    with pytest.raises(QxError, match=match) as e:
+        call()
+    assert e.value.status == status and not lib.made
+
+
+@pytest.mark.parametrize("model", [MODEL_GRANITE, MODEL_QWEN3])
+def test_outputs_must_be_dense(model):
+    """A part of a joint projection may be an input; written as dense rows it would
+    run over its neighbours."""
+    ctx, arena = bare(model)
+    lib, (hq, hkv, d) = arena.lib, model_shape(model)
+    joint = torch.zeros(10, hq + 2 * hkv, d, dtype=torch.bfloat16)
+    q, k, v = joint[:, :hq], joint[:, hq:hq + hkv], joint[:, hq + hkv:]
+    dense = lambda x: torch.zeros(x.shape, dtype=x.dtype)  # noqa: E731
+    append = lambda **kw: arena.append(q, k, v, [0], [10], in_dtype=_lib.BF16, **{"q_rot": dense(q), **kw})  # noqa: E731
+    prefill = lambda out: arena.prefill_packed(q, k, v, out, [10])  # noqa: E731
+    attend = lambda out: ctx.attend_packed(model, q, k, v, out, [10])  # noqa: E731
+    read = lambda a, b: arena.read_rows(a, b, [0], [10], out_dtype=_lib.BF16)  # noqa: E731
+    wide = torch.zeros(20, hq, d, dtype=torch.bfloat16)
+    for call in (lambda: append(q_rot=q), lambda: append(k_rot=k), lambda: prefill(q), lambda: attend(q),
+                 lambda: attend(wide[::2]), lambda: read(k, dense(v)), lambda: read(None, v)):
+        refused(lib, call, match="dense")
+    append(k_rot=dense(k))
+    prefill(dense(q))
+    attend(wide[10:])
+    read(dense(k), dense(v))
+    assert lib.made == ["qxc_kv_append", "qxc_prefill_packed", "qxc_attend_packed", "qxc_kv_read_rows"]
