@@ -73,20 +73,43 @@ def _ints(values):
     return a, a.buffer_info()[0]
 
 
-def _room(x, elements: int):
-    """The pointer of a dense tensor of at least `elements` elements; a raw
-    pointer as it is."""
-    if x is None:
-        return None
+_float_types = {}  # of torch, their qxc_dtype (filled by the first tensor that is checked)
+
+
+def _operand(x, dtype: int, device: int):
+    """The pointer of a tensor of `dtype` on `device` (page-locked host memory is
+    the device's too; an integer type of the same size may hold it); a raw
+    pointer as it is. A type that is none of a tensor's is left to the call."""
+    if x is None or isinstance(x, int):
+        return x
+    if isinstance(x, np.ndarray):
+        raise QxError(_lib.ERR_INVALID_ARG, "a host array where a device tensor is needed")
+    try:
+        at, kind, size = x.get_device(), x.dtype, x.element_size()
+    except AttributeError:  # no tensor
+        return _ptr(x)
+    if not _float_types:
+        import torch
+        _float_types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    if dtype in (F32, BF16, F16) and (_float_types.get(kind, dtype) != dtype or size != (4 if dtype == F32 else 2)):
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {kind}, another type than the call's ({dtype})")
+    if at != device and not (at < 0 and x.is_pinned()):
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor on {x.device}, the context is on device {device}")
+    return x.data_ptr()
+
+
+def _room(x, elements: int, dtype: int, device: int):
+    """_operand for a dense tensor of at least `elements` elements."""
+    ptr = _operand(x, dtype, device)
     try:
         held = x.numel()
-    except AttributeError:
-        return _ptr(x)
+    except AttributeError:  # no tensor
+        return ptr
     if not x.is_contiguous():
-        raise QxError(_lib.ERR_INVALID_ARG, f"an output must be dense: shape {tuple(x.shape)}, strides {x.stride()}")
+        raise QxError(_lib.ERR_INVALID_ARG, f"a tensor must be dense: shape {tuple(x.shape)}, strides {x.stride()}")
     if held < elements:
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {held} elements, {elements} needed")
-    return x.data_ptr()
+    return ptr
 
 
 def _token_stride(x, features: int, tokens: int = 0) -> int:
@@ -200,8 +223,9 @@ class Context:
         tensors; out is dense."""
         hq, hkv, d = model_shape(model)
         (keep, n), tokens = _ints(lengths), sum(lengths)
-        a = _lib.PackedArgs(model, len(lengths), n, _ptr(q), _ptr(k), _ptr(v), _room(out, tokens * hq * d),
-                            _token_stride(q, hq * d, tokens), _token_stride(k, hkv * d, tokens),
+        at = self.device
+        a = _lib.PackedArgs(model, len(lengths), n, _operand(q, dtype, at), _operand(k, dtype, at),
+                            _operand(v, dtype, at), _room(out, tokens * hq * d, dtype, at), _token_stride(q, hq * d, tokens), _token_stride(k, hkv * d, tokens),
                             _token_stride(v, hkv * d, tokens), dtype)
         self.check(self.lib.qxc_attend_packed(self.handle, C.byref(a)))
 
@@ -416,6 +440,10 @@ class KvArena:
             return BF16 if self.model == MODEL_QWEN3 else F32
         return self.key_dtype if self.model == MODEL_QWEN3 else F32
 
+    def _norm(self, weight):
+        """The pointer of a norm weight (Granite has none, and reads none)."""
+        return None if self.model != MODEL_QWEN3 else _room(weight, self.d, F32, self.ctx.device)
+
     def _tokens(self, counts) -> int:
         """Tokens that the tensors of a call hold at least; 0 for more than its
         sequences have room for, which the call refuses."""
@@ -436,11 +464,13 @@ class KvArena:
         qn, kn = layer_count * self.hq * self.d, layer_count * self.hkv * self.d
         tokens = self._tokens(counts)
         (keep_s, ids), (keep_p, at), (keep_c, n) = _ints(seq_ids), _ints(positions), _ints(counts)
+        in_dtype, on = self._default_dtype() if in_dtype is None else in_dtype, self.ctx.device
         a = _lib.AppendArgs(layer_begin, layer_count, len(positions), ids, at, n,
-                            _ptr(q), _ptr(k), _ptr(v), _room(q_rot, tokens * qn), _room(k_rot, tokens * kn),
+                            _operand(q, in_dtype, on), _operand(k, in_dtype, on), _operand(v, in_dtype, on),
+                            _room(q_rot, tokens * qn, rot_dtype, on), _room(k_rot, tokens * kn, rot_dtype, on),
                             _token_stride(q, qn, tokens), _token_stride(k, kn, tokens),
-                            _token_stride(v, kn, tokens), _ptr(q_norm), _ptr(k_norm),
-                            self._default_dtype() if in_dtype is None else in_dtype, rot_dtype, flags)
+                            _token_stride(v, kn, tokens), self._norm(q_norm), self._norm(k_norm), in_dtype,
+                            rot_dtype, flags)
         self.ctx.check(self.lib.qxc_kv_append(self.ctx.handle, self.handle, C.byref(a)))
 
     def read_rows(self, key_out, value_out, begins, counts, seq_ids=None, layer_begin: int = 0,
@@ -451,10 +481,11 @@ class KvArena:
         layer_count = self.layers - layer_begin if layer_count is None else layer_count
         if len(counts) != len(begins) or (seq_ids is not None and len(seq_ids) != len(begins)):
             raise QxError(_lib.ERR_INVALID_ARG, "begins, counts and seq_ids differ in length")
-        elements = self._tokens(counts) * layer_count * self.hkv * self.d
+        elements, on = self._tokens(counts) * layer_count * self.hkv * self.d, self.ctx.device
         (keep_s, ids), (keep_b, at), (keep_c, n) = _ints(seq_ids), _ints(begins), _ints(counts)
         a = _lib.ReadRowsArgs(layer_begin, layer_count, len(begins), ids, at, n,
-                              _room(key_out, elements), _room(value_out, elements), out_dtype)
+                              _room(key_out, elements, out_dtype, on), _room(value_out, elements, out_dtype, on),
+                              out_dtype)
         self.ctx.check(self.lib.qxc_kv_read_rows(self.ctx.handle, self.handle, C.byref(a)))
 
     def prefill_packed(self, q, k, v, out, lengths, seq_ids=None, layer: int = 0, dtype: int = BF16, q_norm=None,
@@ -466,10 +497,11 @@ class KvArena:
             raise QxError(_lib.ERR_INVALID_ARG, "lengths and seq_ids differ in length")
         qn, kn, tokens = self.hq * self.d, self.hkv * self.d, self._tokens(lengths)
         (keep_s, ids), (keep_l, n) = _ints(seq_ids), _ints(lengths)
-        a = _lib.PrefillPackedArgs(layer, len(lengths), ids, n, _ptr(q), _ptr(k), _ptr(v),
-                                   _room(out, tokens * qn), _token_stride(q, qn, tokens),
-                                   _token_stride(k, kn, tokens), _token_stride(v, kn, tokens), _ptr(q_norm),
-                                   _ptr(k_norm), dtype, flags)
+        on = self.ctx.device
+        a = _lib.PrefillPackedArgs(layer, len(lengths), ids, n, _operand(q, dtype, on), _operand(k, dtype, on),
+                                   _operand(v, dtype, on), _room(out, tokens * qn, dtype, on),
+                                   _token_stride(q, qn, tokens), _token_stride(k, kn, tokens),
+                                   _token_stride(v, kn, tokens), self._norm(q_norm), self._norm(k_norm), dtype, flags)
         self.ctx.check(self.lib.qxc_prefill_packed(self.ctx.handle, self.handle, C.byref(a)))
 
     def _decode_args(self, q, k, v, out, positions, layer_begin, layer_count, seq_ids, q_dtype, in_dtype,

@@ -143,3 +143,52 @@ def test_outputs_must_be_dense(model):
     attend(wide[10:])
     read(dense(k), dense(v))
     assert lib.made == ["qxc_kv_append", "qxc_prefill_packed", "qxc_attend_packed", "qxc_kv_read_rows"]
+
+
+@pytest.mark.parametrize("model", [MODEL_GRANITE, MODEL_QWEN3])
+def test_types_are_those_of_the_call(model):
+    """A tensor of another type would be read or written past its end, or as other numbers."""
+    ctx, arena = bare(model)
+    lib, (hq, hkv, d) = arena.lib, model_shape(model)
+    make = lambda h, t: torch.zeros(10, h, d, dtype=t)  # noqa: E731
+    types = {_lib.F32: torch.float32, _lib.BF16: torch.bfloat16, _lib.F16: torch.float16}
+
+    def append(t=torch.bfloat16, rot=torch.bfloat16, v=None, norm=None, **kw):
+        arena.append(make(hq, t), make(hkv, t), make(hkv, v or t), [0], [10], in_dtype=_lib.BF16, q_rot=make(hq, rot),
+                     k_rot=make(hkv, rot), k_norm=norm, **kw)
+    read = lambda t, **kw: arena.read_rows(make(hkv, t), make(hkv, t), [0], [10], **kw)  # noqa: E731
+    prefill = lambda t, o: arena.prefill_packed(make(hq, t), make(hkv, t), make(hkv, t), make(hq, o), [10])  # noqa: E731
+    attend = lambda t, o: ctx.attend_packed(model, make(hq, t), make(hkv, t), make(hkv, t), make(hq, o), [10])  # noqa: E731
+    b16, f16, f32 = torch.bfloat16, torch.float16, torch.float32
+    bad = [lambda: append(f32), lambda: append(f16), lambda: append(torch.float64), lambda: append(v=f16),
+           lambda: append(rot=f32), lambda: append(rot=torch.int8), lambda: read(b16), lambda: read(f32, out_dtype=_lib.F16),
+           lambda: prefill(f32, b16), lambda: prefill(b16, f32), lambda: attend(f16, b16), lambda: attend(b16, f16)]
+    if model == MODEL_QWEN3:
+        bad += [lambda: append(norm=torch.zeros(d, dtype=b16)), lambda: append(norm=torch.zeros(2 * d)[::2]),
+                lambda: append(norm=torch.zeros(d - 1))]
+    for call in bad:
+        refused(lib, call, match="type|dense|needed")
+    for dt, t in types.items():
+        read(t, out_dtype=dt)
+    read(torch.int16, out_dtype=_lib.BF16)  # as KvArena.tensor shows 16-bit storage
+    append()
+    append(norm=torch.zeros(d))
+    prefill(b16, b16)
+    attend(b16, b16)
+    assert len(lib.made) == 8
+
+
+def test_tensors_are_on_the_context_device():
+    """Host memory that the device cannot address, or another device's, would fault there."""
+    ctx, arena = bare(device=0)
+    q, k = torch.zeros(10, 16, 64, dtype=torch.bfloat16), torch.zeros(10, 8, 64, dtype=torch.bfloat16)
+    raw = 1 << 20
+    for call in (lambda: arena.append(None, k, raw, [0], [10], in_dtype=_lib.BF16),
+                 lambda: arena.append(None, raw, raw, [0], [10], k_rot=k, in_dtype=_lib.BF16),
+                 lambda: arena.append(None, k.float().numpy(), raw, [0], [10], in_dtype=_lib.F32),
+                 lambda: arena.read_rows(k.float(), raw, [0], [10]), lambda: arena.read_rows(raw, k.float().numpy(), [0], [10]),
+                 lambda: arena.prefill_packed(q, raw, raw, raw, [10]), lambda: arena.prefill_packed(raw, raw, raw, q, [10]),
+                 lambda: ctx.attend_packed(MODEL_GRANITE, raw, raw, k, raw, [10])):
+        refused(arena.lib, call, match="device|host")
+    arena.read_rows(raw, raw, [0], [10])
+    assert arena.lib.made == ["qxc_kv_read_rows"]
