@@ -119,7 +119,7 @@ def _token_stride(x, features: int, tokens: int = 0) -> int:
     if x is None or isinstance(x, int):
         return 0
     try:
-        held = x.shape[0]
+        held = x.shape[0] if x.dim() else 0
         plain = x.is_contiguous() and x.numel() == held * features
     except AttributeError:  # no tensor
         return 0

@@ -192,3 +192,9 @@ def test_tensors_are_on_the_context_device():
         refused(arena.lib, call, match="device|host")
     arena.read_rows(raw, raw, [0], [10])
     assert arena.lib.made == ["qxc_kv_read_rows"]
+
+
+def test_a_tensor_without_tokens_is_refused():
+    ctx, arena = bare()
+    for x in (torch.zeros(()), torch.zeros(512)):
+        refused(arena.lib, lambda: arena.append(None, x, x, [0], [1], in_dtype=_lib.F32))
