@@ -56,9 +56,19 @@ def _ptr(x) -> int | None:
     raise TypeError(f"cannot take a pointer of {type(x)}")
 
 
-def _i32(values):
-    """A host int32 array of `values`, or None."""
-    return None if values is None else (C.c_int32 * len(values)).from_buffer(array("i", values))
+def _i32(values, n: int):
+    """A host int32 array of `values`, n of them (fewer: the rest are 0), or None."""
+    if values is None:
+        return None
+    if not hasattr(values, "__len__"):
+        values = list(values)  # may be read twice
+    try:
+        a = array("i", values)
+        if len(a) == n > 0:
+            return (C.c_int32 * n).from_buffer(a)
+    except (TypeError, OverflowError):  # not whole numbers, or of more bits, which are dropped
+        pass
+    return (C.c_int32 * n)(*[int(x) for x in values])
 
 
 _no_ints = array("i")
@@ -507,11 +517,7 @@ class KvArena:
     def _decode_args(self, q, k, v, out, positions, layer_begin, layer_count, seq_ids, q_dtype, in_dtype,
                      out_dtype, flags, split, q_rot_out, q_norm, k_norm):
         n = len(positions)
-        try:
-            pos, ids = _i32(positions), _i32(seq_ids)
-        except TypeError:  # not whole numbers
-            pos = (C.c_int32 * n)(*[int(x) for x in positions])
-            ids = (C.c_int32 * n)(*[int(x) for x in seq_ids]) if seq_ids is not None else None
+        pos, ids = _i32(positions, n), _i32(seq_ids, n)
         a = _lib.DecodeArgs(layer_begin, layer_count, n, ids, pos, _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                             _ptr(q_rot_out), _ptr(q_norm), _ptr(k_norm), q_dtype, in_dtype, out_dtype, flags,
                             split)

@@ -198,3 +198,21 @@ def test_a_tensor_without_tokens_is_refused():
     ctx, arena = bare()
     for x in (torch.zeros(()), torch.zeros(512)):
         refused(arena.lib, lambda: arena.append(None, x, x, [0], [1], in_dtype=_lib.F32))
+
+
+def test_positions_and_sequences_of_a_decode():
+    """Any iterable of numbers; as many sequences as positions are read by the library,
+    so a list that is shorter is filled up and one that is longer is an error."""
+    arena = bare()[1]
+    args = lambda p, ids: arena._decode_args(1, 1, 1, 1, p, 0, 1, ids, 0, 0, 0, 0, 0, None, None, None)  # noqa: E731
+    for p, ids in (([5, 7], [1, 0]), ((5, 7), np.array([1, 0])), (np.array([5.0, 7.0]), (x for x in (1, 0))),
+                   ([5, 7.0], (x for x in (1.0, 0))),
+                   (torch.tensor([5, 7]), torch.tensor([1.0, 0.0]))):
+        pos, seq = args(p, ids)._keep
+        assert list(pos) == [5, 7] and list(seq) == [1, 0]
+    pos, seq = args([5, 7], [3])._keep
+    assert len(seq) == 2 and list(seq) == [3, 0]
+    with pytest.raises(IndexError):
+        args([5, 7], [1, 0, 2])
+    assert len(args([], None)._keep[0]) == 0 and len(args([], [])._keep[1]) == 0
+    assert list(args([2 ** 31], None)._keep[0]) == [-2 ** 31]  # which the library refuses
