@@ -79,7 +79,12 @@ def _ints(values):
     its address; None gives address None."""
     if values is None:
         return _no_ints, None
-    a = array("i", values)
+    try:
+        a = array("i", values)
+    except OverflowError:
+        raise QxError(_lib.ERR_INVALID_ARG, f"numbers of more than 32 bits: {values}") from None
+    except TypeError:  # not whole numbers
+        a = array("i", [int(x) for x in values])
     return a, a.buffer_info()[0]
 
 

@@ -216,3 +216,14 @@ def test_positions_and_sequences_of_a_decode():
         args([5, 7], [1, 0, 2])
     assert len(args([], None)._keep[0]) == 0 and len(args([], [])._keep[1]) == 0
     assert list(args([2 ** 31], None)._keep[0]) == [-2 ** 31]  # which the library refuses
+
+
+def test_numbers_of_more_than_32_bits_are_refused():
+    ctx, arena = bare()
+    for big in (2 ** 31, -2 ** 31 - 1, 2 ** 40):
+        for call in (lambda: arena.append(None, 1, 1, [big], [1]), lambda: arena.append(None, 1, 1, [0], [big]),
+                     lambda: arena.append(None, 1, 1, [0], [1], seq_ids=[big]), lambda: arena.read_rows(1, 1, [big], [1]),
+                     lambda: arena.prefill_packed(1, 1, 1, 1, [big]), lambda: ctx.attend_packed(0, 1, 1, 1, 1, [big])):
+            refused(arena.lib, call)
+    arena.append(None, 1, 1, np.array([0.0]), [1.0])
+    assert arena.lib.made == ["qxc_kv_append"]
