@@ -440,6 +440,11 @@ class KvArena:
 
     def write(self, seq: int, layer: int, begin: int, keys: np.ndarray | None, values: np.ndarray | None):
         count = (keys if keys is not None else values).shape[0]
+        if self.key_dtype == Q4:
+            for rows in (keys, values):
+                if rows is not None and (rows.dtype != np.uint8 or rows.shape != (count, *self.row_shape)):
+                    raise QxError(_lib.ERR_INVALID_ARG, f"a 4-bit arena takes raw rows: uint8 {(count, *self.row_shape)}, "
+                                                        f"not {rows.dtype} {rows.shape}")
         if keys is not None:
             keys = np.ascontiguousarray(keys, _np_dtype(self.key_dtype))
         if values is not None:

@@ -227,3 +227,15 @@ def test_numbers_of_more_than_32_bits_are_refused():
             refused(arena.lib, call)
     arena.append(None, 1, 1, np.array([0.0]), [1.0])
     assert arena.lib.made == ["qxc_kv_append"]
+
+
+def test_raw_rows_written_to_a_4bit_arena():
+    """Values are no rows: cut to bytes, the first 288 of 512 would be written."""
+    arena = bare()[1]
+    raw = np.zeros((3, 288), np.uint8)
+    for k, v in ((np.zeros((3, 8, 64), np.float32), None), (raw[:, :287], None), (raw, raw[:2]), (raw, raw.astype(np.int32)),
+                 (None, np.zeros((3, 8, 64), np.uint8))):
+        refused(arena.lib, lambda: arena.write(0, 0, 0, k, v))
+    arena.write(0, 0, 0, raw, None)
+    arena.write(0, 0, 0, np.zeros((6, 288), np.uint8)[::2], raw)
+    assert arena.lib.made == ["qxc_kv_write"] * 2
