@@ -516,12 +516,14 @@ __global__ void __launch_bounds__(Packed<M, T>::NT, 1) qx_packed_kernel(const __
 #pragma unroll
         for (int c = 4; c < 124; c += 8) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) m4[e] = fmax3f(m4[e], s[c + 2 * e], s[c + 2 * e + 1]);
+          for (int e = 0; e < 4; ++e) m4[e] = fmax3f_nan(m4[e], s[c + 2 * e], s[c + 2 * e + 1]);
         }
-        m4[0] = fmax3f(m4[0], s[124], s[125]);
-        m4[1] = fmax3f(m4[1], s[126], s[127]);
-        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * C::UNIT;
-        const bool raise = top > m + C::TAU;  // true on the first tile (m = -inf)
+        m4[0] = fmax3f_nan(m4[0], s[124], s[125]);
+        m4[1] = fmax3f_nan(m4[1], s[126], s[127]);
+        const float top = fmax3f_nan(fmax3f_nan(m4[0], m4[1], m4[2]), m4[3], m4[3]) * C::UNIT;
+        // true on the first tile (m = -inf), and for a score that is NaN: it becomes the
+        // reference and with it the row (exp2_fma would make it a weight of zero)
+        const bool raise = !(top <= m + C::TAU);
         if (__any_sync(0xffffffffu, raise)) {
           const float keep = raise ? fast_exp2(m - top) : 1.0f;
           if (i > 0) {

@@ -105,6 +105,13 @@ __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   return d;
 }
 
+// The same, NaN where one of them is (fmax3f leaves NaNs out).
+__device__ __forceinline__ float fmax3f_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 __device__ __forceinline__ float softmax_exp(float x, bool pinned) {
   return pinned ? pinned_exp(x) : native_exp(x);
 }

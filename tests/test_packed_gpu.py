@@ -424,3 +424,59 @@ def test_refusals(gpu_ctx):
     gpu_ctx.sync()
     arena.close()
     plain.close()
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_bad_key_reaches_every_row_that_attends_it(gpu_ctx, model, dtype):
+    """Wherever in a tile it lies: the rows from it on are not finite and reported,
+    the rows before it as without it. An infinite element makes a score infinite: of
+    +inf nothing can be made, -inf is a weight of zero."""
+    rng = np.random.default_rng([model, dtype, 32])
+    lengths = [40, 300, 30]
+    q, k, v = inputs(rng, model, sum(lengths), dtype)
+    clean = attend(gpu_ctx, model, q, k, v, lengths, dtype)
+    end = 340
+    hq, hkv, _ = model_shape(model)
+    for at in [40 + o for o in range(32)] + [40 + 128 + o for o in range(32)] + [339]:
+        for bad in (float("nan"), float("inf")):
+            keep = k[at].clone()
+            if bad != bad:
+                k[at] = bad
+                hit = torch.ones(end - at, hq, dtype=torch.bool, device="cuda")
+            else:
+                k[at, :, 3] = bad
+                hit = q[at:end, :, 3] > 0
+            out = torch.zeros_like(clean)
+            gpu_ctx.attend_packed(model, q, k, v, out, lengths, dtype=dtype)
+            if hit.any():
+                with pytest.raises(QxError) as e:
+                    gpu_ctx.sync()
+                assert e.value.status == _lib.ERR_NONFINITE
+            else:
+                gpu_ctx.sync()
+            k[at] = keep
+            finite = torch.isfinite(out[at:end])
+            assert not finite[hit].any(), (at, bad)
+            if bad == bad:  # its weight is 0: rows of more than one token are still means of the others
+                assert finite[1:][~hit[1:]].all(), (at, bad)
+            assert torch.equal(out[:at], clean[:at]) and torch.equal(out[end:], clean[end:])
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_a_bad_query_is_its_own_rows_affair(gpu_ctx, model):
+    rng = np.random.default_rng([model, 33])
+    q, k, v = inputs(rng, model, 333, BF16)
+    clean = attend(gpu_ctx, model, q, k, v, [333], BF16)
+    hq, _, d = model_shape(model)
+    for row, head, dim in ((0, 0, 0), (77, hq - 1, d - 1), (200, 3, 17), (332, 1, 5)):
+        keep = q[row, head, dim].clone()
+        q[row, head, dim] = float("nan")
+        out = torch.zeros_like(clean)
+        gpu_ctx.attend_packed(model, q, k, v, out, [333])
+        with pytest.raises(QxError) as e:
+            gpu_ctx.sync()
+        q[row, head, dim] = keep
+        assert e.value.status == _lib.ERR_NONFINITE and not torch.isfinite(out[row, head]).any()
+        out[row, head] = clean[row, head]
+        assert torch.equal(out, clean)
