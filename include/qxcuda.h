@@ -162,7 +162,8 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
 /* Write the rows of counts[i] new tokens of each of seq_count sequences
  * (packed one after another) into layers [layer_begin, layer_begin +
  * layer_count), and rotate their queries, in one pass: per head RMSNorm (Qwen:
- * sum of squares in f64) and rotation of q and k at positions positions[i],
+ * sum of squares in f64 for keys, in f32 for queries and in f64 where that
+ * overflows) and rotation of q and k at positions positions[i],
  * positions[i] + 1, ..., keys and values quantised into the cache. positions[i]
  * must equal the sequence's length, positions[i] + counts[i] <= capacity, else
  * QXC_ERR_POSITION; counts may be 0, a sequence may appear once. Lengths

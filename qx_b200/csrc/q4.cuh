@@ -92,17 +92,18 @@ __device__ __forceinline__ void store8(void* base, long long i, int dtype, bool 
   }
 }
 
-// 1 / sqrt(mean + 1e-6) of a key head, rounded once to f32. The sum of squares is
-// a double (products of two 16-bit inputs and their sum are exact in it), so its
-// order does not matter: quantised keys sit next to rounding borders, where an ulp
-// of the norm would decide a code.
-template <class M>
-__device__ __forceinline__ float key_inv_rms(const float* x) {
+// 1 / sqrt(mean + 1e-6) of a head over LANES lanes of N elements each, rounded
+// once to f32. The sum of squares is a double (products of two 16-bit inputs and
+// their sum are exact in it), so its order does not matter: quantised keys sit next
+// to rounding borders, where an ulp of the norm would decide a code. Queries, which
+// are not quantised to 4 bits, are summed in f32 and come here where that overflows.
+template <class M, int N = 8, int LANES = Q4Row<M>::LPH>
+__device__ __forceinline__ float exact_inv_rms(const float* x) {
   double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sum = fma((double)x[e], (double)x[e], sum);
+  for (int e = 0; e < N; ++e) sum = fma((double)x[e], (double)x[e], sum);
 #pragma unroll
-  for (int o = Q4Row<M>::LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return (float)rsqrt(sum * (1.0 / M::D) + 1.0e-6);
 }
 
@@ -115,7 +116,7 @@ template <class M>
 __device__ __forceinline__ void rotate_key(float* x, int c, const float* norm, const float2* tab) {
   constexpr int LPH = Q4Row<M>::LPH;
   if constexpr (M::QWEN) {
-    const float inv = key_inv_rms<M>(x);
+    const float inv = exact_inv_rms<M>(x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inv), norm ? norm[8 * c + e] : 1.0f);
   }

@@ -175,7 +175,11 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 4) qx_q4_append_kernel(co
         float sum = s2.x + s2.y;
 #pragma unroll
         for (int o = R::LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = rsqrtf(fmaf(sum, 1.0f / M::D, 1.0e-6f));
+        float inv = rsqrtf(fmaf(sum, 1.0f / M::D, 1.0e-6f));
+        if (__any_sync(0xffffffffu, !isfinite(sum))) {  // elements beyond 1.6e18 may pass f32 in their squares
+          const float x8[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+          inv = exact_inv_rms<M>(x8);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(__fmul2_rn(v[e], make_float2(inv, inv)), w[e]);
       }

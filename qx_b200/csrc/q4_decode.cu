@@ -204,7 +204,8 @@ __device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long fi
     float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    const float inv = __frcp_rn(__fsqrt_rn(fmaf(sum, 1.0f / M::D, 1.0e-6f)));
+    float inv = __frcp_rn(__fsqrt_rn(fmaf(sum, 1.0f / M::D, 1.0e-6f)));
+    if (__any_sync(0xffffffffu, !isfinite(sum))) inv = exact_inv_rms<M, NG * 8, 4>(x);
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll

@@ -715,3 +715,37 @@ def test_an_append_right_behind_a_step(gpu_ctx):
             outs.append(out.clone())
     assert all(torch.equal(outs[-1], o) for o in outs)
     arena.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e17, 1e20, 1e30, 3e37])
+def test_norms_of_the_largest_queries_and_keys(gpu_ctx, dtype, size):
+    """Elements whose squares pass f32: the norm brings any of them back to size 1."""
+    rng = np.random.default_rng([dtype, int(np.log10(size))])
+    arena = make_arena(gpu_ctx, MODEL_QWEN3, [41])
+    q, k = (tensor(rng, (40, 1, h, 128), dtype) for h in (32, 4))
+    q[3:, 0, 5:9] *= size
+    q[::2, 0, 20, 77] = size
+    k[:, 0, 1] *= size
+    v = tensor(rng, (40, 1, 4, 128), dtype)
+    rot, keys = torch.zeros(40, 1, 32, 128, device="cuda"), torch.zeros(40, 1, 4, 128, device="cuda")
+    arena.append(q, k, v, [0], [40], in_dtype=dtype, q_rot=rot, k_rot=keys, rot_dtype=F32)
+    gpu_ctx.sync()
+    for x, got in ((q, rot), (k, keys)):
+        want = ref.rotate64(MODEL_QWEN3, host(x[:, 0]), range(40))
+        pair = np.hypot(want[..., :64], want[..., 64:])
+        # as in test_append_and_read_rows; the reciprocal of a root beyond 2^126 has fewer
+        # bits: half a step of 2^-149 of at least 2^-128
+        assert ref.close(host(got[:, 0]), want, (8 * 2.0 ** -24 + 2.0 ** -22) * np.concatenate([pair, pair], -1) + 1e-30) <= 1
+    dq = tensor(rng, (1, 1, 32, 128), dtype)
+    dq[0, 0, 4:7] *= size
+    dk, dv = tensor(rng, (1, 1, 4, 128), dtype, size), tensor(rng, (1, 1, 4, 128), dtype)
+    out, turned = torch.zeros(1, 1, 32, 128, device="cuda"), torch.zeros(1, 1, 32, 128, device="cuda")
+    arena.decode(dq, dk, dv, out, [40], q_dtype=dtype, in_dtype=dtype, q_rot_out=turned)
+    gpu_ctx.sync()
+    want = ref.rotate64(MODEL_QWEN3, host(dq[0]), [40])
+    pair = np.hypot(want[..., :64], want[..., 64:])
+    assert ref.close(host(turned[0]), want, (8 * 2.0 ** -24 + 2.0 ** -22) * np.concatenate([pair, pair], -1) + 1e-30) <= 1
+    if size < 1e37:  # (check_decode knows of eight roundings of a query)
+        check_decode(gpu_ctx, arena, dq, dk, dv, out, [40], F32)
+    arena.close()
