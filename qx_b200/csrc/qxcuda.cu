@@ -1172,14 +1172,15 @@ qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
 // 13.6 for 8 sequences of 1000.
 int q4_least_tiles(int total, int sms) { return std::max(2, std::min(8, (total + sms - 1) / sms)); }
 
-// One decode step on a 4-bit arena, its arguments checked and its pages mapped.
-qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
+// One decode step on a 4-bit arena, its arguments checked; sequence ids[i] attends
+// attend[i] rows. The workspace is reserved for the largest launch before the first,
+// and before pages are mapped: a call that is refused has done nothing.
+qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a, const int* ids, const int* attend) {
   if (!ctx->q4_decode_set) {
     QXC_CUDA(ctx, setup_q4_decode());
     ctx->q4_decode_set = true;
   }
-  std::vector<int32_t> attend(a->seq_count), ones(a->seq_count, 1);
-  for (int i = 0; i < a->seq_count; ++i) attend[i] = a->positions[i] + 1;
+  std::vector<int32_t> ones(a->seq_count, 1);
   Q4DecodeParams p;
   p.arena = q4_arena(kv);
   p.layer_begin = a->layer_begin;
@@ -1197,7 +1198,9 @@ qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
   p.out_dtype = a->out_dtype;
   p.vec = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16);
   p.err = ctx->err_dev;
-  return each_part(a->seq_count, a->seq_ids, attend.data(), ones.data(), [&](const Q4Seq* seqs, int n, int first, int) {
+  size_t operands = 0, units = 0, sums = 0, bytes = 0;  // of the planned launch's workspace
+  // how a launch's cells lie on the line of tiles
+  auto plan = [&](const Q4Seq* seqs, int n, int first) -> qxc_status {
     memcpy(p.seqs, seqs, n * sizeof(Q4Seq));
     p.n_seq = n;
     p.seq_begin = first;
@@ -1215,7 +1218,6 @@ qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
     // every CTA the GPU holds at once takes the same stretch of the line
     const int slots = q4_decode_blocks_per_sm() * ctx->sm_count;
     if (!p.padded) p.per_cta = std::max(q4_least_tiles(p.total, ctx->sm_count), (p.total + slots - 1) / slots);
-    ctx->last_split = p.per_cta * kQ4Tile;
     const int ctas = (p.total + p.per_cta - 1) / p.per_cta;
     p.max_parts = 1;
     for (int i = 0; i < n; ++i) {  // a cell between two borders of its own touches a CTA more than it fills
@@ -1226,10 +1228,24 @@ qxc_status q4_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
     // workspace: the queries' operands and their units, then, where cells may be
     // shared by CTAs, two partials a CTA: [HQ][D] sums, then [HQ] (m, l)
     const size_t cells = (size_t)n * a->layer_count, heads = p.max_parts > 1 ? 2 * (size_t)ctas * kv->hq : 0;
-    const size_t operands = cells * q4_operand_bytes(kv->hq, kv->d, a->out_dtype);
-    const size_t units = (cells * kv->hq * sizeof(float) + 15) / 16 * 16, sums = heads * kv->d * sizeof(float);
-    qxc_status st = reserve(ctx, &ctx->q4_work, operands + units + sums + heads * sizeof(float2));
-    if (st != QXC_OK) return st;
+    operands = cells * q4_operand_bytes(kv->hq, kv->d, a->out_dtype);
+    units = (cells * kv->hq * sizeof(float) + 15) / 16 * 16;
+    sums = heads * kv->d * sizeof(float);
+    bytes = operands + units + sums + heads * sizeof(float2);
+    return QXC_OK;
+  };
+  size_t most = 0;
+  qxc_status st = each_part(a->seq_count, ids, attend, ones.data(), [&](const Q4Seq* seqs, int n, int first, int) {
+    qxc_status planned = plan(seqs, n, first);
+    most = std::max(most, bytes);
+    return planned;
+  });
+  if (st == QXC_OK) st = reserve(ctx, &ctx->q4_work, most);
+  if (st == QXC_OK) st = ensure_pages(ctx, kv, a->seq_count, ids, attend);
+  if (st != QXC_OK) return st;
+  return each_part(a->seq_count, ids, attend, ones.data(), [&](const Q4Seq* seqs, int n, int first, int) -> qxc_status {
+    if (a->seq_count > kQ4Seqs) plan(seqs, n, first);  // else it is the plan made above
+    ctx->last_split = p.per_cta * kQ4Tile;
     p.operands = reinterpret_cast<uint4*>(ctx->q4_work.ptr);
     p.units = reinterpret_cast<float*>(ctx->q4_work.ptr + operands);
     p.part_o = reinterpret_cast<float*>(ctx->q4_work.ptr + operands + units);
@@ -1806,14 +1822,14 @@ qxc_status qxc_decode(qxc_ctx* ctx, qxc_kv* kv, const qxc_decode_args* a) {
   {
     std::vector<int> ids(a->seq_count);
     for (int i = 0; i < a->seq_count; ++i) ids[i] = a->seq_ids ? a->seq_ids[i] : i;
+    if (is_q4(kv)) {
+      qxc_status st = guarded(ctx, [&] { return q4_decode(ctx, kv, a, ids.data(), attend.data()); });
+      if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
+        for (int i = 0; i < a->seq_count; ++i) kv->len[ids[i]] += 1;
+      return st;
+    }
     qxc_status st = ensure_pages(ctx, kv, a->seq_count, ids.data(), attend.data());
     if (st != QXC_OK) return st;
-  }
-  if (is_q4(kv)) {
-    qxc_status st = guarded(ctx, [&] { return q4_decode(ctx, kv, a); });
-    if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
-      for (int i = 0; i < a->seq_count; ++i) kv->len[a->seq_ids ? a->seq_ids[i] : i] += 1;
-    return st;
   }
   CallPlan plan;
   qxc_status st = plan_call(ctx, kv, a->seq_count, a->seq_ids, attend.data(), new_slot.data(), rope.data(),

@@ -749,3 +749,62 @@ def test_norms_of_the_largest_queries_and_keys(gpu_ctx, dtype, size):
     if size < 1e37:  # (check_decode knows of eight roundings of a query)
         check_decode(gpu_ctx, arena, dq, dk, dv, out, [40], F32)
     arena.close()
+
+
+def refused_capture(ctx, status, *calls):
+    """The last of `calls` is refused under capture."""
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.set_stream(stream)
+    with torch.cuda.stream(stream), pytest.raises(QxError) as e:
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            for call in calls:
+                launches = ctx.launch_count
+                call()
+    assert e.value.status == status
+    ctx.set_stream(None)
+    return ctx.launch_count - launches
+
+
+def test_a_refused_capture_of_many_sequences_holds_none_of_its_launches():
+    """The last of three launches is the one whose workspace is too small."""
+    rng = np.random.default_rng(34)
+    ctx = Context(0)
+    rows = [1] * 400 + [2000] * 30
+    arena = make_arena(ctx, MODEL_GRANITE, [n + 1 for n in rows], page=64)
+    fill(ctx, arena, rng, rows)
+    q, k, v = (tensor(rng, (430, 1, h, 64), BF16) for h in (16, 8, 8))
+    out = torch.zeros(430, 1, 16, 64, device="cuda")
+    torch.cuda.synchronize()
+    go = lambda n: arena.decode(q, k, v, out, rows[:n], q_dtype=BF16, in_dtype=BF16, flags=DECODE_NO_ADVANCE)  # noqa: E731
+    go(400)
+    ctx.sync()
+    assert refused_capture(ctx, _lib.ERR_UNSUPPORTED, lambda: go(200), lambda: go(430)) == 0
+    go(430)
+    ctx.sync()
+    some = [0, 199, 200, 399, 400, 429]
+    check_decode(ctx, arena, q[some], k[some], v[some], out[some], [rows[i] for i in some], F32, ids=some)
+    arena.close()
+    ctx.close()
+
+
+def test_a_refused_capture_maps_no_page():
+    """A mapping that is captured and thrown away with the graph would leave the device without it."""
+    rng = np.random.default_rng(35)
+    ctx = Context(0)
+    arena = KvArena(ctx, MODEL_QWEN3, 1, 2, 200, Q4, page_size=64, pool_pages=6)
+    fill(ctx, arena, rng, [64, 64])
+    q, k, v = (tensor(rng, (2, 1, h, 128), BF16) for h in (32, 4, 4))
+    out = torch.zeros(2, 1, 32, 128, device="cuda")
+    torch.cuda.synchronize()
+    go = lambda n: arena.decode(q, k, v, out, [64] * n, out_dtype=F32)  # noqa: E731
+    kv = [torch.zeros(1, 1, 4, 128, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    refused_capture(ctx, _lib.ERR_UNSUPPORTED, lambda: arena.read_rows(*kv, [0], [1]), lambda: go(2))
+    assert arena.page_stats() == (2, 4) and [arena.len(i) for i in range(2)] == [64, 64]
+    go(2)
+    ctx.sync()
+    assert arena.page_stats() == (4, 2)
+    check_decode(ctx, arena, q, k, v, out, [64, 64], F32)
+    arena.close()
+    ctx.close()
