@@ -2858,7 +2858,7 @@ qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed
     ap.seq_ids = a->seq_ids;
     ap.positions = zeros.data();
     ap.counts = a->lengths;
-    ap.q = a->q;
+    ap.q = total ? a->q : nullptr;
     ap.k = a->k;
     ap.v = a->v;
     ap.q_rot = total ? ctx->packed_rot.ptr : nullptr;

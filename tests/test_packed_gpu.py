@@ -480,3 +480,21 @@ def test_a_bad_query_is_its_own_rows_affair(gpu_ctx, model):
         assert e.value.status == _lib.ERR_NONFINITE and not torch.isfinite(out[row, head]).any()
         out[row, head] = clean[row, head]
         assert torch.equal(out, clean)
+
+
+def test_a_prefill_without_tokens(gpu_ctx):
+    """Only empty prompts: nothing is launched or written, the positions still have to hold."""
+    arena = KvArena(gpu_ctx, MODEL_GRANITE, 1, 3, 16, Q4)
+    q, k = (torch.zeros(4, h, 64, device="cuda", dtype=torch.bfloat16) for h in (16, 8))
+    out = torch.full((4, 16, 64), 5.0, device="cuda", dtype=torch.bfloat16)
+    launches = gpu_ctx.launch_count
+    arena.prefill_packed(q, k, k, out, [0, 0], seq_ids=[2, 0])
+    arena.prefill_packed(None, None, None, None, [0])
+    gpu_ctx.sync()
+    assert gpu_ctx.launch_count == launches and (out == 5.0).all() and [arena.len(i) for i in range(3)] == [0, 0, 0]
+    arena.prefill_packed(q, k, k, out, [4])
+    with pytest.raises(QxError) as e:
+        arena.prefill_packed(q, k, k, out, [0])
+    assert e.value.status == _lib.ERR_POSITION
+    gpu_ctx.sync()
+    arena.close()
