@@ -91,10 +91,15 @@ def _ints(values):
 _float_types = {}  # of torch, their qxc_dtype (filled by the first tensor that is checked)
 
 
-def _operand(x, dtype: int, device: int):
+def _16bit(dtype: int):
+    """The type that a packed prompt's tensors have; None for one that the call refuses."""
+    return dtype if dtype in (BF16, F16) else None
+
+
+def _operand(x, dtype: int | None, device: int):
     """The pointer of a tensor of `dtype` on `device` (page-locked host memory is
     the device's too; an integer type of the same size may hold it); a raw
-    pointer as it is. A type that is none of a tensor's is left to the call."""
+    pointer as it is. A type that no tensor has is left to the call to refuse."""
     if x is None or isinstance(x, int):
         return x
     if isinstance(x, np.ndarray):
@@ -113,7 +118,7 @@ def _operand(x, dtype: int, device: int):
     return x.data_ptr()
 
 
-def _room(x, elements: int, dtype: int, device: int):
+def _room(x, elements: int, dtype: int | None, device: int):
     """_operand for a dense tensor of at least `elements` elements."""
     ptr = _operand(x, dtype, device)
     try:
@@ -238,9 +243,9 @@ class Context:
         tensors; out is dense."""
         hq, hkv, d = model_shape(model)
         (keep, n), tokens = _ints(lengths), sum(lengths)
-        at = self.device
-        a = _lib.PackedArgs(model, len(lengths), n, _operand(q, dtype, at), _operand(k, dtype, at),
-                            _operand(v, dtype, at), _room(out, tokens * hq * d, dtype, at), _token_stride(q, hq * d, tokens), _token_stride(k, hkv * d, tokens),
+        at, kind = self.device, _16bit(dtype)
+        a = _lib.PackedArgs(model, len(lengths), n, _operand(q, kind, at), _operand(k, kind, at),
+                            _operand(v, kind, at), _room(out, tokens * hq * d, kind, at), _token_stride(q, hq * d, tokens), _token_stride(k, hkv * d, tokens),
                             _token_stride(v, hkv * d, tokens), dtype)
         self.check(self.lib.qxc_attend_packed(self.handle, C.byref(a)))
 
@@ -517,9 +522,9 @@ class KvArena:
             raise QxError(_lib.ERR_INVALID_ARG, "lengths and seq_ids differ in length")
         qn, kn, tokens = self.hq * self.d, self.hkv * self.d, self._tokens(lengths)
         (keep_s, ids), (keep_l, n) = _ints(seq_ids), _ints(lengths)
-        on = self.ctx.device
-        a = _lib.PrefillPackedArgs(layer, len(lengths), ids, n, _operand(q, dtype, on), _operand(k, dtype, on),
-                                   _operand(v, dtype, on), _room(out, tokens * qn, dtype, on),
+        on, kind = self.ctx.device, _16bit(dtype)
+        a = _lib.PrefillPackedArgs(layer, len(lengths), ids, n, _operand(q, kind, on), _operand(k, kind, on),
+                                   _operand(v, kind, on), _room(out, tokens * qn, kind, on),
                                    _token_stride(q, qn, tokens), _token_stride(k, kn, tokens),
                                    _token_stride(v, kn, tokens), self._norm(q_norm), self._norm(k_norm), dtype, flags)
         self.ctx.check(self.lib.qxc_prefill_packed(self.ctx.handle, self.handle, C.byref(a)))

@@ -239,3 +239,16 @@ def test_raw_rows_written_to_a_4bit_arena():
     arena.write(0, 0, 0, raw, None)
     arena.write(0, 0, 0, np.zeros((6, 288), np.uint8)[::2], raw)
     assert arena.lib.made == ["qxc_kv_write"] * 2
+
+
+def test_types_that_a_call_refuses_reach_it():
+    """The library says that a type is unsupported, not that a tensor has another."""
+    ctx, arena = bare()
+    q, k = torch.zeros(10, 16, 64, dtype=torch.bfloat16), torch.zeros(10, 8, 64, dtype=torch.bfloat16)
+    for dt in (_lib.F32, _lib.Q4, 9):
+        ctx.attend_packed(MODEL_GRANITE, q, k, k, torch.zeros_like(q), [10], dtype=dt)
+        arena.prefill_packed(q, k, k, torch.zeros_like(q), [10], dtype=dt)
+    for dt in (_lib.Q4, 9):
+        arena.append(None, k, k, [0], [10], in_dtype=dt)
+        arena.read_rows(k, k, [0], [10], out_dtype=dt)
+    assert len(arena.lib.made) == 10
