@@ -1129,6 +1129,30 @@ qxc_status check_rows(qxc_ctx* ctx, const qxc_kv* kv, int layer_begin, int layer
   return QXC_OK;
 }
 
+// The arguments of an append; ids[i] and ends[i] as in check_rows.
+qxc_status check_append(qxc_ctx* ctx, const qxc_kv* kv, const qxc_append_args* a, std::vector<int>* ids,
+                        std::vector<int>* ends, long long* total) {
+  qxc_status st = check_rows(ctx, kv, a->layer_begin, a->layer_count, a->seq_count, a->seq_ids, a->positions, a->counts,
+                             ids, ends, total);
+  if (st != QXC_OK) return st;
+  if (!valid_dtype(a->in_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
+  if (!a->q != !a->q_rot) return fail(ctx, QXC_ERR_INVALID_ARG, "q and q_rot go together");
+  if ((a->q_rot || a->k_rot) && !valid_dtype(a->rot_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
+  if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0)
+    return fail(ctx, QXC_ERR_INVALID_ARG, "negative token stride");
+  std::vector<char> seen(kv->desc.sequences, 0);
+  for (int i = 0; i < a->seq_count; ++i) {
+    const int seq = (*ids)[i];
+    if (seen[seq]) return fail(ctx, QXC_ERR_INVALID_ARG, "sequence %d appears twice in one call", seq);
+    seen[seq] = 1;
+    // KvCache::append (qx-runtime lib.rs:385-398)
+    if (a->positions[i] != kv->len[seq])
+      return fail(ctx, QXC_ERR_POSITION, "KV position %d does not follow cache length %d", a->positions[i], kv->len[seq]);
+  }
+  if (*total && (!a->k || !a->v)) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+  return QXC_OK;
+}
+
 qxc_status q4_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
   Q4AppendParams p;
   p.arena = q4_arena(kv);
@@ -2744,25 +2768,8 @@ qxc_status qxc_kv_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* a) {
   return guarded(ctx, [&]() -> qxc_status {
     std::vector<int> ids, ends;
     long long total;
-    qxc_status st = check_rows(ctx, kv, a->layer_begin, a->layer_count, a->seq_count, a->seq_ids, a->positions,
-                               a->counts, &ids, &ends, &total);
-    if (st != QXC_OK) return st;
-    if (!valid_dtype(a->in_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
-    if (!a->q != !a->q_rot) return fail(ctx, QXC_ERR_INVALID_ARG, "q and q_rot go together");
-    if ((a->q_rot || a->k_rot) && !valid_dtype(a->rot_dtype)) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown tensor dtype");
-    if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0)
-      return fail(ctx, QXC_ERR_INVALID_ARG, "negative token stride");
-    std::vector<char> seen(kv->desc.sequences, 0);
-    for (int i = 0; i < a->seq_count; ++i) {
-      if (seen[ids[i]]) return fail(ctx, QXC_ERR_INVALID_ARG, "sequence %d appears twice in one call", ids[i]);
-      seen[ids[i]] = 1;
-      // KvCache::append (qx-runtime lib.rs:385-398)
-      if (a->positions[i] != kv->len[ids[i]])
-        return fail(ctx, QXC_ERR_POSITION, "KV position %d does not follow cache length %d", a->positions[i],
-                    kv->len[ids[i]]);
-    }
-    if (total == 0) return QXC_OK;
-    if (!a->k || !a->v) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+    qxc_status st = check_append(ctx, kv, a, &ids, &ends, &total);
+    if (st != QXC_OK || total == 0) return st;
     DeviceGuard device(ctx->device);
     if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
     st = ensure_pages(ctx, kv, a->seq_count, ids.data(), ends.data());
@@ -2844,11 +2851,6 @@ qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed
       return fail(ctx, QXC_ERR_INVALID_ARG, "v and out must be 16-byte aligned, v's token stride a multiple of 8");
     if (a->v_stride && a->v_stride < (long long)kv->hkv * kv->d)
       return fail(ctx, QXC_ERR_INVALID_ARG, "a token stride is shorter than a token's heads");
-    DeviceGuard device(ctx->device);
-    if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
-    const size_t qn = (size_t)total * kv->hq * kv->d, kn = (size_t)total * kv->hkv * kv->d;
-    st = reserve(ctx, &ctx->packed_rot, 2 * (qn + kn));
-    if (st != QXC_OK) return st;
     std::vector<int32_t> zeros(a->seq_count, 0);
     qxc_append_args ap;
     memset(&ap, 0, sizeof(ap));
@@ -2858,20 +2860,28 @@ qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed
     ap.seq_ids = a->seq_ids;
     ap.positions = zeros.data();
     ap.counts = a->lengths;
-    ap.q = total ? a->q : nullptr;
     ap.k = a->k;
     ap.v = a->v;
-    ap.q_rot = total ? ctx->packed_rot.ptr : nullptr;
-    ap.k_rot = total ? ctx->packed_rot.ptr + 2 * qn : nullptr;
     ap.q_stride = a->q_stride;
     ap.k_stride = a->k_stride;
     ap.v_stride = a->v_stride;
     ap.q_norm = a->q_norm;
     ap.k_norm = a->k_norm;
     ap.in_dtype = ap.rot_dtype = a->dtype;
-    ap.flags = a->flags;
-    st = qxc_kv_append(ctx, kv, &ap);
+    std::vector<int> ids, ends;
+    st = check_append(ctx, kv, &ap, &ids, &ends, &total);
     if (st != QXC_OK || total == 0) return st;
+    DeviceGuard device(ctx->device);
+    if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
+    const size_t qn = (size_t)total * kv->hq * kv->d, kn = (size_t)total * kv->hkv * kv->d;
+    st = reserve(ctx, &ctx->packed_rot, 2 * (qn + kn));
+    if (st == QXC_OK) st = ensure_pages(ctx, kv, a->seq_count, ids.data(), ends.data());
+    if (st != QXC_OK) return st;
+    ap.q = a->q;
+    ap.q_rot = ctx->packed_rot.ptr;
+    ap.k_rot = ctx->packed_rot.ptr + 2 * qn;
+    st = q4_append(ctx, kv, &ap);
+    if (st != QXC_OK) return st;
     qxc_packed_args pa;
     memset(&pa, 0, sizeof(pa));
     pa.model = kv->desc.model;
@@ -2883,7 +2893,10 @@ qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed
     pa.out = a->out;
     pa.v_stride = a->v_stride;
     pa.dtype = a->dtype;
-    return attend_packed(ctx, &pa);
+    st = attend_packed(ctx, &pa);
+    if (st == QXC_OK && !(a->flags & QXC_DECODE_NO_ADVANCE))
+      for (int i = 0; i < a->seq_count; ++i) kv->len[ids[i]] = ends[i];
+    return st;
   });
 }
 

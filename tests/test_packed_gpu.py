@@ -498,3 +498,20 @@ def test_a_prefill_without_tokens(gpu_ctx):
     assert e.value.status == _lib.ERR_POSITION
     gpu_ctx.sync()
     arena.close()
+
+
+def test_a_refused_prefill_allocates_nothing(gpu_ctx):
+    arena = KvArena(gpu_ctx, MODEL_GRANITE, 1, 8, 16, Q4)
+    q, k = (torch.zeros(8, h, 64, device="cuda", dtype=torch.bfloat16) for h in (16, 8))
+    out = torch.zeros_like(q)
+    gpu_ctx.sync()
+    for status, lengths, kw in ((_lib.ERR_POSITION, [2 ** 18] * 8, {}), (_lib.ERR_INVALID_ARG, [2 ** 18] * 8, {"layer": 1}),
+                                (_lib.ERR_INVALID_ARG, [2 ** 18] * 8, {"seq_ids": [0] * 8})):
+        free = torch.cuda.mem_get_info()[0]
+        with pytest.raises(QxError) as e:
+            arena.prefill_packed(q, k, k, out, lengths, **kw)
+        assert torch.cuda.mem_get_info()[0] == free
+        assert e.value.status in (status, _lib.ERR_POSITION)
+    arena.prefill_packed(q, k, k, out, [1] * 8)
+    gpu_ctx.sync()
+    arena.close()
