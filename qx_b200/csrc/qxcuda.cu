@@ -1045,9 +1045,16 @@ qxc_status reserve(qxc_ctx* ctx, Workspace* w, size_t bytes) {
   if (capture != cudaStreamCaptureStatusNone)
     return fail(ctx, QXC_ERR_UNSUPPORTED, "a workspace of %zu bytes is needed: make the call once before its capture",
                 bytes);
-  const size_t want = std::max(bytes, 2 * w->bytes);
+  // twice the last one, so that it grows a few times only, where there is room for it
+  size_t want = std::max(bytes, 2 * w->bytes);
   void* p = nullptr;
-  QXC_CUDA(ctx, cudaMalloc(&p, want));
+  ctx->outgrown.reserve(ctx->outgrown.size() + 1);
+  if (want > bytes && cudaMalloc(&p, want) != cudaSuccess) {
+    cudaGetLastError();
+    p = nullptr;
+    want = bytes;
+  }
+  if (!p) QXC_CUDA(ctx, cudaMalloc(&p, want));
   if (w->ptr) ctx->outgrown.push_back(w->ptr);
   w->ptr = static_cast<char*>(p);
   w->bytes = want;

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 import q4_reference as ref
-from qx_b200 import BF16, F16, F32, MODEL_GRANITE, MODEL_QWEN3, Q4, KvArena, QxError, _lib
+from qx_b200 import BF16, F16, F32, MODEL_GRANITE, MODEL_QWEN3, Q4, Context, KvArena, QxError, _lib
 from qx_b200.runtime import model_shape
 from test_q4_gpu import check_decode, host, norms, stored, tensor
 
@@ -515,3 +515,33 @@ def test_a_refused_prefill_allocates_nothing(gpu_ctx):
     arena.prefill_packed(q, k, k, out, [1] * 8)
     gpu_ctx.sync()
     arena.close()
+
+
+def test_a_workspace_grows_to_what_is_asked_where_more_does_not_fit():
+    """With less than twice the last workspace free, a slightly larger call still runs."""
+    rng = np.random.default_rng(36)
+    ctx = Context(0)
+    lengths = [256] * 500  # 128000 tokens, 3 KB of workspace each
+    arena = KvArena(ctx, MODEL_GRANITE, 1, 500, 256, Q4)
+    q, k, v = inputs(rng, MODEL_GRANITE, sum(lengths), BF16)
+    out = torch.zeros_like(q)
+    go = lambda n: arena.prefill_packed(q, k, v, out, lengths[:n], flags=_lib.DECODE_NO_ADVANCE)  # noqa: E731
+    ctx.attend_packed(MODEL_GRANITE, q, k, v, out, lengths)  # what a first launch loads
+    ctx.sync()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    hog = torch.empty(torch.cuda.mem_get_info()[0] - 950_000_000, dtype=torch.uint8, device="cuda")
+    try:
+        go(440)
+        ctx.sync()
+        assert torch.cuda.mem_get_info()[0] < 2 * 440 * 256 * 3072
+        go(500)
+        ctx.sync()
+    finally:
+        del hog
+        torch.cuda.empty_cache()
+    (_, _), (vc, vs) = stored(arena, 499, 0, 0, 256)
+    want = ref.quantise(v[-256:].float().cpu().numpy())
+    assert np.array_equal(vc, want[0]) and np.array_equal(vs, want[1])
+    arena.close()
+    ctx.close()
