@@ -186,9 +186,11 @@ qxc_status fail(qxc_ctx* ctx, qxc_status st, const char* fmt, ...) {
 #define QXC_CUDA(ctx, call)                                                                          \
   do {                                                                                               \
     cudaError_t e_ = (call);                                                                         \
-    if (e_ != cudaSuccess)                                                                           \
+    if (e_ != cudaSuccess) {                                                                         \
+      cudaGetLastError(); /* reported here, not by the next launch's check too */                    \
       return fail((ctx), e_ == cudaErrorMemoryAllocation ? QXC_ERR_OUT_OF_MEMORY : QXC_ERR_CUDA,     \
                   "%s: %s", #call, cudaGetErrorString(e_));                                          \
+    }                                                                                                \
   } while (0)
 
 size_t dtype_size(int dt) { return dt == QXC_F32 ? 4 : 2; }
@@ -1574,6 +1576,7 @@ static qxc_status kv_create(qxc_ctx* ctx, const qxc_kv_desc* desc, const qxc_kv_
     if (e != cudaSuccess) cudaFree(kv->base);
   }
   if (e != cudaSuccess) {
+    cudaGetLastError();
     delete kv;
     return fail(ctx, e == cudaErrorMemoryAllocation ? QXC_ERR_OUT_OF_MEMORY : QXC_ERR_CUDA,
                 "KV arena of %zu bytes: %s", koff_v + vbytes, cudaGetErrorString(e));

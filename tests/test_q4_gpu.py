@@ -808,3 +808,19 @@ def test_a_refused_capture_maps_no_page():
     check_decode(ctx, arena, q, k, v, out, [64, 64], F32)
     arena.close()
     ctx.close()
+
+
+def test_an_allocation_that_fails_is_reported_once():
+    """An arena larger than the GPU is refused; the arenas, pages and steps after it are not."""
+    rng = np.random.default_rng(37)
+    for model in MODELS:
+        ctx = Context(0)
+        for page in (0, 64):
+            with pytest.raises(QxError) as e:
+                KvArena(ctx, model, 48, 4000, 4096, Q4, page_size=page, pool_pages=200000)
+            assert e.value.status == _lib.ERR_OUT_OF_MEMORY
+            arena = KvArena(ctx, model, 1, 1, 70, Q4, page_size=page, pool_pages=2)
+            fill(ctx, arena, rng, [66])
+            run_decode(ctx, arena, rng, [66], BF16, F32)
+            arena.close()
+        ctx.close()
