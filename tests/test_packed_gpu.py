@@ -545,3 +545,39 @@ def test_a_workspace_grows_to_what_is_asked_where_more_does_not_fit():
     assert np.array_equal(vc, want[0]) and np.array_equal(vs, want[1])
     arena.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_rows_computed_again_attend_every_token(gpu_ctx, model):
+    """The rows that share a tile with a bad value at the end of a long prompt, against 64
+    bits. Nearly all of their weight is on 16 tokens, at the ends of the prompt and around
+    the borders of the stretches that the recomputation takes, each with dims of its own:
+    one left out or counted twice is off by all of its output."""
+    n = 140001
+    hq, hkv, d = model_shape(model)
+    gen = torch.Generator(device="cuda").manual_seed(38)
+    q, k, v = (torch.randn(n, h, d, device="cuda", generator=gen).bfloat16() for h in (hq, hkv, hkv))
+    hot = [0, 1, 31, 32, 63, 64, 4095, 4096, 65535, 65536, 70001, 131071, n - 400, n - 257, n - 160, n - 140]
+    q[:, :, 0] = 8.0
+    k[:, :, 0] = 0.0
+    k[hot, :, 0] = 100.0 if model == MODEL_GRANITE else 18.0  # a logit of 12.5: 2.7e5 times the others' weight
+    for i, t in enumerate(hot):
+        v[t] = 0.0
+        v[t, :, i::16] = 8.0
+    v[n - 1] = float("nan")
+    out = torch.zeros_like(q)
+    gpu_ctx.attend_packed(model, q, k, v, out, [n])
+    with pytest.raises(QxError) as e:
+        gpu_ctx.sync()
+    assert e.value.status == _lib.ERR_NONFINITE and torch.isnan(out[n - 1]).all()
+    rows = torch.arange(n - 1 - n % 128 - 20, n - 1, device="cuda")  # the key tile of the bad value, and some before it
+    later = torch.arange(n - 1, device="cuda") > rows[:, None]
+    for h in (0, hq // 2 + 1, hq - 1):
+        kd, vd = k[:n - 1, h * hkv // hq].double(), v[:n - 1, h * hkv // hq].double()
+        qd = q[rows, h].double()
+        p = torch.softmax((qd @ kd.T * ref.SCALE[model]).masked_fill(later, -torch.inf), -1)
+        want, mean = p @ vd, p @ vd.abs()
+        assert float(want.abs().amax(1).min()) > 0.3  # a token's share
+        size = (qd.abs() @ kd.abs().T).masked_fill(later, 0).amax(-1, keepdim=True) * ref.SCALE[model]
+        rel = 2 * size * (d + 2) * 2.0 ** -24 + ref.HALF_STEP[BF16] + 2.0 ** -13 + n * 2.0 ** -24
+        assert float(((out[rows, h].double() - want).abs() / (ref.HALF_STEP[BF16] * want.abs() + rel * mean)).max()) <= 1
