@@ -154,7 +154,12 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
  * any arena, qxc_decode reads and writes it (with the hardware exponential;
  * its workspace grows with sequences and layers, and a call that grows it
  * cannot be captured: QXC_ERR_UNSUPPORTED), qxc_attention_layer and
- * qxc_attention_stack run on it through qxc_decode. The verify, partials,
+ * qxc_attention_stack run on it through qxc_decode. Its roundings follow the
+ * output's type: for bf16 a rotated query head is rounded to integers of 15
+ * bits against its largest element (off by up to 2^-14.97 of that: scores of
+ * hundreds that hang on small elements beside a far larger one want another
+ * output type), for f16 and f32 to 29; a weight enters its product with the
+ * values in fp16, for f32 in two fp16 terms. The verify, partials,
  * exchange, prefill and hash calls return QXC_ERR_UNSUPPORTED. A value beyond
  * 7 * 65504, an infinity or a NaN in a new row is reported by qxc_sync
  * (QXC_ERR_NONFINITE); what that row then holds is unspecified. */
@@ -496,7 +501,8 @@ qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* args);
  * another: token i of a prompt attends tokens 0..i of the same prompt, softmax
  * scale and head layout of `model`. q and k are already rotated. bf16 or f16
  * in and out, f32 scores, softmax and accumulation (the weights of one key
- * tile are rounded to the input type for their product with the values).
+ * tile are rounded to the input type for their product with the values; an
+ * exponential is off by up to 2^-13 of itself).
  * lengths may be 0; at most 2^18 tokens a prompt and 2^24 together. Each tensor is [tokens][heads *
  * head_dim], 16-byte aligned, with token strides in elements that are
  * multiples of 8 (0 = dense): q, k and v may be parts of one joint projection.

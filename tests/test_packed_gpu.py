@@ -581,3 +581,22 @@ def test_rows_computed_again_attend_every_token(gpu_ctx, model):
         size = (qd.abs() @ kd.abs().T).masked_fill(later, 0).amax(-1, keepdim=True) * ref.SCALE[model]
         rel = 2 * size * (d + 2) * 2.0 ** -24 + ref.HALF_STEP[BF16] + 2.0 ** -13 + n * 2.0 ** -24
         assert float(((out[rows, h].double() - want).abs() / (ref.HALF_STEP[BF16] * want.abs() + rel * mean)).max()) <= 1
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_a_bad_value_at_the_end_of_the_longest_prompt(gpu_ctx, model):
+    """2^18 tokens, the most a prompt may have: no wait for the recomputed rows runs out
+    (which would be another status), and the rows before its tile are as without it."""
+    n = 2 ** 18
+    hq, hkv, d = model_shape(model)
+    gen = torch.Generator(device="cuda").manual_seed(40)
+    q, k, v = (torch.randn(n, h, d, device="cuda", generator=gen).bfloat16() for h in (hq, hkv, hkv))
+    clean = attend(gpu_ctx, model, q, k, v, [n], BF16)
+    v[n - 1] = float("nan")
+    out = torch.zeros_like(q)
+    gpu_ctx.attend_packed(model, q, k, v, out, [n])
+    with pytest.raises(QxError) as e:
+        gpu_ctx.sync()
+    assert e.value.status == _lib.ERR_NONFINITE
+    assert torch.isnan(out[n - 1]).all() and torch.isfinite(out[:n - 1]).all()
+    assert torch.equal(out[:n - 128], clean[:n - 128])

@@ -824,3 +824,33 @@ def test_an_allocation_that_fails_is_reported_once():
             run_decode(ctx, arena, rng, [66], BF16, F32)
             arena.close()
         ctx.close()
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q_scale,loud", [(1.0, 1.0), (1.0, 30.0), (40.0, 1.0)])
+def test_decode_peaked_scores_into_bf16(gpu_ctx, model, dtype, q_scale, loud):
+    """For a bf16 output a query head's elements are rounded to multiples of its largest /
+    16128, off by half of that: a logit by up to that times the sum of a key's |elements|,
+    twice in a weight (its own and the sum's)."""
+    rng = np.random.default_rng([model, dtype, 39])
+    arena = make_arena(gpu_ctx, model, [301])
+    fill(gpu_ctx, arena, rng, [300], scale=3.0)
+    hq, hkv, d = model_shape(model)
+    q, k, v = (tensor(rng, (1, 1, h, d), dtype) for h in (hq, hkv, hkv))
+    q[..., 9] *= loud
+    qw = torch.full((128,), q_scale, device="cuda") if model == MODEL_QWEN3 else None  # (its norm undoes q's own scale)
+    q = q if model == MODEL_QWEN3 else q * q_scale
+    out = torch.zeros(1, 1, hq, d, device="cuda", dtype=torch.bfloat16)
+    arena.decode(q, k, v, out, [300], q_dtype=dtype, in_dtype=dtype, out_dtype=BF16, q_norm=qw)
+    gpu_ctx.sync()
+    (kc, ks), (vc, vs) = stored(arena, 0, 0, 0, 301)
+    keys, vals = ref.values(kc, ks), ref.values(vc, vs)
+    qr = ref.rotate64(model, host(q[0, 0])[None], [300], None if qw is None else host(qw))[0]
+    want, mean = ref.attend64(model, qr, keys, vals)
+    size = np.repeat(np.abs(keys).sum(-1).max(0), hq // hkv)  # of each query head's keys
+    logit = np.abs(qr).max(-1) / 16128 / 2 * size * ref.SCALE[model] + ref.logit_error(model, qr, keys, 76)
+    weights = np.expm1(2 * logit)[:, None] + 2.0 ** -20 + 2.0 ** -11
+    tol = ref.HALF_STEP[BF16] * np.abs(want) + weights * mean + 301 * 2.0 ** -31 * 7 * vs.astype(np.float64).max()
+    assert ref.close(host(out[0, 0]), want, tol) <= 1
+    arena.close()
