@@ -682,10 +682,13 @@ __global__ void __launch_bounds__(kThreads, 2) qx_q4_decode_kernel(const __grid_
 // Cells shared by CTAs: a CTA joins 1024 / SHARES outputs of a cell, SHARES
 // threads (of neighbouring 256 / SHARES) taking every SHARES-th part of the same
 // four. One share where cells have few parts, 32 (then 32 dims of one head)
-// where they have many: up to 8 parts, or more, of a cell. Always one against always
-// 32, the decode as a whole: 48 sequences of 2 to 7 parts 68.5 | 95.3 us, 128
-// sequences of 2 or 3 120.8 | 149.3, 2000 rows in 32 parts 14.7 | 9.3, 32768 rows in
-// 147 parts 42.2 | 14.2.
+// where they have many: more than 8 of a Granite cell, 16 of a Qwen3 one, whose 128
+// CTAs a cell then cost more. Always one against always 32, the decode as a whole in us:
+//   Granite  128 sequences of 2 or 3 parts 120.8 | 149.3; 40 of 9 25.6 | 26.2, 36 of 9
+//            25.3 | 25.1, 28 of 12 22.2 | 21.1, 20 of 15 19.8 | 16.3, 8 of 19 15.6 | 12.7
+//   Qwen3    48 of 2 to 7 68.5 | 95.3; 40 of 9 30.9 | 41.6, 28 of 12 25.1 | 30.9, 20 of
+//            16 52.2 | 55.0, 12 of 17 21.2 | 21.2, 8 of 19 18.8 | 16.7, 10 of 31 36.9 |
+//            31.5, one of 32 14.7 | 9.3, of 147 42.2 | 14.2
 template <class M, int SHARES>
 __global__ void __launch_bounds__(256) qx_q4_merge_kernel(const __grid_constant__ Q4DecodeParams p) {
   constexpr int E = 1024 / SHARES, SLICES = M::HQ * M::D / E, LANES = 256 / SHARES;
@@ -780,7 +783,7 @@ cudaError_t decode(const Q4DecodeParams& p, cudaStream_t stream, int* launched) 
   if (e == cudaSuccess) e = launch_dependent(qx_q4_decode_kernel<M, OUT>, ctas, kThreads, Dec<M>::SMEM, stream, p, launched);
   if (e != cudaSuccess || p.max_parts == 1) return e;
   constexpr int OUTPUTS = M::HQ * M::D;
-  if (p.max_parts <= 8)
+  if (p.max_parts <= (M::QWEN ? 16 : 8))
     return launch_dependent(qx_q4_merge_kernel<M, 1>, cells * (OUTPUTS / 1024), 256, 0, stream, p, launched);
   return launch_dependent(qx_q4_merge_kernel<M, 32>, cells * (OUTPUTS / 32), 256, 0, stream, p, launched);
 }

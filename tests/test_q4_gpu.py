@@ -854,3 +854,16 @@ def test_decode_peaked_scores_into_bf16(gpu_ctx, model, dtype, q_scale, loud):
     tol = ref.HALF_STEP[BF16] * np.abs(want) + weights * mean + 301 * 2.0 ** -31 * 7 * vs.astype(np.float64).max()
     assert ref.close(host(out[0, 0]), want, tol) <= 1
     arena.close()
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("parts", [2, 7, 8, 9, 12, 16, 17, 18, 33])
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+def test_decode_joins_any_number_of_parts(gpu_ctx, model, parts, out_dtype):
+    """On both sides of the numbers from which on several threads share an output's parts."""
+    rng = np.random.default_rng([model, parts])
+    rows = [64 * parts - 3, 64 * (parts - 1), 1, 64 * parts - 64 + 5]
+    arena = make_arena(gpu_ctx, model, [n + 1 for n in rows], layers=2)
+    fill(gpu_ctx, arena, rng, rows)
+    run_decode(gpu_ctx, arena, rng, rows, BF16, out_dtype, split=64)
+    arena.close()
