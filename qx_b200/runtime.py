@@ -88,7 +88,7 @@ def _ints(values):
     return a, a.buffer_info()[0]
 
 
-_float_types = {}  # of torch, their qxc_dtype (filled by the first tensor that is checked)
+_torch_types = {}  # torch's type of a qxc_dtype (filled by the first tensor that is checked)
 
 
 def _16bit(dtype: int):
@@ -100,7 +100,14 @@ def _operand(x, dtype: int | None, device: int):
     """The pointer of a tensor of `dtype` on `device` (page-locked host memory is
     the device's too; an integer type of the same size may hold it); a raw
     pointer as it is. A type that no tensor has is left to the call to refuse."""
-    if x is None or isinstance(x, int):
+    if x is None or type(x) is int:
+        return x
+    try:
+        if x.dtype is _torch_types[dtype] and x.get_device() == device:
+            return x.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    if isinstance(x, int):
         return x
     if isinstance(x, np.ndarray):
         raise QxError(_lib.ERR_INVALID_ARG, "a host array where a device tensor is needed")
@@ -108,10 +115,11 @@ def _operand(x, dtype: int | None, device: int):
         at, kind, size = x.get_device(), x.dtype, x.element_size()
     except AttributeError:  # no tensor
         return _ptr(x)
-    if not _float_types:
+    if not _torch_types:
         import torch
-        _float_types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
-    if dtype in (F32, BF16, F16) and (_float_types.get(kind, dtype) != dtype or size != (4 if dtype == F32 else 2)):
+        _torch_types.update({F32: torch.float32, BF16: torch.bfloat16, F16: torch.float16})
+    if dtype in _torch_types and kind is not _torch_types[dtype] and (
+            kind in _torch_types.values() or size != (4 if dtype == F32 else 2)):
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {kind}, another type than the call's ({dtype})")
     if at != device and not (at < 0 and x.is_pinned()):
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor on {x.device}, the context is on device {device}")
@@ -120,12 +128,14 @@ def _operand(x, dtype: int | None, device: int):
 
 def _room(x, elements: int, dtype: int | None, device: int):
     """_operand for a dense tensor of at least `elements` elements."""
+    if x is None or type(x) is int:
+        return x
     ptr = _operand(x, dtype, device)
     try:
-        held = x.numel()
+        held, dense = x.numel(), x.is_contiguous()
     except AttributeError:  # no tensor
         return ptr
-    if not x.is_contiguous():
+    if not dense:
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor must be dense: shape {tuple(x.shape)}, strides {x.stride()}")
     if held < elements:
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {held} elements, {elements} needed")
@@ -136,10 +146,11 @@ def _token_stride(x, features: int, tokens: int = 0) -> int:
     """Elements between the tokens of a tensor [tokens, ...], `tokens` of them
     at least, whose remaining dimensions are dense and hold `features`
     elements; 0 (dense) for a raw pointer."""
-    if x is None or isinstance(x, int):
+    if x is None or type(x) is int:
         return 0
     try:
-        held = x.shape[0] if x.dim() else 0
+        shape = x.shape
+        held = shape[0] if shape else 0
         plain = x.is_contiguous() and x.numel() == held * features
     except AttributeError:  # no tensor
         return 0
@@ -147,7 +158,7 @@ def _token_stride(x, features: int, tokens: int = 0) -> int:
         raise QxError(_lib.ERR_INVALID_ARG, f"a tensor of {held} tokens, {tokens} needed")
     if plain:
         return features if held > 1 else 0
-    shape, stride, dense = x.shape, x.stride(), 1
+    stride, dense = x.stride(), 1
     for i in range(len(shape) - 1, 0, -1):
         if shape[i] != 1 and stride[i] != dense:
             raise QxError(_lib.ERR_INVALID_ARG, f"the heads of a token must be dense: strides {stride}")
