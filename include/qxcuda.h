@@ -175,7 +175,9 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
  * advance by counts unless QXC_DECODE_NO_ADVANCE. Device pointers of any
  * element alignment (16-byte aligned ones are read and written faster);
  * asynchronous. q and q_rot may both be NULL (keys and values only), k_rot may
- * be NULL. q_rot may be q itself, and k_rot k, where type and layout are the same. */
+ * be NULL. q_rot may be q itself, and k_rot k, where type and layout are the
+ * same; an output that overlaps anything else of the call is refused
+ * (QXC_ERR_INVALID_ARG). */
 typedef struct qxc_append_args {
   int32_t layer_begin;
   int32_t layer_count;
@@ -506,8 +508,8 @@ qxc_status qxc_prefill(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_args* args);
  * lengths may be 0; at most 2^18 tokens a prompt and 2^24 together. Each tensor is [tokens][heads *
  * head_dim], 16-byte aligned, with token strides in elements that are
  * multiples of 8 (0 = dense): q, k and v may be parts of one joint projection.
- * Rows of `out` past the last prompt are not written; `out` must not overlap
- * an input. What a row that attends a NaN or an infinity holds is unspecified
+ * Rows of `out` past the last prompt are not written; an `out` that overlaps
+ * an input is refused (QXC_ERR_INVALID_ARG). What a row that attends a NaN or an infinity holds is unspecified
  * in every dim that it can reach (all of them from a query or a key, its own
  * from a value); a row that is not finite is reported by qxc_sync
  * (QXC_ERR_NONFINITE). Rows that do not attend it are unaffected. The weights

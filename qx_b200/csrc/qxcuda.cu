@@ -1065,6 +1065,21 @@ qxc_status reserve(qxc_ctx* ctx, Workspace* w, size_t bytes) {
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// A tensor of a call: `tokens` rows of `row` bytes, `stride` bytes apart.
+struct Span {
+  const void* ptr;
+  long long tokens, row, stride;
+  // May it share memory with `o`? (Whole spans are compared: none lies between another's rows.)
+  bool meets(const Span& o) const {
+    if (!ptr || !o.ptr || tokens < 1 || o.tokens < 1) return false;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(ptr), b = reinterpret_cast<uintptr_t>(o.ptr);
+    return a < b + (uintptr_t)((o.tokens - 1) * o.stride + o.row) && b < a + (uintptr_t)((tokens - 1) * stride + row);
+  }
+  bool same(const Span& o) const {
+    return ptr == o.ptr && row == o.row && (tokens == 1 || stride == o.stride);
+  }
+};
+
 Q4Arena q4_arena(const qxc_kv* kv) {
   Q4Arena a;
   a.k = kv->k_region;
@@ -1159,6 +1174,19 @@ qxc_status check_append(qxc_ctx* ctx, const qxc_kv* kv, const qxc_append_args* a
       return fail(ctx, QXC_ERR_POSITION, "KV position %d does not follow cache length %d", a->positions[i], kv->len[seq]);
   }
   if (*total && (!a->k || !a->v)) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+  // rows are read and written by different warps in any order: an output may be an
+  // input only where each warp writes what it has read itself
+  const long long in = (long long)dtype_size(a->in_dtype), rot = (long long)dtype_size(a->rot_dtype);
+  const long long qn = (long long)a->layer_count * kv->hq * kv->d, kn = (long long)a->layer_count * kv->hkv * kv->d;
+  auto input = [&](const void* p, long long n, long long stride) {
+    return Span{p, *total, n * in, (stride ? stride : n) * in};
+  };
+  const Span q = input(a->q, qn, a->q_stride), k = input(a->k, kn, a->k_stride), v = input(a->v, kn, a->v_stride);
+  const Span q_rot{a->q_rot, *total, qn * rot, qn * rot}, k_rot{a->k_rot, *total, kn * rot, kn * rot};
+  if ((q_rot.meets(q) && !(q_rot.same(q) && in == rot)) || (k_rot.meets(k) && !(k_rot.same(k) && in == rot)) ||
+      q_rot.meets(k) || q_rot.meets(v) || k_rot.meets(q) || k_rot.meets(v) || q_rot.meets(k_rot))
+    return fail(ctx, QXC_ERR_INVALID_ARG, "q_rot or k_rot overlaps another tensor of the call, or its own input otherwise "
+                                          "than in place");
   return QXC_OK;
 }
 
@@ -1341,6 +1369,12 @@ qxc_status attend_packed(qxc_ctx* ctx, const qxc_packed_args* a) {
     return fail(ctx, QXC_ERR_INVALID_ARG, "packed tensors must be 16-byte aligned, their token strides multiples of 8");
   if (p.q_stride < (long long)hq * d || p.k_stride < (long long)hkv * d || p.v_stride < (long long)hkv * d)
     return fail(ctx, QXC_ERR_INVALID_ARG, "a token stride is shorter than a token's heads");
+  long long total = 0;
+  for (int i = 0; i < a->seq_count; ++i) total += a->lengths[i];
+  const Span out{a->out, total, 2ll * hq * d, 2ll * hq * d};
+  if (out.meets({a->q, total, 2ll * hq * d, 2 * p.q_stride}) || out.meets({a->k, total, 2ll * hkv * d, 2 * p.k_stride}) ||
+      out.meets({a->v, total, 2ll * hkv * d, 2 * p.v_stride}))
+    return fail(ctx, QXC_ERR_INVALID_ARG, "out overlaps an input");
   if (!ctx->packed_set) {
     QXC_CUDA(ctx, setup_packed());
     ctx->packed_set = true;
@@ -2805,6 +2839,9 @@ qxc_status qxc_kv_read_rows(qxc_ctx* ctx, qxc_kv* kv, const qxc_read_rows_args* 
                     ends[i], kv->mapped[ids[i]], 1 << kv->page_shift);
     if (total == 0) return QXC_OK;
     if (!a->key_out && !a->value_out) return fail(ctx, QXC_ERR_INVALID_ARG, "null tensor pointer");
+    const long long row = (long long)a->layer_count * kv->hkv * kv->d * (long long)dtype_size(a->out_dtype);
+    if (Span{a->key_out, total, row, row}.meets({a->value_out, total, row, row}))
+      return fail(ctx, QXC_ERR_INVALID_ARG, "key_out overlaps value_out");
     DeviceGuard device(ctx->device);
     if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
     Q4ReadParams p;
@@ -2881,6 +2918,9 @@ qxc_status qxc_prefill_packed(qxc_ctx* ctx, qxc_kv* kv, const qxc_prefill_packed
     std::vector<int> ids, ends;
     st = check_append(ctx, kv, &ap, &ids, &ends, &total);
     if (st != QXC_OK || total == 0) return st;
+    const long long out_row = 2ll * kv->hq * kv->d, v_row = 2ll * kv->hkv * kv->d;
+    if (Span{a->out, total, out_row, out_row}.meets({a->v, total, v_row, a->v_stride ? 2 * a->v_stride : v_row}))
+      return fail(ctx, QXC_ERR_INVALID_ARG, "out overlaps v");
     DeviceGuard device(ctx->device);
     if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
     const size_t qn = (size_t)total * kv->hq * kv->d, kn = (size_t)total * kv->hkv * kv->d;

@@ -867,3 +867,41 @@ def test_decode_joins_any_number_of_parts(gpu_ctx, model, parts, out_dtype):
     fill(gpu_ctx, arena, rng, rows)
     run_decode(gpu_ctx, arena, rng, rows, BF16, out_dtype, split=64)
     arena.close()
+
+
+def test_overlapping_tensors_are_refused(gpu_ctx):
+    """Warps read inputs and write outputs in any order, so only an output in its own
+    input's place is written by the warp that has read it."""
+    arena = KvArena(gpu_ctx, MODEL_GRANITE, 1, 1, 64, Q4)
+    joint = torch.zeros(10, 32, 64, device="cuda", dtype=torch.bfloat16)
+    q, k, v = joint[:, :16], joint[:, 16:24], joint[:, 24:]
+    dq, dk, dv = (x.clone() for x in (q, k, v))
+    flat = joint.view(-1)
+    inside, behind = flat[:10 * 1024].view(10, 16, 64), torch.zeros(10, 16, 64, device="cuda", dtype=torch.bfloat16)
+
+    def refused(call):
+        launches = gpu_ctx.launch_count
+        with pytest.raises(QxError, match="overlap") as e:
+            call()
+        assert e.value.status == _lib.ERR_INVALID_ARG and gpu_ctx.launch_count == launches
+    append = lambda q, k, v, **kw: arena.append(q, k, v, [0], [10], in_dtype=BF16, flags=DECODE_NO_ADVANCE, **kw)  # noqa: E731
+    refused(lambda: append(q, k, v, q_rot=inside))
+    refused(lambda: append(None, k, v, k_rot=flat[-5120:].view(10, 8, 64)))
+    refused(lambda: append(dq, dk, dv, q_rot=dq.view(-1), k_rot=dv))
+    refused(lambda: append(dq, dk, dv, q_rot=behind, k_rot=behind.view(-1)[5120:]))
+    refused(lambda: append(dq, dk, dk.view(10, 8, 64), q_rot=behind, k_rot=dk))
+    refused(lambda: append(dq, dk, dv, q_rot=dq.data_ptr(), rot_dtype=F32))
+    refused(lambda: arena.read_rows(dk, dk, [0], [10], out_dtype=BF16))
+    refused(lambda: arena.read_rows(behind.view(-1)[8:], behind, [0], [9], out_dtype=BF16))
+    refused(lambda: gpu_ctx.attend_packed(MODEL_GRANITE, q, k, v, inside, [10]))
+    refused(lambda: gpu_ctx.attend_packed(MODEL_GRANITE, dq, dk, dv, dq, [10]))
+    refused(lambda: arena.prefill_packed(dq, dk, behind[:, :8], behind, [10]))
+    append(dq, dk, dv, q_rot=dq, k_rot=dk)
+    append(q, k, v, q_rot=dq, k_rot=dk)
+    arena.read_rows(dk, dv, [0], [10], out_dtype=BF16)
+    arena.read_rows(flat[:512], flat[512:], [0], [1], out_dtype=BF16)
+    gpu_ctx.attend_packed(MODEL_GRANITE, q, k, v, behind, [10])
+    gpu_ctx.attend_packed(MODEL_GRANITE, behind[:4], k, v, behind[4:], [4])
+    arena.prefill_packed(dq, dk, dv, dq, [10])  # its rotated queries are copies
+    gpu_ctx.sync()
+    arena.close()
