@@ -152,6 +152,10 @@ struct qxc_kv {
   std::vector<int> table;
   std::vector<int> mapped;
   std::vector<int> free_pages;  // a stack: the next page to hand out is at the back
+  // table entries that only captured work has sent (the last capture is unsent_by): the
+  // device lacks them until its graph runs, for good if it never does
+  std::vector<int> unsent;
+  unsigned long long unsent_by = 0;
   bool paged() const { return page_shift != 0; }
   int pages_for(long long rows) const { return (int)((rows + (1ll << page_shift) - 1) >> page_shift); }
 };
@@ -866,30 +870,52 @@ qxc_status push_table(qxc_ctx* ctx, qxc_kv* kv, const std::vector<int>& idx, con
   return QXC_OK;
 }
 
+// Send the block table's entries `fresh`, and those that only another capture's graph
+// holds (it may run later than this call's work, or never). What is sent under capture
+// stays on that list until a call sends it eagerly.
+qxc_status send_entries(qxc_ctx* ctx, qxc_kv* kv, const std::vector<int>& fresh) {
+  if (fresh.empty() && kv->unsent.empty()) return QXC_OK;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  QXC_CUDA(ctx, cudaStreamGetCaptureInfo(ctx->stream, &capture, &id));
+  const bool capturing = capture != cudaStreamCaptureStatusNone;
+  std::vector<int> idx = fresh, val;
+  if (!capturing || id != kv->unsent_by)
+    for (int e : kv->unsent)
+      if (kv->table[e] >= 0) idx.push_back(e);  // not released since
+  for (int e : idx) val.push_back(kv->table[e]);
+  if (capturing) {
+    if (id != kv->unsent_by) kv->unsent.clear();
+    kv->unsent.insert(kv->unsent.end(), idx.begin(), idx.end());
+    kv->unsent_by = id;
+  } else {
+    kv->unsent.clear();
+  }
+  return push_table(ctx, kv, idx, val);
+}
+
 // Map pages so that rows [0, rows[i]) of sequence seqs[i] exist, all or
 // nothing: when the pool cannot cover every request, nothing is mapped.
 qxc_status ensure_pages(qxc_ctx* ctx, qxc_kv* kv, int n, const int* seqs, const int* rows) {
   if (!kv->paged()) return QXC_OK;
   long long need = 0;
   for (int i = 0; i < n; ++i) need += std::max(0, kv->pages_for(rows[i]) - kv->mapped[seqs[i]]);
-  if (need == 0) return QXC_OK;
   if (need > (long long)kv->free_pages.size())
     return fail(ctx, QXC_ERR_OUT_OF_MEMORY, "KV page pool exhausted: %lld more pages needed, %zu of %d free", need,
                 kv->free_pages.size(), kv->pool_pages);
-  std::vector<int> idx, val;
-  for (int i = 0; i < n; ++i) {
+  std::vector<int> fresh;
+  for (int i = 0; need && i < n; ++i) {
     const int seq = seqs[i], want = kv->pages_for(rows[i]);
     while (kv->mapped[seq] < want) {
       const int page = kv->free_pages.back();
       kv->free_pages.pop_back();
       const int e = seq * kv->table_stride + kv->mapped[seq];
       kv->table[e] = page;
-      idx.push_back(e);
-      val.push_back(page);
+      fresh.push_back(e);
       kv->mapped[seq]++;
     }
   }
-  return push_table(ctx, kv, idx, val);
+  return send_entries(ctx, kv, fresh);
 }
 
 // Return the pages of `seq` past its first `keep` logical pages to the pool.
@@ -2844,6 +2870,8 @@ qxc_status qxc_kv_read_rows(qxc_ctx* ctx, qxc_kv* kv, const qxc_read_rows_args* 
       return fail(ctx, QXC_ERR_INVALID_ARG, "key_out overlaps value_out");
     DeviceGuard device(ctx->device);
     if (!device.ok) return fail(ctx, QXC_ERR_CUDA, "cannot make device %d current", ctx->device);
+    st = send_entries(ctx, kv, {});
+    if (st != QXC_OK) return st;
     Q4ReadParams p;
     p.arena = q4_arena(kv);
     p.layer_begin = a->layer_begin;
@@ -2979,6 +3007,8 @@ qxc_status qxc_verification_hashes(qxc_ctx* ctx, qxc_kv* kv, const qxc_verificat
   p.checkpoint_interval = a->checkpoint_interval;
   p.out = a->digests;
   QXC_CUDA(ctx, cudaSetDevice(ctx->device));
+  st = send_entries(ctx, kv, {});
+  if (st != QXC_OK) return st;
   return launch_hash(ctx, p, (layers + 1 + kHashWarps - 1) / kHashWarps);
 }
 
@@ -3010,6 +3040,8 @@ qxc_status qxc_kv_slot_hashes(qxc_ctx* ctx, qxc_kv* kv, int32_t seq, int32_t lay
   if (slots > (1ll << 31) - 1) return fail(ctx, QXC_ERR_INVALID_ARG, "too many slots");
   if (flags < QXC_HASH_AUTO || flags > QXC_HASH_PER_SLOT) return fail(ctx, QXC_ERR_INVALID_ARG, "unknown hash flags");
   QXC_CUDA(ctx, cudaSetDevice(ctx->device));
+  st = send_entries(ctx, kv, {});
+  if (st != QXC_OK) return st;
   // a lane pair per slot once the range gives every SM at least 8 full warps
   bool serial = flags == QXC_HASH_PER_SLOT;
   if (flags == QXC_HASH_AUTO) serial = slots >= 16ll * 8 * ctx->sm_count;

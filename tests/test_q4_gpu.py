@@ -905,3 +905,52 @@ def test_overlapping_tensors_are_refused(gpu_ctx):
     arena.prefill_packed(dq, dk, dv, dq, [10])  # its rotated queries are copies
     gpu_ctx.sync()
     arena.close()
+
+
+def test_pages_mapped_by_a_capture_that_is_thrown_away(gpu_ctx):
+    """The device gets their table entries from the next call that runs, also one that only reads."""
+    rng = np.random.default_rng(41)
+    hkv, d = model_shape(MODEL_QWEN3)[1:]
+    old, stream = gpu_ctx.stream, torch.cuda.Stream()
+    k, v = (tensor(rng, (300, hkv, d), BF16) for _ in range(2))
+    torch.cuda.synchronize()
+    graphs = []  # kept: one that goes while another is captured ends that capture
+    for first in ("append", "read", "decode", "capture"):
+        graphs += [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+        arena = KvArena(gpu_ctx, MODEL_QWEN3, 1, 2, 400, Q4, page_size=64, pool_pages=14)
+        append = lambda seq, flags=0: arena.append(None, k, v, [0], [300], seq_ids=[seq], in_dtype=BF16, flags=flags)  # noqa: E731
+        gpu_ctx.set_stream(stream)
+        with torch.cuda.stream(stream), pytest.raises(KeyError):
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                append(1, DECODE_NO_ADVANCE)
+                append(1, DECODE_NO_ADVANCE)
+                raise KeyError
+        assert arena.page_stats(1)[0] == 5
+        if first == "read":
+            got = [torch.ones(300, hkv, d, device="cuda") for _ in range(2)]
+            stream.wait_stream(torch.cuda.default_stream())
+            arena.read_rows(*got, [0], [300], seq_ids=[1])
+            gpu_ctx.sync()
+            assert not got[0].any() and not got[1].any()  # rows that were never written
+        elif first == "decode":
+            arena.set_len(1, 300)
+            run_decode(gpu_ctx, arena, rng, [300], BF16, F32, ids=[1], check=False)
+            arena.set_len(1, 0)
+        if first == "capture":
+            with torch.cuda.stream(stream):
+                with torch.cuda.graph(graphs[-2], stream=stream):
+                    append(1)
+                graphs[-2].replay()
+        else:
+            append(1)
+        append(0)
+        gpu_ctx.sync()
+        gpu_ctx.set_stream(old)
+        want = ref.quantise(v.float().cpu().numpy())
+        rows = [stored(arena, seq, 0, 0, 300) for seq in range(2)]
+        for (kc, ks), (vc, vs) in rows:
+            assert np.array_equal(vc, want[0]) and np.array_equal(vs, want[1])
+        assert np.array_equal(rows[0][0][0], rows[1][0][0]) and arena.page_stats() == (10, 4)
+        torch.cuda.synchronize()
+        run_decode(gpu_ctx, arena, rng, [300, 300], BF16, F32)
+        arena.close()
