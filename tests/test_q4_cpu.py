@@ -252,3 +252,19 @@ def test_types_that_a_call_refuses_reach_it():
         arena.append(None, k, k, [0], [10], in_dtype=dt)
         arena.read_rows(k, k, [0], [10], out_dtype=dt)
     assert len(arena.lib.made) == 10
+
+
+def test_a_seventh_without_a_division():
+    """quantise8 makes top / 7 of a product with the rounded seventh and a correction by its
+    residual: the correctly rounded quotient for every mantissa. (64 bits hold the residual,
+    a few units of the quotient's last place, and the corrected sum exactly, so rounding
+    that sum once to 32 bits is what a fused multiply-add does.)"""
+    seventh = np.float32(1.0) / np.float32(7.0)
+    for begin in range(0, 1 << 23, 1 << 21):
+        top = (np.arange(begin, begin + (1 << 21), dtype=np.uint32) + np.uint32(0x3f800000)).view(np.float32)
+        guess = top * seventh
+        residual = top.astype(np.float64) - 7.0 * guess.astype(np.float64)
+        # 7 times: half a unit of a guess in [1/4, 2/7), 2^-26, and top times the seventh's own error, 2 * 2^-27
+        assert np.abs(residual).max() <= 7 * 2.0 ** -25
+        got = (residual * np.float64(seventh) + guess.astype(np.float64)).astype(np.float32)
+        assert np.array_equal(got, top / np.float32(7.0))
