@@ -25,12 +25,13 @@
 // item's first P V starts O afresh; its weights are written after the tile's
 // threads have read the last item's O.
 //
-// Measured: a Qwen3 prompt of 16384 tokens 1.56 to 1.60 ms (1375 to 1410 TFLOP/s of
-// the causal half; a library product of bf16 matrices reaches 1646 for a moment, 1373
-// for seconds), 11 ragged Qwen3 prompts of together 12345 tokens 160 to 165 us (1000 to
-// 1030), one of 2048 33 to 39 us, 3 Granite prompts of 8200 tokens 175 us (785), 7 of
-// 777 10 us. A step, both tiles against a key tile, takes 3100 cycles of which the
-// tensor pipe needs 2048: a tile's scores (512, and about 270 to hand them over), its
+// Measured, medians: a Qwen3 prompt of 16384 tokens 1.58 to 1.64 ms for a moment (1340
+// to 1390 TFLOP/s of the causal half; a library product of bf16 matrices reaches 1646
+// for a moment, 1373 for seconds), 1.85 ms call after call at the power cap; 11 ragged
+// Qwen3 prompts of together 12345 tokens 165 us (1000), one of 2048 34 to 35 us; 3
+// Granite prompts of 8200 tokens 176 to 180 us (765 to 780), 200 to 230 in replays
+// back to back, one of 4096 51 to 54 us (635 to 670), 7 of 777 9.3 us. A step,
+// both tiles against a key tile, takes 3100 cycles of which the tensor pipe needs 2048: a tile's scores (512, and about 270 to hand them over), its
 // row maxima (400), its exponentials (1400) and the products of their last half (256)
 // follow one another, and the other tile's do not fill all of the gaps. An item adds
 // about 3000 cycles for its outputs. Steps:
@@ -87,9 +88,10 @@ struct Packed {
   static constexpr float TAU = 8.0f;
   // Every POLY-th pair of exponentials is made on the FMA pipe (0: none). With 64
   // dims the special-function unit has as many exponentials a product as with 128 but
-  // half the time: none, every fourth, third, second pair take 202, 179, 171, 182 us
-  // for 3 Granite prompts of 8200 tokens; with 128 dims none, every fourth, third 1563,
-  // 1549, 1570 us for 16384 tokens and 160, 160, 161 for 11 ragged prompts.
+  // half the time: none, every fourth, every third pair take 187, 180, 178 us for 3
+  // Granite prompts of 8200 tokens, 450, 433, 434 for 10 of together 30000, 54.1, 52.8,
+  // 52.6 for one of 4096 (every second: 60 there); with 128 dims 1578, 1586, 1591 us for
+  // 16384 tokens and 162, 163, 165 for 11 ragged prompts.
   static constexpr int POLY = M::D == 64 ? 3 : 0;
   static constexpr float UNIT = M::SCALE * 1.4426950408889634f;  // base-2 logit of a score
   static_assert(SMEM <= 227 * 1024, "fits one SM");
@@ -110,7 +112,8 @@ __device__ __forceinline__ uint32_t pack_pair(float2 x) {
 // 2^x, x <= TAU, of a pair on the FMA pipe: x = n + f, n rounded by adding and
 // taking off 1.5 * 2^23, 2^f by a polynomial of degree 3 (fitted for the smallest
 // relative error on [-0.5, 0.5], 7.5e-5; a weight's rounding to fp16 is up to
-// 4.9e-4), 2^n through the exponent field. x below -126, -inf among them, gives 0:
+// 4.9e-4), 2^n through the exponent field. x below -126, -inf among them, gives 0 (so does
+// NaN, but a row with such a score has NaN for its reference):
 // the value at -126 is taken off, which no larger result notices.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   constexpr float C0 = 0.9999281167984009f, C1 = 0.6932609677314758f, C2 = 0.24261054396629333f, C3 = 0.05517132207751274f;

@@ -6,14 +6,15 @@
 // once. qx_q4_read_kernel expands rows into plain tensors.
 //
 // Measured: 32768 bf16 Qwen3 tokens (norm, rotation, 4-bit rows; 640 MB) written in
-// 131 us, 4.9 TB/s, 75% of a copy's rate; read back as bf16 in 18 us, 4.8 TB/s.
-// 9001 bf16 Granite tokens: 17.3 and 6.1 us; one token: 1.6 and 1.5 us. The writes
+// 133.5 us, 4.8 TB/s, 73% of a copy's rate; read back as bf16 in 18 us, 4.8 TB/s.
+// 9001 bf16 Granite tokens: 17.3 and 6.4 us; one token: 1.8 and 1.6 us. The writes
 // are bound by instructions and latency together: issue slots are busy 68% of the
-// time, DRAM 54%, with 32 warps an SM of which most wait for their loads. What
-// brought them there from 312 us: inputs of known types, all loaded before the
-// first is used; one lane layout for queries that needs no exchange for the
-// rotation; the table and the norm weights once a lane for all its heads; codes
-// without a division or a conversion.
+// time (Granite 70%), DRAM 53%, with 28 of 32 warps an SM active, most of which
+// wait for loads. What brought them there from 312 us: inputs of known types, all
+// loaded before the first is used; one lane layout for queries that needs no
+// exchange for the rotation; the table and the norm weights once a lane for all its
+// heads; codes without a division or a conversion. (The check for norms that pass
+// f32 is 2 us of the 133.5; by half warps or once for all heads it takes 3 or 4.)
 #include "q4.cuh"
 
 namespace qx {
@@ -22,7 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 
 // N neighbouring elements as loaded, f32 (WIDE) or two 16-bit ones to a word;
-// VEC: 16-byte aligned rows (the 32768 tokens above: 131 us, 158 where the tensors
+// VEC: 16-byte aligned rows (the 32768 tokens above: 133.5 us, 162 where the inputs
 // start at an odd element; read back 17 and 55). Types that the compiler knows, so that no load waits
 // for another's branch.
 template <int N, bool WIDE, bool VEC>

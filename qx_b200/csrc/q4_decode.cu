@@ -35,12 +35,16 @@
 //
 // Measured (the rows' bytes at a copy's 6.5 TB/s in brackets): 48 ragged Qwen3
 // sequences of up to 8190 rows, 2 layers, 68.7 us (38.5); 128 ragged Granite ones of
-// up to 4096, 4 layers, 120.5 us (91.9); one Qwen3 layer of 32768 rows 14.1 us (2.9);
-// 24 Granite layers of 4064 rows, f32 in and out, 24.4 us (8.6); one of 512 rows 8.1
-// us. Bound by instructions: with every row in L2 the two batches take 64 and 110
-// us, the stream of rows without the work 50 and 100 (tensor pipe 22% busy, an
-// instruction issued in 54% of the cycles); single sequences by the chain of three
-// launches and the joining of the parts. Steps: f16 products only 117 and 225 us,
+// up to 4096, 4 layers, 121 us (91.9); one Qwen3 layer of 32768 rows 14.1 us (2.9);
+// 24 Granite layers of 4064 rows, f32 in and out, 24.6 us (8.6); one of 512 rows 8.3
+// us. The batches are bound by latency at 16 warps an SM: an instruction issues in
+// 55% of the cycles, the tensor pipe is busy 23% (Granite 30%), DRAM 46% (60%), and
+// a warp's stalls are spread over loads, fixed latencies and full pipes: each walks
+// one chain of wait, products, scaling, maximum, exponentials, products. With every
+// row in L2 they still take 64 and 110 us, the stream of rows without the work 50
+// and 100. In f32 a row takes twice the products (the 24 layers: tensor pipe 29%,
+// issue 40%). Single sequences are bound by the chain of three launches and the
+// joining of the parts. Steps: f16 products only 117 and 225 us,
 // integer scores 102 and 169, masks of one instruction 98 and 156, a grid of their
 // own for queries and new rows 92 and 145, one line of tiles 69 and 120.
 //
