@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 3 : 4) qx_q4_append_kernel(co
         float inv = rsqrtf(fmaf(sum, 1.0f / M::D, 1.0e-6f));
         if (__any_sync(0xffffffffu, !isfinite(sum))) {  // elements beyond 1.6e18 may pass f32 in their squares
           const float x8[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-          inv = exact_inv_rms<M>(x8);
+          const float exact = exact_inv_rms<M>(x8);
+          if (!isfinite(sum)) inv = exact;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(__fmul2_rn(v[e], make_float2(inv, inv)), w[e]);

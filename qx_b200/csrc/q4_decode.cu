@@ -209,7 +209,10 @@ __device__ __forceinline__ bool load_query(const Q4DecodeParams& p, long long fi
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     float inv = __frcp_rn(__fsqrt_rn(fmaf(sum, 1.0f / M::D, 1.0e-6f)));
-    if (__any_sync(0xffffffffu, !isfinite(sum))) inv = exact_inv_rms<M, NG * 8, 4>(x);
+    if (__any_sync(0xffffffffu, !isfinite(sum))) {
+      const float exact = exact_inv_rms<M, NG * 8, 4>(x);
+      if (!isfinite(sum)) inv = exact;
+    }
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll

@@ -954,3 +954,23 @@ def test_pages_mapped_by_a_capture_that_is_thrown_away(gpu_ctx):
         torch.cuda.synchronize()
         run_decode(gpu_ctx, arena, rng, [300, 300], BF16, F32)
         arena.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_head_is_normed_alike_whatever_the_others_hold(gpu_ctx, dtype):
+    """Heads whose squares pass f32 are normed another way; the heads beside them are not."""
+    rng = np.random.default_rng([dtype, 42])
+    q, k, v = (tensor(rng, (64, 1, h, 128), dtype) for h in (32, 4, 4))
+    big = q.clone()
+    big[:, :, ::3] *= 1e25
+    rest = [h for h in range(32) if h % 3]
+    got = []
+    for x in (q, big):
+        arena = make_arena(gpu_ctx, MODEL_QWEN3, [65])
+        rot, turned, out = (torch.zeros(n, 1, 32, 128, device="cuda") for n in (64, 1, 1))
+        arena.append(x, k, v, [0], [64], in_dtype=dtype, q_rot=rot, rot_dtype=F32)
+        arena.decode(x[:1], k[:1], v[:1], out, [64], q_dtype=dtype, in_dtype=dtype, q_rot_out=turned)
+        gpu_ctx.sync()
+        got.append([y[:, :, rest] for y in (rot, turned, out)])
+        arena.close()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
