@@ -457,8 +457,8 @@ class KvArena:
     def write(self, seq: int, layer: int, begin: int, keys: np.ndarray | None, values: np.ndarray | None):
         count = (keys if keys is not None else values).shape[0]
         if self.key_dtype == Q4:
-            for rows in (keys, values):
-                if rows is not None and (rows.dtype != np.uint8 or rows.shape != (count, *self.row_shape)):
+            for rows in (np.asarray(x) for x in (keys, values) if x is not None):
+                if rows.dtype != np.uint8 or rows.shape != (count, *self.row_shape):
                     raise QxError(_lib.ERR_INVALID_ARG, f"a 4-bit arena takes raw rows: uint8 {(count, *self.row_shape)}, "
                                                         f"not {rows.dtype} {rows.shape}")
         if keys is not None:

@@ -238,7 +238,8 @@ def test_raw_rows_written_to_a_4bit_arena():
         refused(arena.lib, lambda: arena.write(0, 0, 0, k, v))
     arena.write(0, 0, 0, raw, None)
     arena.write(0, 0, 0, np.zeros((6, 288), np.uint8)[::2], raw)
-    assert arena.lib.made == ["qxc_kv_write"] * 2
+    arena.write(0, 0, 0, torch.zeros(3, 288, dtype=torch.uint8), None)
+    assert arena.lib.made == ["qxc_kv_write"] * 3
 
 
 def test_types_that_a_call_refuses_reach_it():
