@@ -171,10 +171,10 @@ qxc_status qxc_kv_write(qxc_kv* kv, int32_t seq, int32_t layer, int32_t begin, i
  * overflows) and rotation of q and k at positions positions[i],
  * positions[i] + 1, ..., keys and values quantised into the cache. positions[i]
  * must equal the sequence's length, positions[i] + counts[i] <= capacity, else
- * QXC_ERR_POSITION; counts may be 0, a sequence may appear once. Lengths
- * advance by counts unless QXC_DECODE_NO_ADVANCE. Device pointers of any
- * element alignment (16-byte aligned ones are read and written faster);
- * asynchronous. q and q_rot may both be NULL (keys and values only), k_rot may
+ * QXC_ERR_POSITION; counts may be 0, a sequence may appear once; fewer than 2^27
+ * tokens x layers a call. Lengths advance by counts unless
+ * QXC_DECODE_NO_ADVANCE. Device pointers of any element alignment (16-byte
+ * aligned ones are read and written faster); asynchronous. q and q_rot may both be NULL (keys and values only), k_rot may
  * be NULL. q_rot may be q itself, and k_rot k, where type and layout are the
  * same; an output that overlaps anything else of the call is refused
  * (QXC_ERR_INVALID_ARG). */
@@ -204,8 +204,9 @@ qxc_status qxc_kv_append(qxc_ctx* ctx, qxc_kv* kv, const qxc_append_args* args);
 /* Rows [begins[i], begins[i] + counts[i]) of each of seq_count sequences
  * (packed one after another) of a 4-bit arena as plain values, rounded once to
  * out_dtype. The rows may lie past the sequence's length but not past its
- * capacity (QXC_ERR_POSITION) or its mapped pages. A sequence may appear more
- * than once. Either output may be NULL. Device pointers, asynchronous. */
+ * capacity (QXC_ERR_POSITION) or its mapped pages, fewer than 2^27 rows x
+ * layers a call. A sequence may appear more than once. Either output may be
+ * NULL. Device pointers, asynchronous. */
 typedef struct qxc_read_rows_args {
   int32_t layer_begin;
   int32_t layer_count;

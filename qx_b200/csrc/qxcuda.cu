@@ -884,14 +884,18 @@ qxc_status send_entries(qxc_ctx* ctx, qxc_kv* kv, const std::vector<int>& fresh)
     for (int e : kv->unsent)
       if (kv->table[e] >= 0) idx.push_back(e);  // not released since
   for (int e : idx) val.push_back(kv->table[e]);
-  if (capturing) {
+  const qxc_status st = push_table(ctx, kv, idx, val);
+  if (st != QXC_OK) {  // the pages stay mapped, so a later call has to send them
+    kv->unsent.insert(kv->unsent.end(), fresh.begin(), fresh.end());
+    kv->unsent_by = 0;
+  } else if (!capturing) {
+    kv->unsent.clear();
+  } else {
     if (id != kv->unsent_by) kv->unsent.clear();
     kv->unsent.insert(kv->unsent.end(), idx.begin(), idx.end());
     kv->unsent_by = id;
-  } else {
-    kv->unsent.clear();
   }
-  return push_table(ctx, kv, idx, val);
+  return st;
 }
 
 // Map pages so that rows [0, rows[i]) of sequence seqs[i] exist, all or
