@@ -974,3 +974,63 @@ def test_a_head_is_normed_alike_whatever_the_others_hold(gpu_ctx, dtype):
         got.append([y[:, :, rest] for y in (rot, turned, out)])
         arena.close()
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("page", [0, 64])
+def test_a_step_writes_the_rows_that_an_append_writes(gpu_ctx, model, dtype, page):
+    """Raw rows of keys and values, bit for bit, and the same outputs and rows from inputs
+    that start one element past a 16-byte boundary."""
+    rng = np.random.default_rng([model, dtype, page, 43])
+    hq, hkv, d = model_shape(model)
+    qw, kw = norms(rng, model)
+    rows = [0, 1, 63, 64, 200]
+    arenas = [make_arena(gpu_ctx, model, [n + 1 for n in rows], layers=2, page=page) for _ in range(3)]
+    q, k, v = (tensor(rng, (5, 2, h, d), dtype, 2.0) for h in (hq, hkv, hkv))
+    old = [tensor(rng, (sum(rows), 2, hkv, d), dtype) for _ in range(2)]
+    for a in arenas:
+        a.append(None, *old, [0] * 5, rows, in_dtype=dtype, k_norm=kw)
+    shifted = []
+    for x in (q, k, v):
+        flat = torch.zeros(x.numel() + 1, device="cuda", dtype=x.dtype)[1:]
+        shifted.append(flat.copy_(x.flatten()).view(x.shape))
+    outs = [torch.zeros(5, 2, hq, d, device="cuda") for _ in range(2)]
+    for a, ins, out in zip(arenas, ((q, k, v), shifted), outs):
+        a.decode(*ins, out, rows, q_dtype=dtype, in_dtype=dtype, q_norm=qw, k_norm=kw)
+    arenas[2].append(None, k, v, rows, [1] * 5, in_dtype=dtype, k_norm=kw)
+    gpu_ctx.sync()
+    assert torch.equal(*outs)
+    for i, n in enumerate(rows):
+        for l in range(2):
+            raw = [a.read(i, l, 0, n + 1) for a in arenas]
+            for other in raw[1:]:
+                assert all(np.array_equal(x, y) for x, y in zip(raw[0], other))
+    for a in arenas:
+        a.close()
+
+
+@pytest.mark.parametrize("model,capacity", [(MODEL_GRANITE, 4096), (MODEL_QWEN3, 40960)])
+def test_a_prompt_that_fills_its_sequence(gpu_ctx, model, capacity):
+    """The longest positions of a model: written by a prefill, read back, and then full."""
+    rng = np.random.default_rng([model, 44])
+    hq, hkv, d = model_shape(model)
+    arena = KvArena(gpu_ctx, model, 1, 1, capacity, Q4)
+    q, k, v = (tensor(rng, (capacity, h, d), BF16) for h in (hq, hkv, hkv))
+    out = torch.zeros(capacity, hq, d, device="cuda", dtype=torch.bfloat16)
+    arena.prefill_packed(q, k, v, out, [capacity])
+    keys, values = (torch.zeros(2, hkv, d, device="cuda") for _ in range(2))
+    arena.read_rows(keys, values, [capacity - 2], [2])
+    gpu_ctx.sync()
+    assert arena.len(0) == capacity and torch.isfinite(out).all()
+    want = ref.quantise(keys32(gpu_ctx, model, k[-2:], capacity - 2, None))
+    assert np.array_equal(host(keys), ref.values(*want))
+    want = ref.quantise(v[-2:].float().cpu().numpy())
+    assert np.array_equal(host(values), ref.values(*want))
+    one = [x[:1, None] for x in (q, k, v)]
+    for call in (lambda: arena.decode(*one, out[:1], [capacity], q_dtype=BF16, in_dtype=BF16, out_dtype=BF16),
+                 lambda: arena.append(None, *one[1:], [capacity], [1], in_dtype=BF16)):
+        with pytest.raises(QxError) as e:
+            call()
+        assert e.value.status == _lib.ERR_POSITION
+    arena.close()
