@@ -534,7 +534,7 @@ def test_a_workspace_grows_to_what_is_asked_where_more_does_not_fit():
     try:
         go(440)
         ctx.sync()
-        assert torch.cuda.mem_get_info()[0] < 2 * 440 * 256 * 3072
+        assert torch.cuda.mem_get_info()[0] < 2 * 440 * 256 * 2 * (1024 + 512)
         go(500)
         ctx.sync()
     finally:
